@@ -231,6 +231,26 @@ int swvr_rmsnorm_bwd(int64_t n_rows, int64_t hidden, const void* grad_h, int32_t
                      size_t workspace_bytes, void* stream);
 
 /*
+ * Embedding lookup with scaling, and its gradient by token (no counterpart in the reference).
+ *   out[n, :] = scale * E[tokens[n], :]                       E [vocab, dim], rows lde apart
+ *   grad_E[v, :] = scale * sum_{n: tokens[n] = v} grad_out[n, :],  grad_E[padding_idx, :] = 0
+ * tokens are [n_tokens] integers of token_bits (32 or 64), contiguous; out is contiguous in E's
+ * dtype; grad_out, grad_E and E share `dtype`.  Products and sums run in fp32 (fp64 for F64) and
+ * are rounded once; the sums follow the tokens' order and use no atomics, so the
+ * gradient is deterministic.  Every row of grad_E is written.  padding_idx < 0: none.
+ * A token outside [0, vocab) reads nothing: its row of out is NaN, grad_E leaves it out, and
+ * swvr_device_error() reports a code of SWVR_TOKEN_CODE.
+ */
+#define SWVR_TOKEN_CODE 0x400u
+
+int swvr_embed_fwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tokens, int32_t token_bits, const void* E,
+                   int32_t dtype, int64_t lde, double scale, void* out, void* stream);
+int swvr_embed_bwd_workspace_size(int64_t n_tokens, int64_t vocab, int64_t dim, int32_t dtype, size_t* bytes);
+int swvr_embed_bwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tokens, int32_t token_bits,
+                   const void* grad_out, int64_t ld_grad_out, double scale, int64_t padding_idx, void* grad_E,
+                   int32_t dtype, int64_t ld_grad_E, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Launch accounting for benchmarks (no counterpart in the reference).  Between
  * swvr_profile_start() and swvr_profile_stop(), every kernel the library launches from any
  * host thread is counted per kind and bracketed by a pair of CUDA events on its stream.
@@ -251,7 +271,8 @@ const char* swvr_last_error(void);
 
 /*
  * Read and clear the device error word of the current device: *code = 0 when no bounded
- * device-side wait has expired since the last call.  Synchronises with the device.
+ * device-side wait has expired, and no kernel has met a token out of range
+ * (*code & ~0xff == SWVR_TOKEN_CODE), since the last call.  Synchronises with the device.
  */
 int swvr_device_error(uint32_t* code);
 

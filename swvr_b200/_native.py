@@ -23,6 +23,7 @@ F32, F64, BF16, F16 = 0, 1, 2, 3
 REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
 MSE_STATS_LEN = 514  # SWVR_MSE_STATS_LEN
 SELFTEST_CODE = 0x7F01  # SWVR_SELFTEST_CODE
+TOKEN_CODE = 0x400  # SWVR_TOKEN_CODE
 
 DTYPE_CODE = {torch.float32: F32, torch.float64: F64, torch.bfloat16: BF16, torch.float16: F16}
 
@@ -79,6 +80,11 @@ _SIGNATURES = {
     "swvr_rmsnorm_bwd_workspace_size": (c_int, [c_int64, c_int64, c_int32, c_int32, POINTER(c_size_t)]),
     "swvr_rmsnorm_bwd": (c_int, [c_int64, c_int64, c_void_p, c_int32, c_void_p, c_int32, c_int64, c_void_p, c_int32,
                                  c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
+    "swvr_embed_fwd": (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int32, c_void_p, c_int32, c_int64, c_double,
+                               c_void_p, c_void_p]),
+    "swvr_embed_bwd_workspace_size": (c_int, [c_int64, c_int64, c_int64, c_int32, POINTER(c_size_t)]),
+    "swvr_embed_bwd": (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int32, c_void_p, c_int64, c_double, c_int64,
+                               c_void_p, c_int32, c_int64, c_void_p, c_size_t, c_void_p]),
     "swvr_profile_start": (c_int, []),
     "swvr_profile_stop": (c_int, [POINTER(ProfileRecord), c_int, POINTER(c_int)]),
 }
@@ -124,9 +130,12 @@ def check(rc: int, what: str) -> None:
 
 
 def check_device_error() -> None:
-    """Raise if a bounded device-side wait expired since the last check (synchronises)."""
+    """Raise if a bounded device-side wait expired, or a kernel met a token out of range, since the
+    last check (synchronises)."""
     code = c_uint32(0)
     check(lib().swvr_device_error(ctypes.byref(code)), "swvr_device_error")
+    if code.value & ~0xFF == TOKEN_CODE:
+        raise RuntimeError(f"a token or teacher id was outside [0, V) (device error site 0x{code.value:x})")
     if code.value:
         raise RuntimeError(f"swvr_b200 kernel gave up waiting (device error site 0x{code.value:x})")
 

@@ -15,12 +15,14 @@ constexpr int kNumSMsB200 = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Device error codes written to g_device_error by bounded waits (0 = none).
+// Device error codes written to g_device_error by bounded waits, and by kernels that met an
+// index out of range and left it out (0 = none).
 // The low byte names the kernel, the next byte the wait site.
 enum : uint32_t {
   kErrFwd = 0x100,
   kErrBwdScores = 0x200,
   kErrGemm = 0x300,
+  kErrToken = 0x400,       // a token or teacher id outside [0, V)
   kErrSelftest = 0x7F00,  // swvr_selftest_wait_timeout
 };
 
