@@ -72,8 +72,8 @@ def _operand(x: torch.Tensor, cdt: torch.dtype, pad_cols: int = 0) -> torch.Tens
     path also a 16-byte aligned base and row pitch, padding the row pitch with zeros."""
     if x.dtype != cdt:
         x = x.to(cdt)
-    if x.dim() == 2 and x.shape[1] > 0 and x.stride(1) != 1:
-        x = x.contiguous()
+    if x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()  # also a broadcast or overlapping row, whose pitch the library would take for K
     if not _tensor_core(cdt):
         return x
     rows, cols = x.shape
