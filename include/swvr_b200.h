@@ -251,6 +251,70 @@ int swvr_embed_bwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tok
                    int32_t dtype, int64_t ld_grad_E, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Distillation of the head from a teacher's top logits (no counterpart in the reference).
+ *   z = (logit_scale * h W^T + bias) / T,  p = softmax(z) over the vocabulary,  lse = logsumexp(z)
+ *   q_k = exp(t_k / T - L),  L = logsumexp_k(t_k / T), or teacher_lse[n] where it is given
+ *   each_n = T^2 * sum_k q_k (log q_k - z[id_k] + lse_n)
+ *   out = w_n each_n (NONE, [N]), their sum (SUM), or sum / (sum(w) or N) (MEAN)
+ * over the `teacher` entries (id_k, t_k) of each token; an id may occur more than once.
+ * An entry with a negative id or a logit of -inf is left out; a token with none left has loss
+ * 0 and no gradient.  A zero weight drops its token whatever its loss.  An id >= vocab (with a
+ * logit above -inf) makes its token's loss and gradient NaN and sets SWVR_TOKEN_CODE.
+ *
+ * teacher_ids [N, teacher] (id_bits 32 or 64) and teacher_logits [N, teacher] (any dtype) are
+ * contiguous; teacher_lse and weight ([N] or NULL), out, lse, qsum, each [N], slogq and z
+ * [N, teacher] and stats [2] are in the accumulation dtype, sid [N, teacher] in int32.  sid, slogq,
+ * z, lse, qsum, each and stats are written by the forward and read by the backward: the
+ * caller keeps them, and h, W, bias, weight and the sizes unchanged, in between.  W and h as in
+ * swvr_problem.  At most 1024 teacher entries.  [N, vocab] is never materialised on the
+ * tensor-core path; the fp32 / fp64 path stages `chunk` vocabulary rows of it.
+ */
+typedef struct swvr_distill {
+  int64_t n_tokens, hidden, vocab, teacher;
+  int32_t compute_dtype, bias_dtype, teacher_dtype, id_bits;
+  const void* h;
+  int64_t ldh;
+  const void* W;
+  int64_t ldw;
+  const void* bias;           /* [vocab] contiguous, or NULL */
+  double logit_scale, temperature;
+  int64_t chunk;
+  const void* teacher_ids;
+  const void* teacher_logits;
+  const void* teacher_lse;    /* or NULL */
+  const void* weight;         /* or NULL */
+  int32_t reduction;
+  int32_t* sid;
+  void* slogq;
+  void* z;
+  void* lse;
+  void* qsum;
+  void* each;
+  void* stats;                /* SUM / MEAN */
+} swvr_distill;
+
+/* NULL gradients are not computed.  grad_out is [1] (SUM / MEAN) or [N], in the accumulation
+ * dtype, as is grad_weight [N]; grad_h [N, hidden] is contiguous; on the tensor-core path grad_W is in
+ * the compute dtype or fp32.  dW, db and dh are deterministic. */
+typedef struct swvr_distill_grads {
+  const void* grad_out;
+  void* grad_h;
+  int32_t grad_h_dtype;
+  void* grad_W;
+  int32_t grad_W_dtype;
+  int64_t ld_grad_W;
+  void* grad_bias;
+  int32_t grad_bias_dtype;
+  void* grad_weight;
+} swvr_distill_grads;
+
+int swvr_distill_fwd_workspace_size(const swvr_distill* p, size_t* bytes);
+int swvr_distill_fwd(const swvr_distill* p, void* out, void* workspace, size_t workspace_bytes, void* stream);
+int swvr_distill_bwd_workspace_size(const swvr_distill* p, const swvr_distill_grads* g, size_t* bytes);
+int swvr_distill_bwd(const swvr_distill* p, const swvr_distill_grads* g, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/*
  * Launch accounting for benchmarks (no counterpart in the reference).  Between
  * swvr_profile_start() and swvr_profile_stop(), every kernel the library launches from any
  * host thread is counted per kind and bracketed by a pair of CUDA events on its stream.

@@ -6,8 +6,9 @@ repository's B200 implementation in ``swvr_b200`` (which adds the fused-norm ent
 ``rmsnorm_softmax_readout`` and ``rmsnorm_softmax_readout_mse``); the objects are the same, so
 ``swvr.softmax_readout is swvr_b200.softmax_readout``.
 """
-from swvr_b200 import (SoftmaxReadoutMSE, __version__, embedding_lookup, rmsnorm_softmax_readout,
-                       rmsnorm_softmax_readout_mse, softmax_readout, softmax_readout_mse, softmax_readout_reference)
+from swvr_b200 import (SoftmaxDistill, SoftmaxReadoutMSE, __version__, embedding_lookup, rmsnorm_softmax_readout,
+                       rmsnorm_softmax_readout_mse, softmax_distill, softmax_readout, softmax_readout_mse,
+                       softmax_readout_reference)
 
 __all__ = ["softmax_readout", "softmax_readout_mse", "SoftmaxReadoutMSE", "softmax_readout_reference",
            "rmsnorm_softmax_readout", "rmsnorm_softmax_readout_mse"]

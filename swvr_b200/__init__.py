@@ -4,11 +4,12 @@ A drop-in for pengzhangzhi/swvr (``import swvr_b200 as swvr``) whose compute run
 hand-written sm_100a kernels (libswvr_b200.so, C ABI in include/swvr_b200.h).
 """
 from .api import SoftmaxReadoutMSE, softmax_readout, softmax_readout_mse
+from .distill import SoftmaxDistill, softmax_distill
 from .embedding import embedding_lookup
 from .norm import rmsnorm_softmax_readout, rmsnorm_softmax_readout_mse
 from .reference import softmax_readout_reference
 
-# The readout's own names; the operators on tokens beside it (embedding_lookup) are reached as
+# The readout's own names; the operators on tokens beside it (embedding_lookup, softmax_distill) are reached as
 # attributes of the package.
 __all__ = ["softmax_readout", "softmax_readout_mse", "SoftmaxReadoutMSE", "softmax_readout_reference",
            "rmsnorm_softmax_readout", "rmsnorm_softmax_readout_mse"]

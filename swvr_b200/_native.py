@@ -52,6 +52,32 @@ class Grads(ctypes.Structure):
     ]
 
 
+class Distill(ctypes.Structure):
+    _fields_ = [
+        ("n_tokens", c_int64), ("hidden", c_int64), ("vocab", c_int64), ("teacher", c_int64),
+        ("compute_dtype", c_int32), ("bias_dtype", c_int32), ("teacher_dtype", c_int32), ("id_bits", c_int32),
+        ("h", c_void_p), ("ldh", c_int64),
+        ("W", c_void_p), ("ldw", c_int64),
+        ("bias", c_void_p),
+        ("logit_scale", c_double), ("temperature", c_double),
+        ("chunk", c_int64),
+        ("teacher_ids", c_void_p), ("teacher_logits", c_void_p), ("teacher_lse", c_void_p), ("weight", c_void_p),
+        ("reduction", c_int32),
+        ("sid", c_void_p), ("slogq", c_void_p), ("z", c_void_p), ("lse", c_void_p), ("qsum", c_void_p),
+        ("each", c_void_p), ("stats", c_void_p),
+    ]
+
+
+class DistillGrads(ctypes.Structure):
+    _fields_ = [
+        ("grad_out", c_void_p),
+        ("grad_h", c_void_p), ("grad_h_dtype", c_int32),
+        ("grad_W", c_void_p), ("grad_W_dtype", c_int32), ("ld_grad_W", c_int64),
+        ("grad_bias", c_void_p), ("grad_bias_dtype", c_int32),
+        ("grad_weight", c_void_p),
+    ]
+
+
 class ProfileRecord(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 32), ("launches", c_int64), ("total_ms", c_double)]
 
@@ -85,6 +111,10 @@ _SIGNATURES = {
     "swvr_embed_bwd_workspace_size": (c_int, [c_int64, c_int64, c_int64, c_int32, POINTER(c_size_t)]),
     "swvr_embed_bwd": (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int32, c_void_p, c_int64, c_double, c_int64,
                                c_void_p, c_int32, c_int64, c_void_p, c_size_t, c_void_p]),
+    "swvr_distill_fwd_workspace_size": (c_int, [POINTER(Distill), POINTER(c_size_t)]),
+    "swvr_distill_fwd": (c_int, [POINTER(Distill), c_void_p, c_void_p, c_size_t, c_void_p]),
+    "swvr_distill_bwd_workspace_size": (c_int, [POINTER(Distill), POINTER(DistillGrads), POINTER(c_size_t)]),
+    "swvr_distill_bwd": (c_int, [POINTER(Distill), POINTER(DistillGrads), c_void_p, c_size_t, c_void_p]),
     "swvr_profile_start": (c_int, []),
     "swvr_profile_stop": (c_int, [POINTER(ProfileRecord), c_int, POINTER(c_int)]),
 }

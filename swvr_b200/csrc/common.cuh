@@ -22,6 +22,7 @@ enum : uint32_t {
   kErrFwd = 0x100,
   kErrBwdScores = 0x200,
   kErrGemm = 0x300,
+  kErrHead = 0x500,
   kErrToken = 0x400,       // a token or teacher id outside [0, V)
   kErrSelftest = 0x7F00,  // swvr_selftest_wait_timeout
 };

@@ -116,6 +116,7 @@ struct GemmParams {
   int dh_mt, dh_nt, dh_kb;   // dh: row tiles (tokens / 256), column tiles, k-blocks (chunk rows / 64)
   int v_begin;               // first vocabulary row of the chunk
   int gw_f32;                // dW output is fp32 (else the 16-bit compute dtype)
+  const float* gw_scale;     // dW is multiplied by this device value before it is stored; null: stored as it is
 };
 
 struct GemmMaps {

@@ -78,7 +78,7 @@ __device__ __forceinline__ void stage_row(uint8_t* stg, int r, const uint32_t (&
   }
 }
 
-template <bool kBF16, int NS>
+template <bool kBF16, int NS, bool kScaled>
 __global__ void __launch_bounds__(256, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tm_ds_k, const __grid_constant__ CUtensorMap tm_ds_mn,
                 const __grid_constant__ CUtensorMap tm_h_mn, const __grid_constant__ CUtensorMap tm_w_mn,
@@ -212,6 +212,11 @@ __global__ void __launch_bounds__(256, 1)
     const bool ep_leader = (r == 0);
     const uint32_t trow = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     uint32_t tc = 0, sl = 0;
+    float gw_scale = 1.f;
+    if constexpr (kScaled) {
+      pdl_wait();  // the factor comes from a kernel before this one
+      gw_scale = *p.gw_scale;
+    }
     for (int t = pair; t < ntiles; t += npairs, ++tc) {
       const TileInfo ti = decode_tile(p, t);
       const uint32_t ab = tc & 1u;
@@ -229,6 +234,13 @@ __global__ void __launch_bounds__(256, 1)
           tmem_ld32(acol + s * 64, x0);
           tmem_ld32(acol + s * 64 + 32, x1);
           tmem_wait_ld();
+          if constexpr (kScaled) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              x0[i] = __float_as_uint(__uint_as_float(x0[i]) * gw_scale);
+              x1[i] = __float_as_uint(__uint_as_float(x1[i]) * gw_scale);
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             v[i] = pack2<kBF16>(__uint_as_float(x0[2 * i]), __uint_as_float(x0[2 * i + 1]));
@@ -237,6 +249,12 @@ __global__ void __launch_bounds__(256, 1)
         } else {
           tmem_ld32(acol + s * 32, v);
           tmem_wait_ld();
+          if constexpr (kScaled) {
+            if (ti.dw) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * gw_scale);
+            }
+          }
         }
         uint8_t* stg = smem + Cfg::SMEM_STG + (sl & 1u) * Cfg::STG_BYTES;
         if (ep_leader) tma_store_wait_read<1>();  // the store issued from this slab two steps ago has read it
@@ -270,10 +288,10 @@ done:
   }
 }
 
-template <bool kBF16, int NS>
+template <bool kBF16, int NS, bool kScaled>
 static cudaError_t launch(const GemmMaps& m, const GemmParams& prm, int max_pairs, bool pdl, cudaStream_t st) {
   using Cfg = GemmCfg<NS>;
-  auto kern = gemm_kernel<kBF16, NS>;
+  auto kern = gemm_kernel<kBF16, NS, kScaled>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_ALLOC);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -311,7 +329,10 @@ static cudaError_t launch(const GemmMaps& m, const GemmParams& prm, int max_pair
 
 cudaError_t launch_gemm_kernel(bool bf16, const GemmMaps& maps, const GemmParams& prm, int max_pairs, bool pdl,
                                cudaStream_t st) {
-  return bf16 ? launch<true, 3>(maps, prm, max_pairs, pdl, st) : launch<false, 3>(maps, prm, max_pairs, pdl, st);
+  if (prm.gw_scale)  // fp16 only: its callers scale dS into fp16's range
+    return bf16 ? cudaErrorInvalidValue : launch<false, 3, true>(maps, prm, max_pairs, pdl, st);
+  return bf16 ? launch<true, 3, false>(maps, prm, max_pairs, pdl, st)
+              : launch<false, 3, false>(maps, prm, max_pairs, pdl, st);
 }
 
 }  // namespace tc
