@@ -315,6 +315,46 @@ int swvr_distill_bwd(const swvr_distill* p, const swvr_distill_grads* g, void* w
                      void* stream);
 
 /*
+ * Sampling of one token per row (no counterpart in the reference), from given logits, or from the
+ * head's scores x = logit_scale * h W^T + bias.  With T > 0 and w_i = exp((x_i - max x) / T), tokens ordered by
+ * falling x (equal ones by rising index): top_k keeps the first k, top_p a token while the weight
+ * ahead of it is below top_p times what top_k left, min_p a token with w_i >= min_p.  The result is the
+ * first token in index order whose running kept weight exceeds u times the kept total.  T = 0: the
+ * largest score, the lowest index among equals.  Weights and sums are 64-bit fixed point (2^-44 of the
+ * largest weight, 2^-(62 - log2 V) where V is past 2^18): the result does not depend on a summation order.
+ *
+ * temperature, top_k (0: off), top_p (1: off) and min_p (0: off) hold for all rows, or arrays of
+ * [N] give each row its own (any float dtype; top_ks 32- or 64-bit integers).  Array values out
+ * of range mean: T <= 0 or NaN the largest score, top_k <= 0 off, top_p >= 1 or NaN off, top_p <= 0 the
+ * first token alone, min_p <= 0 or NaN off, min_p > 1 as 1; u is taken into [0, 1], NaN as 0, and u = 1 gives the last
+ * kept token.  Scores of -inf and NaN are never chosen; a row with nothing else gives token -1.
+ * logprobs, where not NULL, receives log softmax(x / T) of the token over the whole row (T = 1 for a
+ * row of the largest score).
+ *
+ * swvr_sample takes h, W, bias, logit_scale and sizes from the problem (E, embed_dim and chunk are
+ * ignored) in bf16, fp16 or fp32; its workspace holds the fp32 scores of as many rows as 256 MiB take.
+ */
+typedef struct swvr_sampling {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const void* temperatures;
+  const void* top_ps;
+  const void* min_ps;
+  const void* top_ks;
+  int32_t temperatures_dtype, top_ps_dtype, min_ps_dtype, top_ks_bits;
+  const void* u;
+  int32_t u_dtype;
+  int64_t* tokens;
+  float* logprobs;
+} swvr_sampling;
+
+int swvr_sample_logits(int64_t n_rows, int64_t vocab, const void* logits, int32_t dtype, int64_t ld,
+                       const swvr_sampling* sampling, void* stream);
+int swvr_sample_workspace_size(const swvr_problem* p, size_t* bytes);
+int swvr_sample(const swvr_problem* p, const swvr_sampling* sampling, void* workspace, size_t workspace_bytes,
+                void* stream);
+
+/*
  * Launch accounting for benchmarks (no counterpart in the reference).  Between
  * swvr_profile_start() and swvr_profile_stop(), every kernel the library launches from any
  * host thread is counted per kind and bracketed by a pair of CUDA events on its stream.

@@ -7,8 +7,8 @@ repository's B200 implementation in ``swvr_b200`` (which adds the fused-norm ent
 ``swvr.softmax_readout is swvr_b200.softmax_readout``.
 """
 from swvr_b200 import (SoftmaxDistill, SoftmaxReadoutMSE, __version__, embedding_lookup, rmsnorm_softmax_readout,
-                       rmsnorm_softmax_readout_mse, softmax_distill, softmax_readout, softmax_readout_mse,
-                       softmax_readout_reference)
+                       rmsnorm_softmax_readout_mse, sample_logits, softmax_distill, softmax_readout,
+                       softmax_readout_mse, softmax_readout_reference, softmax_sample)
 
 __all__ = ["softmax_readout", "softmax_readout_mse", "SoftmaxReadoutMSE", "softmax_readout_reference",
            "rmsnorm_softmax_readout", "rmsnorm_softmax_readout_mse"]

@@ -78,6 +78,16 @@ class DistillGrads(ctypes.Structure):
     ]
 
 
+class Sampling(ctypes.Structure):
+    _fields_ = [
+        ("temperature", c_double), ("top_p", c_double), ("min_p", c_double), ("top_k", c_int64),
+        ("temperatures", c_void_p), ("top_ps", c_void_p), ("min_ps", c_void_p), ("top_ks", c_void_p),
+        ("temperatures_dtype", c_int32), ("top_ps_dtype", c_int32), ("min_ps_dtype", c_int32), ("top_ks_bits", c_int32),
+        ("u", c_void_p), ("u_dtype", c_int32),
+        ("tokens", c_void_p), ("logprobs", c_void_p),
+    ]
+
+
 class ProfileRecord(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 32), ("launches", c_int64), ("total_ms", c_double)]
 
@@ -115,6 +125,9 @@ _SIGNATURES = {
     "swvr_distill_fwd": (c_int, [POINTER(Distill), c_void_p, c_void_p, c_size_t, c_void_p]),
     "swvr_distill_bwd_workspace_size": (c_int, [POINTER(Distill), POINTER(DistillGrads), POINTER(c_size_t)]),
     "swvr_distill_bwd": (c_int, [POINTER(Distill), POINTER(DistillGrads), c_void_p, c_size_t, c_void_p]),
+    "swvr_sample_logits": (c_int, [c_int64, c_int64, c_void_p, c_int32, c_int64, POINTER(Sampling), c_void_p]),
+    "swvr_sample_workspace_size": (c_int, [POINTER(Problem), POINTER(c_size_t)]),
+    "swvr_sample": (c_int, [POINTER(Problem), POINTER(Sampling), c_void_p, c_size_t, c_void_p]),
     "swvr_profile_start": (c_int, []),
     "swvr_profile_stop": (c_int, [POINTER(ProfileRecord), c_int, POINTER(c_int)]),
 }

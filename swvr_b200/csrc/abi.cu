@@ -52,12 +52,13 @@ static int num_sms() {
 
 // ---------------------------------------------------------------------------- launch accounting
 enum ProfKind { kProfFwd = 0, kProfBwdScores, kProfGemm, kProfCombine, kProfReduce, kProfPrologue, kProfCast,
-                kProfMse, kProfSimt, kProfNorm, kProfEmbed, kProfHead, kProfDistill,
+                kProfMse, kProfSimt, kProfNorm, kProfEmbed, kProfHead, kProfDistill, kProfSample,
                 kProfKinds };
 static const char* kProfNames[kProfKinds] = {"fwd_kernel",      "bwd_scores_kernel", "gemm_kernel",
                                              "combine_kernel",  "reduce_de_db_kernel", "prologue_kernel",
                                              "cast_kernel",     "mse_kernel",        "simt_kernels",
-                                             "rmsnorm_kernels", "embed_kernels", "head_kernel", "distill_kernels"};
+                                             "rmsnorm_kernels", "embed_kernels", "head_kernel", "distill_kernels",
+                                             "sample_kernel"};
 static std::mutex g_prof_mu;
 static bool g_prof_on = false;
 static int64_t g_prof_launches[kProfKinds];
