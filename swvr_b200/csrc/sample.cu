@@ -10,14 +10,17 @@
 // point, 2^44 for the largest (2^(62 - log2 V) where V is past 2^18), so sums are exact in any order, by any number of
 // threads.  Weights below 2^-44 of the largest are 0 (30.5 T below the maximum).
 //
-// A row is a cluster of 1 .. 8 CTAs, each holding a contiguous share of the scores in shared memory, so
-// the scores are read from global memory once; longer rows are read again in each pass.  Both thresholds are a
-// selection: one histogram pass puts the scores into 2048 bins of equal width below the maximum (count for
-// top-k, weight for top-p), the bin that holds the threshold is found by a scan, and its members
-// (a few hundred) are gathered in one CTA and ranked against one another.  A bin with more than
-// kList members (equal scores, mostly) is split again by the 64-bit order of (score, index) until it has
-// no more.  A last pass sums the kept weights per warp, in index order, and the warp whose
-// range holds u rescans its range.
+// A row is a cluster of 1 .. 8 CTAs, each holding a contiguous share of the scores in shared memory, in
+// their own type, so the scores are read from global memory once; longer rows are read again in each
+// pass.  The usual filters leave few tokens, and those are found without a weight for every score:
+//   1. scores in, the largest;
+//   2. top-k, top-p: a histogram over kBins bins of equal width below the largest (counts; weights too for a
+//      top-p without top-k), and the bin that holds the threshold; min-p alone knows its threshold;
+//   3. the tokens down to that bin, if there are at most kList, are gathered in one CTA, sorted by (score, index),
+//      cut by prefix sums, sorted by index, and u is looked up in the running sum.
+// Otherwise (no filter, a wide nucleus, long runs of equal scores) thresholds come from `boundary`, which splits the
+// threshold's bin by the order of (score, index) until kList members are left, and a pass over all scores sums
+// the kept weights per warp, in index order; the warp whose range holds u rescans it.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -33,7 +36,7 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 2048, kList = 1024;
+constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
 constexpr float kReach = 30.5f;  // e^-30.5 < 2^-44
 
@@ -55,8 +58,9 @@ struct Params {
   int u_dt;
   int64_t* token;
   float* logprob;
-  int share;      // scores per CTA
-  double one;     // 2^44 or less: the fixed-point weight of the largest score
+  int share;      // scores per CTA, a multiple of 32
+  int lg_one;     // log2 of the fixed-point weight of the largest score: 44 or less
+  bool aligned;   // rows start on 16-byte boundaries
   int64_t row0;   // first row of x among the rows of the settings, u and the outputs
 };
 
@@ -74,6 +78,7 @@ __device__ __forceinline__ float score_of(uint32_t o) {
 __device__ __forceinline__ u64 place_of(float x, uint32_t index) {
   return (static_cast<u64>(order_of(x)) << 32) | (0xffffffffu - index);
 }
+__device__ __forceinline__ uint32_t index_of(u64 place) { return 0xffffffffu - static_cast<uint32_t>(place); }
 
 template <typename T>
 __device__ __forceinline__ T warp_sum(T v) {
@@ -89,28 +94,72 @@ __device__ __forceinline__ u64 warp_max(u64 v) {
   }
   return v;
 }
+// Inclusive prefix sum over the warp.
+__device__ __forceinline__ u64 warp_scan(u64 v) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
 
 struct Shared {
-  u64 mass[kBins], mass_all[kBins];
-  uint32_t count[kBins], count_all[kBins];
+  u64 mass_all[kBins];
+  uint32_t count_all[kBins];
+  uint32_t count[kBins], mass_lo[kBins], mass_hi[kBins];
   u64 list[kList], list_w[kList];
-  u64 part[2 * kWarps];   // per-warp results of a block reduction or scan
+  double root[64];        // 2^(j / 64)
+  u64 part[kWarps];       // per-warp results of a block reduction or scan
   u64 slot[12];           // values other CTAs of the cluster read, each written once
-  u64 found[3];           // boundary bin, and count and weight before it
+  u64 found[3];           // boundary bin, and count or weight before it
   uint32_t n_list;
+
+  __device__ __forceinline__ void add_mass(int b, u64 w) {
+    const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&mass_lo[b], lo);
+    const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old ? 1u : 0u);
+    if (hi) atomicAdd(&mass_hi[b], hi);
+  }
+  __device__ __forceinline__ u64 mass(int b) const { return (static_cast<u64>(mass_hi[b]) << 32) | mass_lo[b]; }
 };
+
+// A float as a double by its bits (a conversion runs at an eighth of the rate); subnormals as 0.
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t b = __float_as_uint(x);
+  if ((b & 0x7f800000u) == 0) return 0.0;
+  return __hiloint2double(static_cast<int>((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)),
+                          static_cast<int>(b << 29));
+}
 
 struct Row {
   float top;      // the largest score
-  double invT, one;
+  double top_d, c64;  // top, and 64 log2(e) / T
+  double invT;
+  int lg_one;
   float reach;    // scores further below have no weight
   float per_bin;  // bins per unit of score
+  const double* root;
 
   __device__ __forceinline__ bool live(float x) const { return x == top || top - x < reach; }
+  // exp((x - top) / T) 2^lg_one, rounded.  With y = 64 log2(e) (x - top) / T = n + f, |f| <= 1/2:
+  // 2^(y / 64) = 2^(n / 64) e^(f ln 2 / 64), the first factor from a table of 64, the second a polynomial of
+  // degree 4 (remainder 2^-44.6), in doubles.  Adding 1.5 2^52 rounds y to n, adding 2^52 rounds the result.
   __device__ __forceinline__ u64 weight(float x) const {
-    if (x == top) return static_cast<u64>(one);
+    if (x == top) return 1ull << lg_one;
     if (!(top - x < reach)) return 0;
-    return static_cast<u64>(exp((static_cast<double>(x) - top) * invT) * one + 0.5);
+    constexpr double kRound = 6755399441055744.0, a1 = 0.6931471805599453 / 64;
+    const double dx = widen(x) - top_d;
+    const double m = fma(dx, c64, kRound);
+    const int n = __double2loint(m);
+    const double f = fma(dx, c64, -(m - kRound));
+    double q = fma(f, a1 * a1 * a1 * a1 / 24, a1 * a1 * a1 / 6);
+    q = fma(f, q, a1 * a1 / 2);
+    q = fma(f, q, a1);
+    q = fma(f, q, 1.0);
+    double v = root[n & 63] * q;
+    v = __hiloint2double(__double2hiint(v) + (((n >> 6) + lg_one) << 20), __double2loint(v));
+    return static_cast<u64>(__double_as_longlong(v + 4503599627370496.0)) & 0xfffffffffffffull;
   }
   // rises as x falls: subtraction, product and conversion are all monotone
   __device__ __forceinline__ int bin(float x) const {
@@ -118,21 +167,43 @@ struct Row {
   }
 };
 
-template <bool kHeld>
+__device__ __forceinline__ float to_score(float v) { return v != v ? -INFINITY : v + 0.f; }  // NaN never wins; -0 equals +0
+__device__ __forceinline__ float to_score(__nv_bfloat16 v) { return to_score(__bfloat162float(v)); }
+__device__ __forceinline__ float to_score(__half v) { return to_score(__half2float(v)); }
+
+// This CTA's scores: in shared memory (kHeld), or where they are.
+template <typename T, bool kHeld>
 struct Scores {
-  const void* x;
-  int dt;
-  int64_t base;  // element of x that this CTA's first score is
-  const float* held;
+  static constexpr int VEC = 16 / sizeof(T);
+  const T* x;      // this CTA's first score
+  const T* held;
+  bool aligned;
   int n;
   uint32_t first;  // its index in the row
-  __device__ __forceinline__ float raw(int i) const {
-    const float v = load_f(x, dt, base + i);
-    return v != v ? -INFINITY : v + 0.f;  // NaN never wins; -0 equals +0
+
+  __device__ __forceinline__ float at(int i) const { return to_score(kHeld ? held[i] : x[i]); }
+  // VEC scores from i on (i a multiple of VEC); -inf past the end
+  __device__ __forceinline__ void vec(int i, float (&v)[VEC]) const {
+    if ((kHeld || aligned) && i + VEC <= n) {
+      struct alignas(16) P { T e[VEC]; };
+      const P p = *reinterpret_cast<const P*>((kHeld ? held : x) + i);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = to_score(p.e[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = i + k < n ? at(i + k) : -INFINITY;
+    }
   }
-  __device__ __forceinline__ float at(int i) const {
-    if constexpr (kHeld) return held[i];
-    else return raw(i);
+  // f(score, index within the CTA) for every score, in no order
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = threadIdx.x * VEC; i < n; i += kThreads * VEC) {
+      float v[VEC];
+      vec(i, v);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (v[k] != -INFINITY) f(v[k], i + k);
+    }
   }
 };
 
@@ -155,8 +226,18 @@ __device__ __forceinline__ u64 block_sum(u64 v, Shared& s) {
   for (int i = 0; i < kWarps; ++i) r += s.part[i];
   return r;
 }
+// Exclusive prefix sum over the block's threads, in thread order.
+__device__ __forceinline__ u64 block_scan(u64 v, Shared& s) {
+  const u64 inc = warp_scan(v);
+  __syncthreads();
+  if (threadIdx.x % 32 == 31) s.part[threadIdx.x / 32] = inc;
+  __syncthreads();
+  u64 r = inc - v;
+  for (int i = 0; i < static_cast<int>(threadIdx.x) / 32; ++i) r += s.part[i];
+  return r;
+}
 
-// The cluster's maximum / sum of a block value, through slot `at` (each used once).
+// The cluster's maximum of a block value, through slot `at` (each used once).
 __device__ __forceinline__ u64 cluster_max(u64 v, int at, Shared& s, cg::cluster_group& cl) {
   if (threadIdx.x == 0) s.slot[at] = v;
   cl.sync();
@@ -168,20 +249,30 @@ __device__ __forceinline__ u64 cluster_max(u64 v, int at, Shared& s, cg::cluster
   return r;
 }
 
+__device__ __forceinline__ void clear_bins(bool masses, Shared& s) {
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    s.count[b] = 0;
+    if (masses) s.mass_lo[b] = s.mass_hi[b] = 0;
+  }
+  __syncthreads();
+}
+
 // Adds up the CTAs' histograms: each CTA sums its share of the bins and hands the sums to all.
-__device__ __forceinline__ void merge_bins(bool counts, bool masses, Shared& s, cg::cluster_group& cl) {
+__device__ __forceinline__ void merge_bins(bool masses, Shared& s, cg::cluster_group& cl) {
   const unsigned C = cl.num_blocks(), me = cl.block_rank();
   cl.sync();  // every CTA's bins are complete, and nobody reads the sums of the pass before
   for (int b = me * (kBins / C) + threadIdx.x; b < static_cast<int>((me + 1) * (kBins / C)); b += kThreads) {
     uint32_t c = 0;
     u64 m = 0;
     for (unsigned r = 0; r < C; ++r) {
-      if (counts) c += *cl.map_shared_rank(&s.count[b], r);
-      if (masses) m += *cl.map_shared_rank(&s.mass[b], r);
+      const Shared* o = cl.map_shared_rank(&s, r);
+      c += o->count[b];
+      if (masses) m += o->mass(b);
     }
     for (unsigned r = 0; r < C; ++r) {
-      if (counts) *cl.map_shared_rank(&s.count_all[b], r) = c;
-      if (masses) *cl.map_shared_rank(&s.mass_all[b], r) = m;
+      Shared* o = cl.map_shared_rank(&s, r);
+      o->count_all[b] = c;
+      if (masses) o->mass_all[b] = m;
     }
   }
   cl.sync();
@@ -191,29 +282,18 @@ __device__ __forceinline__ void merge_bins(bool counts, bool masses, Shared& s, 
 // counts or by weights.  found[0] = kBins when the bins sum to less.
 template <bool kByCount>
 __device__ __forceinline__ void find_bin(u64 goal, Shared& s) {
-  const int t = threadIdx.x, lane = t % 32, warp = t / 32;
   u64 v[kBinsPer], sum = 0;
 #pragma unroll
   for (int i = 0; i < kBinsPer; ++i) {
-    v[i] = kByCount ? s.count_all[t * kBinsPer + i] : s.mass_all[t * kBinsPer + i];
+    v[i] = kByCount ? s.count_all[threadIdx.x * kBinsPer + i] : s.mass_all[threadIdx.x * kBinsPer + i];
     sum += v[i];
   }
-  u64 inc = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 up = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += up;
-  }
-  __syncthreads();
-  if (lane == 31) s.part[warp] = inc;
-  if (t == 0) s.found[0] = kBins;
-  __syncthreads();
-  u64 before = inc - sum;
-  for (int i = 0; i < warp; ++i) before += s.part[i];
+  if (threadIdx.x == 0) s.found[0] = kBins;
+  u64 before = block_scan(sum, s);
 #pragma unroll
   for (int i = 0; i < kBinsPer; ++i) {
     if (before < goal && goal <= before + v[i]) {
-      s.found[0] = t * kBinsPer + i;
+      s.found[0] = threadIdx.x * kBinsPer + i;
       s.found[1] = before;
     }
     before += v[i];
@@ -221,65 +301,172 @@ __device__ __forceinline__ void find_bin(u64 goal, Shared& s) {
   __syncthreads();
 }
 
+// The weight, or the number, in the bins ahead of b.
+template <bool kByCount>
+__device__ __forceinline__ u64 ahead_of(int b, Shared& s) {
+  u64 w = 0;
+  for (int i = threadIdx.x; i < b; i += kThreads) w += kByCount ? s.count_all[i] : s.mass_all[i];
+  return block_sum(w, s);
+}
+
+// What top-p compares running weights with: ceil(p total), at least 1 so that one token stays.
+__device__ __forceinline__ u64 nucleus(double top_p, u64 total) {
+  const double g = ceil(fmax(top_p, 0.0) * static_cast<double>(total));
+  return g < 1.0 ? 1ull : min(static_cast<u64>(g), total);
+}
+
+// The running weight that the chosen token is the first to reach: floor(u total) + 1, at most total.
+__device__ __forceinline__ u64 goal_of(double u, u64 total) {
+  const double at = floor((u > 0.0 ? u : 0.0) * static_cast<double>(total));
+  return at >= static_cast<double>(total) ? total : min(static_cast<u64>(at) + 1ull, total);
+}
+
+// Bitonic sort of the list's first n entries (a power of two), largest key first; weights move along.
+__device__ __forceinline__ void sort_list(int n, Shared& s) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      for (int t = threadIdx.x; t < n / 2; t += kThreads) {
+        const int i = 2 * t - (t & (stride - 1)), j = i + stride;
+        const u64 a = s.list[i], b = s.list[j];
+        if ((a < b) == ((i & size) == 0)) {
+          s.list[i] = b;
+          s.list[j] = a;
+          const u64 w = s.list_w[i];
+          s.list_w[i] = s.list_w[j];
+          s.list_w[j] = w;
+        }
+      }
+      __syncthreads();
+    }
+}
+
+// The token from a list of m places and weights that holds every token the filters may keep (one CTA).
+// total: the weight that top-p refers to, or 0 for that of the first k.
+__device__ __forceinline__ void choose_from_list(int m, bool by_k, u64 k, bool by_p, double top_p, u64 total, u64 cut,
+                                                 double u, int64_t* token, float* x_token, bool* mine, Shared& s) {
+  constexpr int PER = kList / kThreads;
+  int n = 32;
+  while (n < m) n <<= 1;
+  for (int i = m + threadIdx.x; i < n; i += kThreads) s.list[i] = 0, s.list_w[i] = 0;
+  __syncthreads();
+  sort_list(n, s);
+  // entries of this thread: consecutive ones, so that prefix sums follow the order
+  u64 w[PER], sum = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = threadIdx.x * PER + e;
+    w[e] = i < n && !(by_k && static_cast<u64>(i) >= k) ? s.list_w[i] : 0;
+    sum += w[e];
+  }
+  u64 ahead = block_scan(sum, s);
+  const u64 goal_p = by_p ? nucleus(top_p, total ? total : block_sum(sum, s)) : ~0ull;
+  // kept ones keep their weight and are put in index order (places below 2^32 order by index)
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = threadIdx.x * PER + e;
+    const bool keep = w[e] != 0 && ahead < goal_p && s.list[i] >= cut;
+    ahead += w[e];
+    if (i < n && !keep) s.list_w[i] = 0;
+  }
+  __syncthreads();
+  // the order of the first sort's high words is not needed any more, but the score of the token is (logprob):
+  // it comes from the place, so only the comparison key changes
+  u64 key[PER], kw[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = threadIdx.x * PER + e;
+    key[e] = i < n ? (s.list[i] << 32) | (s.list[i] >> 32) : 0;  // index first, score behind
+    kw[e] = i < n ? s.list_w[i] : 0;
+    if (kw[e] == 0) key[e] = 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = threadIdx.x * PER + e;
+    if (i < n) s.list[i] = key[e], s.list_w[i] = kw[e];
+  }
+  __syncthreads();
+  sort_list(n, s);  // complemented indices, largest first: rising index
+  sum = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = threadIdx.x * PER + e;
+    w[e] = i < n ? s.list_w[i] : 0;
+    sum += w[e];
+  }
+  ahead = block_scan(sum, s);
+  const u64 goal = goal_of(u, block_sum(sum, s));
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    if (ahead < goal && goal <= ahead + w[e]) {
+      const u64 kx = s.list[threadIdx.x * PER + e];
+      *token = 0xffffffffu - static_cast<uint32_t>(kx >> 32);
+      *x_token = score_of(static_cast<uint32_t>(kx));
+      *mine = true;
+    }
+    ahead += w[e];
+  }
+}
+
+// Gathers in CTA 0 the places and weights of the scores that pass; returns their number, which may be over
+// kList (then the list is not complete).
+template <typename T, bool kHeld, typename F>
+__device__ __forceinline__ uint32_t gather(const Scores<T, kHeld>& sc, const Row& row, F pass, Shared& s, cg::cluster_group& cl) {
+  Shared* s0 = cl.map_shared_rank(&s, 0);
+  if (threadIdx.x == 0) s.n_list = 0;
+  cl.sync();
+  sc.each([&](float x, int i) {
+    if (!pass(x, i)) return;
+    const uint32_t j = atomicAdd(&s0->n_list, 1u);
+    if (j < kList) {
+      s0->list[j] = place_of(x, sc.first + i);
+      s0->list_w[j] = row.weight(x);
+    }
+  });
+  cl.sync();
+  return s0->n_list;
+}
+
 // The lowest kept place when tokens are kept while what is ahead of them (their number, or their weight) is
-// below goal; `bin` holds the boundary and `before` is ahead of it.  *kept: the weight of all kept.
-template <bool kHeld, bool kByCount>
-__device__ u64 boundary(const Scores<kHeld>& sc, const Row& row, int bin, u64 before, u64 goal, bool masses,
-                        u64 mass_before, u64* kept, Shared& s, cg::cluster_group& cl) {
+// below goal; `bin` holds the boundary and `before` is ahead of it.
+template <bool kByCount, typename T, bool kHeld>
+__device__ __noinline__ u64 boundary(const Scores<T, kHeld>& sc, const Row& row, int bin, u64 before, u64 goal, Shared& s,
+                                     cg::cluster_group& cl) {
   u64 lo = 0, hi = ~0ull;  // places of the members still in question
   Shared* s0 = cl.map_shared_rank(&s, 0);
+  auto member = [&](float x, int i) {
+    if (!row.live(x) || row.bin(x) != bin) return false;
+    const u64 pl = place_of(x, sc.first + i);
+    return pl >= lo && pl <= hi;
+  };
   while (true) {
-    if (threadIdx.x == 0) s.n_list = 0;
-    cl.sync();
-    for (int i = threadIdx.x; i < sc.n; i += kThreads) {
-      const float x = sc.at(i);
-      if (!row.live(x) || row.bin(x) != bin) continue;
-      const u64 pl = place_of(x, sc.first + i);
-      if (pl < lo || pl > hi) continue;
-      const uint32_t j = atomicAdd(&s0->n_list, 1u);
-      if (j < kList) {
-        s0->list[j] = pl;
-        s0->list_w[j] = kByCount && !masses ? 0 : row.weight(x);
-      }
-    }
-    cl.sync();
-    const uint32_t m = *cl.map_shared_rank(&s.n_list, 0);
+    const uint32_t m = gather(sc, row, member, s, cl);
     if (m <= kList) {
       if (cl.block_rank() == 0) {
-        u64 low = ~0ull, w_kept = 0;
+        u64 low = ~0ull;
         for (int i = threadIdx.x; i < static_cast<int>(m); i += kThreads) {
           const u64 mine = s.list[i];
           u64 ahead = before;
           for (uint32_t j = 0; j < m; ++j)
             if (s.list[j] > mine) ahead += kByCount ? 1 : s.list_w[j];
-          if (ahead < goal) {
-            low = mine < low ? mine : low;
-            w_kept += s.list_w[i];
-          }
+          if (ahead < goal) low = mine < low ? mine : low;
         }
-        const u64 lowest = ~block_max(~low, s);
-        const u64 w = block_sum(w_kept, s);
-        if (threadIdx.x == 0) {
-          s.found[0] = lowest;
-          s.found[1] = mass_before + w;
-        }
+        low = ~block_max(~low, s);
+        if (threadIdx.x == 0) s.found[0] = low;
       }
       cl.sync();
       const u64 r = s0->found[0];
-      *kept = s0->found[1];
       cl.sync();  // found is written again only after everyone has read it
       return r;
     }
-    // too many for the list: split [least, greatest] place of the members into kBins equal ranges
+    // too many for the list: split [least, most] place of the members into kBins equal ranges
     u64 least = ~0ull, most = 0;
-    for (int i = threadIdx.x; i < sc.n; i += kThreads) {
-      const float x = sc.at(i);
-      if (!row.live(x) || row.bin(x) != bin) continue;
+    sc.each([&](float x, int i) {
+      if (!member(x, i)) return;
       const u64 pl = place_of(x, sc.first + i);
-      if (pl < lo || pl > hi) continue;
       least = pl < least ? pl : least;
       most = pl > most ? pl : most;
-    }
+    });
     least = ~block_max(~least, s);
     most = block_max(most, s);
     cl.sync();
@@ -292,62 +479,111 @@ __device__ u64 boundary(const Scores<kHeld>& sc, const Row& row, int bin, u64 be
     }
     int shift = 0;
     while (((most - least) >> shift) >= kBins) ++shift;
-    for (int b = threadIdx.x; b < kBins; b += kThreads) s.count[b] = 0, s.mass[b] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < sc.n; i += kThreads) {
-      const float x = sc.at(i);
-      if (!row.live(x) || row.bin(x) != bin) continue;
-      const u64 pl = place_of(x, sc.first + i);
-      if (pl < lo || pl > hi) continue;
-      const int b = static_cast<int>((most - pl) >> shift);
-      atomicAdd(&s.count[b], 1u);
-      if (masses) atomicAdd(&s.mass[b], row.weight(x));
-    }
-    merge_bins(true, masses, s, cl);
+    clear_bins(!kByCount, s);
+    sc.each([&](float x, int i) {
+      if (!member(x, i)) return;
+      const int b = static_cast<int>((most - place_of(x, sc.first + i)) >> shift);
+      if (kByCount) atomicAdd(&s.count[b], 1u);
+      else s.add_mass(b, row.weight(x));
+    });
+    merge_bins(!kByCount, s, cl);
     find_bin<kByCount>(goal - before, s);
     const int b = static_cast<int>(s.found[0]);
     before += s.found[1];
-    if (masses) {
-      u64 w = 0;
-      for (int i = threadIdx.x; i < b; i += kThreads) w += s.mass_all[i];
-      mass_before += block_sum(w, s);
-    }
     hi = most - (static_cast<u64>(b) << shift);
     const u64 width = (1ull << shift) - 1;
     lo = hi >= width ? hi - width : 0;
   }
 }
 
-template <bool kHeld>
+// The lowest kept place of top-k and top-p, whatever they leave.
+template <typename T, bool kHeld>
+__device__ __noinline__ u64 thresholds(const Scores<T, kHeld>& sc, const Row& row, bool by_k, u64 k, bool by_p, double top_p,
+                                       Shared& s, cg::cluster_group& cl) {
+  u64 cut = 0;
+  if (by_k) {
+    clear_bins(false, s);
+    sc.each([&](float x, int i) {
+      if (row.live(x)) atomicAdd(&s.count[row.bin(x)], 1u);
+    });
+    merge_bins(false, s, cl);
+    find_bin<true>(k, s);
+    const int b = static_cast<int>(s.found[0]);
+    const u64 before = s.found[1];
+    if (b < kBins) cut = boundary<true>(sc, row, b, before, k, s, cl);  // else all that have weight fit
+  }
+  if (by_p) {
+    clear_bins(true, s);
+    sc.each([&](float x, int i) {
+      if (row.live(x) && place_of(x, sc.first + i) >= cut) s.add_mass(row.bin(x), row.weight(x));
+    });
+    merge_bins(true, s, cl);
+    const u64 goal = nucleus(top_p, ahead_of<false>(kBins, s));
+    find_bin<false>(goal, s);
+    const int b = static_cast<int>(s.found[0]);
+    const u64 before = s.found[1];
+    if (b < kBins) {
+      const u64 c = boundary<false>(sc, row, b, before, goal, s, cl);
+      cut = c > cut ? c : cut;
+    }
+  }
+  return cut;
+}
+
+template <typename T, bool kHeld>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
-  float* held = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
+  T* held = reinterpret_cast<T*>(smem_raw + sizeof(Shared));
   cg::cluster_group cl = cg::this_cluster();
   const unsigned C = cl.num_blocks(), me = cl.block_rank();
   const int64_t r = blockIdx.x / C, row_id = p.row0 + r;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  Scores<kHeld> sc;
-  sc.x = p.x;
-  sc.dt = p.dt;
+  constexpr int VEC = Scores<T, kHeld>::VEC;
   const int64_t first = static_cast<int64_t>(me) * p.share;
-  sc.base = r * p.ld + first;
+  Scores<T, kHeld> sc;
+  sc.x = static_cast<const T*>(p.x) + r * p.ld + first;
   sc.held = held;
+  sc.aligned = p.aligned;
   sc.first = static_cast<uint32_t>(first);
   sc.n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(p.share), p.V - first)));
+  if (tid < 64) s.root[tid] = exp2(tid / 64.0);
 
   // ---------------------------------------------------------------- scores in, the largest
   u64 best = 0;
-  for (int i = tid; i < sc.n; i += kThreads) {
-    const float x = sc.raw(i);
-    if constexpr (kHeld) held[i] = x;
-    const u64 pl = place_of(x, sc.first + i);
-    best = pl > best ? pl : best;
+  {
+    struct alignas(16) P { T e[VEC]; };
+    constexpr int U = 4;  // packs in flight per thread
+    for (int i = tid * VEC; i < sc.n; i += U * kThreads * VEC) {
+      P q[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int at = i + j * kThreads * VEC;
+        if (p.aligned && at + VEC <= sc.n) {
+          q[j] = *reinterpret_cast<const P*>(sc.x + at);
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            if (at + k < sc.n) q[j].e[k] = sc.x[at + k];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int at = i + j * kThreads * VEC;
+        if (at >= sc.n) break;
+        if constexpr (kHeld) *reinterpret_cast<P*>(held + at) = q[j];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          if (at + k < sc.n) {
+            const u64 pl = place_of(to_score(q[j].e[k]), sc.first + at + k);
+            best = pl > best ? pl : best;
+          }
+      }
+    }
   }
   best = cluster_max(block_max(best, s), 0, s, cl);
   Row row;
   row.top = score_of(static_cast<uint32_t>(best >> 32));
-  const uint32_t arg = 0xffffffffu - static_cast<uint32_t>(best);
   if (p.V == 0 || row.top == -INFINITY) {  // nothing to choose from
     if (me == 0 && tid == 0) {
       p.token[row_id] = -1;
@@ -356,139 +592,143 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     cl.sync();
     return;
   }
-  double T = setting(p.T, row_id);
-  const bool greedy = !(T > 0.0);
-  if (greedy) T = 1.0;
-  row.invT = 1.0 / T;
-  row.one = p.one;
-  row.reach = kReach * static_cast<float>(T);
+  double temp = setting(p.T, row_id);
+  const bool greedy = !(temp > 0.0);
+  if (greedy) temp = 1.0;
+  row.invT = 1.0 / temp;
+  row.c64 = 64 * 1.4426950408889634 * row.invT;
+  row.top_d = widen(row.top);
+  row.lg_one = p.lg_one;
+  row.reach = kReach * static_cast<float>(temp);
   row.per_bin = static_cast<float>(kBins) / row.reach;
+  row.root = s.root;
 
-  int64_t token = arg;
+  int64_t token = index_of(best);
   float x_token = row.top;
   bool mine = me == 0 && tid == 0;  // the thread that writes the result
   if (!greedy) {
-    // -------------------------------------------------------------- thresholds
     const int64_t k = p.k_ptr ? (p.k_bits == 64 ? static_cast<const int64_t*>(p.k_ptr)[row_id]
                                                 : static_cast<int64_t>(static_cast<const int32_t*>(p.k_ptr)[row_id]))
                               : p.k;
-    const double top_p = setting(p.p, row_id), min_p = setting(p.m, row_id);
-    const bool by_k = k > 0 && k < p.V, by_p = top_p < 1.0;
+    const double top_p = setting(p.p, row_id), min_p = setting(p.m, row_id), u = load_d(p.u, p.u_dt, row_id);
+    const bool by_k = k > 0 && k < p.V, by_p = top_p < 1.0, by_m = min_p > 0.0;
+    mine = false;
     u64 cut = 0;  // kept: place >= cut
-    if (by_k || by_p) {
-      for (int b = tid; b < kBins; b += kThreads) s.count[b] = 0, s.mass[b] = 0;
-      __syncthreads();
-      for (int i = tid; i < sc.n; i += kThreads) {
-        const float x = sc.at(i);
-        if (!row.live(x)) continue;
-        const int b = row.bin(x);
-        if (by_k) atomicAdd(&s.count[b], 1u);
-        if (by_p) atomicAdd(&s.mass[b], row.weight(x));
-      }
-      merge_bins(by_k, by_p, s, cl);
-      u64 total = 0;  // what top-k leaves
-      bool have_total = false;
-      if (by_k) {
-        find_bin<true>(static_cast<u64>(k), s);
-        const int b = static_cast<int>(s.found[0]);
-        if (b < kBins) {
-          const u64 before = s.found[1];
-          u64 w = 0;
-          if (by_p) {
-            for (int i = tid; i < b; i += kThreads) w += s.mass_all[i];
-            w = block_sum(w, s);
-          }
-          cut = boundary<kHeld, true>(sc, row, b, before, static_cast<u64>(k), by_p, w, &total, s, cl);
-          have_total = true;
-        }
-      }
-      if (by_p) {
-        // boundary() may have used the bins for a split: the weights of a pass before are gone, so the
-        // histogram is taken again, over what top-k left
-        if (have_total) {
-          for (int b = tid; b < kBins; b += kThreads) s.mass[b] = 0;
-          __syncthreads();
-          for (int i = tid; i < sc.n; i += kThreads) {
-            const float x = sc.at(i);
-            if (row.live(x) && place_of(x, sc.first + i) >= cut) atomicAdd(&s.mass[row.bin(x)], row.weight(x));
-          }
-          merge_bins(false, true, s, cl);
-        } else {
-          u64 w = 0;
-          for (int i = tid; i < kBins; i += kThreads) w += s.mass_all[i];
-          total = block_sum(w, s);
-        }
-        const double goal_r = ceil(fmax(top_p, 0.0) * static_cast<double>(total));
-        const u64 goal = goal_r < 1.0 ? 1ull : min(static_cast<u64>(goal_r), total);
-        find_bin<false>(goal, s);
-        const int b = static_cast<int>(s.found[0]);
-        if (b < kBins) {
-          const u64 before = s.found[1];
-          u64 ignored;
-          const u64 c = boundary<kHeld, false>(sc, row, b, before, goal, true, before, &ignored, s, cl);
-          cut = c > cut ? c : cut;
-        }
-      }
-    }
-    if (min_p > 0.0) {
+    if (by_m) {
       // the lowest score with exp((x - top) / T) >= min_p: the nearest float to the root, or a neighbour
-      const double lm = log(min(min_p, 1.0));
-      auto keeps = [&](uint32_t o) { return (static_cast<double>(score_of(o)) - row.top) * row.invT >= lm; };
-      uint32_t o = order_of(static_cast<float>(static_cast<double>(row.top) + T * lm));
+      const double lm = log(min(min_p, 1.0)), top = row.top;
+      auto keeps = [&](uint32_t o) { return (static_cast<double>(score_of(o)) - top) * row.invT >= lm || score_of(o) == row.top; };
+      uint32_t o = order_of(static_cast<float>(top + temp * lm));
       const uint32_t o_top = order_of(row.top), o_low = order_of(-INFINITY) + 1;
       o = min(max(o, o_low), o_top);
       for (int i = 0; i < 8 && o > o_low && keeps(o - 1); ++i) --o;
       for (int i = 0; i < 8 && o < o_top && !keeps(o); ++i) ++o;
-      const u64 c = static_cast<u64>(o) << 32;
-      cut = c > cut ? c : cut;
+      cut = static_cast<u64>(o) << 32;
     }
-    // -------------------------------------------------------------- the token
-    const int span = (sc.n + 32 * kWarps - 1) / (32 * kWarps) * 32;  // scores per warp, contiguous
-    const int i0 = min(sc.n, warp * span), i1 = min(sc.n, i0 + span);
-    u64 w = 0;
-    for (int i = i0 + lane; i < i1; i += 32) {
-      const float x = sc.at(i);
-      if (place_of(x, sc.first + i) >= cut) w += row.weight(x);
+    // -------------------------------------------------------------- few tokens left
+    bool done = false;
+    if (by_k || by_p || by_m) {
+      int last = kBins;  // the bin that holds the threshold
+      bool few = !by_k || k <= kList;
+      u64 total = 0;
+      if (few && (by_k || by_p)) {
+        const bool masses = !by_k;
+        clear_bins(masses, s);
+        sc.each([&](float x, int i) {
+          if (!row.live(x)) return;
+          const int b = row.bin(x);
+          atomicAdd(&s.count[b], 1u);
+          if (masses) s.add_mass(b, row.weight(x));
+        });
+        merge_bins(masses, s, cl);
+        if (by_k) {
+          find_bin<true>(static_cast<u64>(k), s);
+        } else {
+          total = ahead_of<false>(kBins, s);
+          find_bin<false>(nucleus(top_p, total), s);
+        }
+        last = static_cast<int>(s.found[0]);
+        few = ahead_of<true>(min(last + 1, kBins), s) <= kList;
+      }
+      if (few) {
+        const uint32_t m = gather(sc, row, [&](float x, int i) {
+          return row.live(x) && (last < kBins ? row.bin(x) <= last : true) &&
+                 (by_k || by_p || place_of(x, sc.first + i) >= cut);
+        }, s, cl);
+        if (m <= kList) {
+          done = true;
+          if (me == 0)
+            choose_from_list(static_cast<int>(m), by_k, static_cast<u64>(k), by_p, top_p, total, cut, u, &token, &x_token,
+                             &mine, s);
+        }
+      }
     }
-    w = warp_sum(w);
-    __syncthreads();
-    if (lane == 0) s.part[warp] = w;
-    __syncthreads();
-    u64 own = 0;
-    for (int i = 0; i < kWarps; ++i) own += s.part[i];
-    if (tid == 0) s.slot[1] = own;
-    cl.sync();
-    u64 ahead = 0, total = 0;
-    for (unsigned c = 0; c < C; ++c) {
-      const u64 o = *cl.map_shared_rank(&s.slot[1], c);
-      if (c < me) ahead += o;
-      total += o;
-    }
-    const double u = load_d(p.u, p.u_dt, row_id);
-    const double at = floor((u > 0.0 ? u : 0.0) * static_cast<double>(total));
-    const u64 goal = at >= static_cast<double>(total) ? total : min(static_cast<u64>(at) + 1ull, total);
-    mine = false;
-    for (int i = 0; i < warp; ++i) ahead += s.part[i];
-    if (ahead < goal && goal <= ahead + s.part[warp]) {  // this warp's range holds it
-      for (int i = i0 + lane; i - lane < i1; i += 32) {
-        const float x = i < i1 ? sc.at(i) : -INFINITY;
-        const u64 wi = i < i1 && place_of(x, sc.first + i) >= cut ? row.weight(x) : 0;
-        u64 inc = wi;
+    // -------------------------------------------------------------- many
+    if (!done) {
+      if (by_k || by_p) {
+        const u64 c = thresholds(sc, row, by_k, static_cast<u64>(k), by_p, top_p, s, cl);
+        cut = c > cut ? c : cut;
+      }
+      constexpr int STEP = 32 * VEC;
+      const int span = (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;  // scores per warp, contiguous
+      const int i0 = min(sc.n, warp * span), i1 = min(sc.n, i0 + span);
+      auto kept_weight = [&](float x, int i) {
+        return x != -INFINITY && place_of(x, sc.first + i) >= cut ? row.weight(x) : 0ull;
+      };
+      u64 w = 0;
+      for (int i = i0 + lane * VEC; i < i1; i += STEP) {
+        float v[VEC];
+        sc.vec(i, v);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const u64 up = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += up;
-        }
-        const uint32_t reached = __ballot_sync(0xffffffffu, ahead + inc >= goal);
-        if (reached) {
-          if (lane == __ffs(reached) - 1) {
-            mine = true;
-            token = sc.first + i;
-            x_token = x;
+        for (int e = 0; e < VEC; ++e) w += kept_weight(v[e], i + e);
+      }
+      w = warp_sum(w);
+      __syncthreads();
+      if (lane == 0) s.part[warp] = w;
+      __syncthreads();
+      u64 own = 0;
+      for (int i = 0; i < kWarps; ++i) own += s.part[i];
+      if (tid == 0) s.slot[1] = own;
+      cl.sync();
+      u64 ahead = 0, total = 0;
+      for (unsigned c = 0; c < C; ++c) {
+        const u64 o = *cl.map_shared_rank(&s.slot[1], c);
+        if (c < me) ahead += o;
+        total += o;
+      }
+      const u64 goal = goal_of(u, total);
+      for (int i = 0; i < warp; ++i) ahead += s.part[i];
+      if (ahead < goal && goal <= ahead + s.part[warp]) {  // this warp's range holds it
+        for (int i = i0 + lane * VEC; i - lane * VEC < i1; i += STEP) {
+          float v[VEC];
+          u64 we[VEC], sum = 0;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = -INFINITY;
+          if (i < i1) sc.vec(i, v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            we[e] = kept_weight(v[e], i + e);
+            sum += we[e];
           }
-          break;
+          const u64 inc = warp_scan(sum);
+          const uint32_t reached = __ballot_sync(0xffffffffu, ahead + inc >= goal);
+          if (reached) {
+            if (lane == __ffs(reached) - 1) {
+              u64 at = ahead + inc - sum;
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) {
+                if (!mine && at + we[e] >= goal && we[e] != 0) {
+                  mine = true;
+                  token = sc.first + i + e;
+                  x_token = v[e];
+                }
+                at += we[e];
+              }
+            }
+            break;
+          }
+          ahead += __shfl_sync(0xffffffffu, inc, 31);
         }
-        ahead += __shfl_sync(0xffffffffu, inc, 31);
       }
     }
   }
@@ -496,7 +736,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   if (p.logprob) {
     // log softmax(x / T) of the token over the whole row
     u64 w = 0;
-    for (int i = tid; i < sc.n; i += kThreads) w += row.weight(sc.at(i));
+    sc.each([&](float x, int i) { w += row.weight(x); });
     w = block_sum(w, s);
     if (tid == 0) s.slot[2] = w;
     cl.sync();
@@ -504,25 +744,27 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     for (unsigned c = 0; c < C; ++c) all += *cl.map_shared_rank(&s.slot[2], c);
     if (mine)
       p.logprob[row_id] = static_cast<float>((x_token == row.top ? 0.0 : (static_cast<double>(x_token) - row.top) * row.invT) -
-                                             log(static_cast<double>(all) / row.one));
+                                             log(ldexp(static_cast<double>(all), -row.lg_one)));
   }
   cl.sync();  // no CTA leaves while another may read its shared memory
 }
 
 // ------------------------------------------------------------------ host
 constexpr size_t kSmemMax = 227 * 1024;
-constexpr int kHeldMax = static_cast<int>((kSmemMax - sizeof(Shared)) / 4 / 32 * 32);
 
-static cudaError_t launch(Params p, cudaStream_t st) {
-  // the smallest cluster whose CTAs hold the row; few rows take the largest, to spread over the SMs
+template <typename T>
+static cudaError_t launch_t(Params p, cudaStream_t st) {
+  constexpr int64_t most = static_cast<int64_t>((kSmemMax - sizeof(Shared)) / sizeof(T) / 32 * 32);
+  // the smallest cluster whose CTAs hold the row; few rows take more, to spread over the SMs
   int C = 1;
-  while (C < 8 && ((p.V + C - 1) / C > kHeldMax || p.N * C < kNumSMsB200 / 2) && p.V > 2048 * C) C *= 2;
+  while (C < 8 && (ceil_div(p.V, C) > most || p.N * C < kNumSMsB200 / 2) && p.V > 2048 * C) C *= 2;
   p.share = static_cast<int>(round_up(ceil_div(std::max<int64_t>(p.V, 1), C), 32));
-  const bool held = p.share <= kHeldMax;
+  const bool held = p.share <= most;
+  p.aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.ld * sizeof(T)) % 16 == 0;
   int lg = 0;
   while ((1ll << lg) < p.V) ++lg;
-  p.one = std::ldexp(1.0, std::min(44, 62 - lg));
-  auto kern = held ? sample_kernel<true> : sample_kernel<false>;
+  p.lg_one = std::min(44, 62 - lg);
+  auto kern = held ? sample_kernel<T, true> : sample_kernel<T, false>;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -533,11 +775,17 @@ static cudaError_t launch(Params p, cudaStream_t st) {
   cfg.numAttrs = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(p.N * C), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = sizeof(Shared) + (held ? static_cast<size_t>(p.share) * 4 : 0);
+  cfg.dynamicSmemBytes = sizeof(Shared) + (held ? static_cast<size_t>(p.share) * sizeof(T) : 0);
   cfg.stream = st;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
   if (e != cudaSuccess) return e;
   return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+static cudaError_t launch(const Params& p, cudaStream_t st) {
+  if (p.dt == SWVR_F32) return launch_t<float>(p, st);
+  if (p.dt == SWVR_BF16) return launch_t<__nv_bfloat16>(p, st);
+  return launch_t<__half>(p, st);
 }
 
 static bool float_dtype(int dt) { return dt >= SWVR_F32 && dt <= SWVR_F16; }
