@@ -12,15 +12,17 @@
 //
 // A row is a cluster of 1 .. 8 CTAs, each holding a contiguous share of the scores in shared memory, in
 // their own type, so the scores are read from global memory once; longer rows are read again in each
-// pass.  The usual filters leave few tokens, and those are found without a weight for every score:
-//   1. scores in, the largest;
-//   2. top-k, top-p: a histogram over kBins bins of equal width below the largest (counts; weights too for a
-//      top-p without top-k), and the bin that holds the threshold; min-p alone knows its threshold;
-//   3. the tokens down to that bin, if there are at most kList, are gathered in one CTA, sorted by (score, index),
-//      cut by prefix sums, sorted by index, and u is looked up in the running sum.
-// Otherwise (no filter, a wide nucleus, long runs of equal scores) thresholds come from `boundary`, which splits the
-// threshold's bin by the order of (score, index) until kList members are left, and a pass over all scores sums
-// the kept weights per warp, in index order; the warp whose range holds u rescans it.
+// pass.  The usual filters leave few tokens, and those are found without a weight or a bin for every score:
+//   1. scores in, the largest, and each thread's largest;
+//   2. a score that enough tokens reach: for top-k, the k-th of the threads' largest scores (k tokens are at
+//      least that large, and few more are, as long as k is well below the number of threads); for a top-p
+//      without top-k the 256-th of them, beside the weight of the whole row; min-p knows its own;
+//   3. the tokens that reach it are gathered in one CTA, ordered by (score, index), cut by prefix sums, and u is
+//      looked up in the running weight by index.
+// Otherwise (no filter, a wide nucleus, long runs of equal scores) thresholds come from a histogram over kBins
+// bins below the largest score and from `boundary`, which splits the threshold's bin by the order of
+// (score, index) until kList members are left; a last pass over all scores sums the kept weights per warp, in
+// index order, and the warp whose range holds u rescans it.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -78,7 +80,7 @@ __device__ __forceinline__ float score_of(uint32_t o) {
 __device__ __forceinline__ u64 place_of(float x, uint32_t index) {
   return (static_cast<u64>(order_of(x)) << 32) | (0xffffffffu - index);
 }
-__device__ __forceinline__ uint32_t index_of(u64 place) { return 0xffffffffu - static_cast<uint32_t>(place); }
+__device__ __forceinline__ uint32_t index_of(u64 place) { return 0xffffffffu - static_cast<uint32_t>(place); }  // of the low half
 
 template <typename T>
 __device__ __forceinline__ T warp_sum(T v) {
@@ -105,6 +107,15 @@ __device__ __forceinline__ u64 warp_scan(u64 v) {
   return v;
 }
 
+// Tokens at or ahead of a place.
+struct Cut {
+  float x;
+  uint32_t index;
+  __device__ __forceinline__ explicit Cut(u64 place) : x(place ? score_of(static_cast<uint32_t>(place >> 32)) : -INFINITY),
+                                                       index(index_of(place)) {}
+  __device__ __forceinline__ bool keeps(float v, uint32_t i) const { return v > x || (v == x && i <= index); }
+};
+
 struct Shared {
   u64 mass_all[kBins];
   uint32_t count_all[kBins];
@@ -127,9 +138,9 @@ struct Shared {
 // A float as a double by its bits (a conversion runs at an eighth of the rate); subnormals as 0.
 __device__ __forceinline__ double widen(float x) {
   const uint32_t b = __float_as_uint(x);
-  if ((b & 0x7f800000u) == 0) return 0.0;
-  return __hiloint2double(static_cast<int>((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)),
-                          static_cast<int>(b << 29));
+  const double v = __hiloint2double(static_cast<int>((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)),
+                                    static_cast<int>(b << 29));
+  return (b & 0x7f800000u) == 0 ? 0.0 : v;
 }
 
 struct Row {
@@ -145,9 +156,8 @@ struct Row {
   // exp((x - top) / T) 2^lg_one, rounded.  With y = 64 log2(e) (x - top) / T = n + f, |f| <= 1/2:
   // 2^(y / 64) = 2^(n / 64) e^(f ln 2 / 64), the first factor from a table of 64, the second a polynomial of
   // degree 4 (remainder 2^-44.6), in doubles.  Adding 1.5 2^52 rounds y to n, adding 2^52 rounds the result.
+  // No branch: several of a thread's scores are in flight at once.
   __device__ __forceinline__ u64 weight(float x) const {
-    if (x == top) return 1ull << lg_one;
-    if (!(top - x < reach)) return 0;
     constexpr double kRound = 6755399441055744.0, a1 = 0.6931471805599453 / 64;
     const double dx = widen(x) - top_d;
     const double m = fma(dx, c64, kRound);
@@ -159,7 +169,8 @@ struct Row {
     q = fma(f, q, 1.0);
     double v = root[n & 63] * q;
     v = __hiloint2double(__double2hiint(v) + (((n >> 6) + lg_one) << 20), __double2loint(v));
-    return static_cast<u64>(__double_as_longlong(v + 4503599627370496.0)) & 0xfffffffffffffull;
+    const u64 w = static_cast<u64>(__double_as_longlong(v + 4503599627370496.0)) & 0xfffffffffffffull;
+    return x == top ? 1ull << lg_one : (top - x < reach ? w : 0ull);
   }
   // rises as x falls: subtraction, product and conversion are all monotone
   __device__ __forceinline__ int bin(float x) const {
@@ -167,9 +178,18 @@ struct Row {
   }
 };
 
-__device__ __forceinline__ float to_score(float v) { return v != v ? -INFINITY : v + 0.f; }  // NaN never wins; -0 equals +0
-__device__ __forceinline__ float to_score(__nv_bfloat16 v) { return to_score(__bfloat162float(v)); }
-__device__ __forceinline__ float to_score(__half v) { return to_score(__half2float(v)); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ void set_lowest(float* v) { *v = -INFINITY; }
+__device__ __forceinline__ void set_lowest(__nv_bfloat16* v) { *v = __ushort_as_bfloat16(0xff80); }
+__device__ __forceinline__ void set_lowest(__half* v) { *v = __ushort_as_half(0xfc00); }
+// NaN never wins; -0 equals +0
+template <typename T>
+__device__ __forceinline__ float to_score(T v) {
+  const float f = to_float(v);
+  return f != f ? -INFINITY : f + 0.f;
+}
 
 // This CTA's scores: in shared memory (kHeld), or where they are.
 template <typename T, bool kHeld>
@@ -237,16 +257,15 @@ __device__ __forceinline__ u64 block_scan(u64 v, Shared& s) {
   return r;
 }
 
-// The cluster's maximum of a block value, through slot `at` (each used once).
-__device__ __forceinline__ u64 cluster_max(u64 v, int at, Shared& s, cg::cluster_group& cl) {
+// A block's value made the cluster's, through slot `at` (each used once): the largest, or the sum.
+template <bool kSum>
+__device__ __forceinline__ u64 cluster_join(u64 v, int at, Shared& s, cg::cluster_group& cl) {
+  if (cl.num_blocks() == 1) return v;
   if (threadIdx.x == 0) s.slot[at] = v;
   cl.sync();
-  u64 r = 0;
-  for (unsigned i = 0; i < cl.num_blocks(); ++i) {
-    const u64 o = *cl.map_shared_rank(&s.slot[at], i);
-    r = o > r ? o : r;
-  }
-  return r;
+  const unsigned lane = threadIdx.x % 32;
+  const u64 o = lane < cl.num_blocks() ? *cl.map_shared_rank(&s.slot[at], lane) : 0;
+  return kSum ? warp_sum(o) : warp_max(o);
 }
 
 __device__ __forceinline__ void clear_bins(bool masses, Shared& s) {
@@ -341,14 +360,53 @@ __device__ __forceinline__ void sort_list(int n, Shared& s) {
 }
 
 // The token from a list of m places and weights that holds every token the filters may keep (one CTA).
-// total: the weight that top-p refers to, or 0 for that of the first k.
-__device__ __forceinline__ void choose_from_list(int m, bool by_k, u64 k, bool by_p, double top_p, u64 total, u64 cut,
+// total: the weight that top-p refers to, or 0 for that of the first k.  `all`: the list is known to hold the
+// whole nucleus; otherwise false is returned when it does not.
+// Up to 256 entries are ranked by comparing each with all others (512 / n threads an entry), more are sorted
+// (55 steps of a barrier each at 1024).
+__device__ __forceinline__ bool choose_from_list(int m, bool by_k, u64 k, bool by_p, double top_p, u64 total, bool all, u64 cut,
                                                  double u, int64_t* token, float* x_token, bool* mine, Shared& s) {
-  constexpr int PER = kList / kThreads;
   int n = 32;
   while (n < m) n <<= 1;
   for (int i = m + threadIdx.x; i < n; i += kThreads) s.list[i] = 0, s.list_w[i] = 0;
   __syncthreads();
+  if (n <= 256) {
+    const int G = kThreads / n, i = threadIdx.x / G, g = threadIdx.x % G;  // G lanes of a warp share entry i
+    const u64 pl = s.list[i];
+    u64 w = s.list_w[i], ahead = 0;
+    uint32_t rank = 0;
+    for (int j = g; j < n; j += G) {
+      const bool before = s.list[j] > pl;
+      rank += before;
+      ahead += before ? s.list_w[j] : 0;
+    }
+    for (int o = 1; o < G; o <<= 1) {
+      rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    }
+    if (by_k && rank >= k) w = 0;  // what is ahead of the others is unchanged: it ranks behind them
+    if (by_p) {
+      const u64 sum = block_sum(g == 0 ? w : 0, s);
+      const u64 goal = nucleus(top_p, total ? total : sum);
+      if (!all && sum < goal) return false;
+      if (ahead >= goal) w = 0;
+    }
+    if (pl < cut) w = 0;
+    __syncthreads();  // everyone has read the weights
+    if (g == 0) s.list_w[i] = w;
+    const u64 goal = goal_of(u, block_sum(g == 0 ? w : 0, s));  // its barriers order the weights too
+    const uint32_t low = static_cast<uint32_t>(pl);             // complemented index: a larger one comes first
+    u64 run = 0;
+    for (int j = g; j < n; j += G) run += static_cast<uint32_t>(s.list[j]) > low ? s.list_w[j] : 0;
+    for (int o = 1; o < G; o <<= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
+    if (g == 0 && run < goal && goal <= run + w) {
+      *token = index_of(pl);
+      *x_token = score_of(static_cast<uint32_t>(pl >> 32));
+      *mine = true;
+    }
+    return true;
+  }
+  constexpr int PER = kList / kThreads;
   sort_list(n, s);
   // entries of this thread: consecutive ones, so that prefix sums follow the order
   u64 w[PER], sum = 0;
@@ -358,32 +416,28 @@ __device__ __forceinline__ void choose_from_list(int m, bool by_k, u64 k, bool b
     w[e] = i < n && !(by_k && static_cast<u64>(i) >= k) ? s.list_w[i] : 0;
     sum += w[e];
   }
-  u64 ahead = block_scan(sum, s);
-  const u64 goal_p = by_p ? nucleus(top_p, total ? total : block_sum(sum, s)) : ~0ull;
-  // kept ones keep their weight and are put in index order (places below 2^32 order by index)
+  u64 ahead = block_scan(sum, s), goal_p = ~0ull;
+  if (by_p) {
+    const u64 listed = block_sum(sum, s);
+    goal_p = nucleus(top_p, total ? total : listed);
+    if (!all && listed < goal_p) return false;
+  }
+  // kept ones, by index: the place with its halves exchanged orders by (index, score)
+  u64 key[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int i = threadIdx.x * PER + e;
-    const bool keep = w[e] != 0 && ahead < goal_p && s.list[i] >= cut;
+    const u64 pl = i < n ? s.list[i] : 0;
+    const bool keep = w[e] != 0 && ahead < goal_p && pl >= cut;
     ahead += w[e];
-    if (i < n && !keep) s.list_w[i] = 0;
-  }
-  __syncthreads();
-  // the order of the first sort's high words is not needed any more, but the score of the token is (logprob):
-  // it comes from the place, so only the comparison key changes
-  u64 key[PER], kw[PER];
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int i = threadIdx.x * PER + e;
-    key[e] = i < n ? (s.list[i] << 32) | (s.list[i] >> 32) : 0;  // index first, score behind
-    kw[e] = i < n ? s.list_w[i] : 0;
-    if (kw[e] == 0) key[e] = 0;
+    key[e] = keep ? (pl << 32) | (pl >> 32) : 0;
+    if (!keep) w[e] = 0;
   }
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int i = threadIdx.x * PER + e;
-    if (i < n) s.list[i] = key[e], s.list_w[i] = kw[e];
+    if (i < n) s.list[i] = key[e], s.list_w[i] = w[e];
   }
   __syncthreads();
   sort_list(n, s);  // complemented indices, largest first: rising index
@@ -400,12 +454,13 @@ __device__ __forceinline__ void choose_from_list(int m, bool by_k, u64 k, bool b
   for (int e = 0; e < PER; ++e) {
     if (ahead < goal && goal <= ahead + w[e]) {
       const u64 kx = s.list[threadIdx.x * PER + e];
-      *token = 0xffffffffu - static_cast<uint32_t>(kx >> 32);
+      *token = index_of(kx >> 32);
       *x_token = score_of(static_cast<uint32_t>(kx));
       *mine = true;
     }
     ahead += w[e];
   }
+  return true;
 }
 
 // Gathers in CTA 0 the places and weights of the scores that pass; returns their number, which may be over
@@ -514,8 +569,9 @@ __device__ __noinline__ u64 thresholds(const Scores<T, kHeld>& sc, const Row& ro
   }
   if (by_p) {
     clear_bins(true, s);
+    const Cut first_k(cut);
     sc.each([&](float x, int i) {
-      if (row.live(x) && place_of(x, sc.first + i) >= cut) s.add_mass(row.bin(x), row.weight(x));
+      if (row.live(x) && first_k.keeps(x, sc.first + i)) s.add_mass(row.bin(x), row.weight(x));
     });
     merge_bins(true, s, cl);
     const u64 goal = nucleus(top_p, ahead_of<false>(kBins, s));
@@ -531,7 +587,7 @@ __device__ __noinline__ u64 thresholds(const Scores<T, kHeld>& sc, const Row& ro
 }
 
 template <typename T, bool kHeld>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
   T* held = reinterpret_cast<T*>(smem_raw + sizeof(Shared));
@@ -550,7 +606,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   if (tid < 64) s.root[tid] = exp2(tid / 64.0);
 
   // ---------------------------------------------------------------- scores in, the largest
-  u64 best = 0;
+  float t_top = -INFINITY;  // of this thread (fmaxf leaves NaN out)
   {
     struct alignas(16) P { T e[VEC]; };
     constexpr int U = 4;  // packs in flight per thread
@@ -565,25 +621,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
 #pragma unroll
           for (int k = 0; k < VEC; ++k)
             if (at + k < sc.n) q[j].e[k] = sc.x[at + k];
+            else set_lowest(&q[j].e[k]);
         }
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int at = i + j * kThreads * VEC;
-        if (at >= sc.n) break;
-        if constexpr (kHeld) *reinterpret_cast<P*>(held + at) = q[j];
+        if constexpr (kHeld)
+          if (at < sc.n) *reinterpret_cast<P*>(held + at) = q[j];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k)
-          if (at + k < sc.n) {
-            const u64 pl = place_of(to_score(q[j].e[k]), sc.first + at + k);
-            best = pl > best ? pl : best;
-          }
+        for (int k = 0; k < VEC; ++k) t_top = fmaxf(t_top, to_float(q[j].e[k]));
       }
     }
   }
-  best = cluster_max(block_max(best, s), 0, s, cl);
+  t_top += 0.f;
   Row row;
-  row.top = score_of(static_cast<uint32_t>(best >> 32));
+  row.top = score_of(static_cast<uint32_t>(cluster_join<false>(block_max(order_of(t_top), s), 0, s, cl)));
   if (p.V == 0 || row.top == -INFINITY) {  // nothing to choose from
     if (me == 0 && tid == 0) {
       p.token[row_id] = -1;
@@ -603,16 +656,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   row.per_bin = static_cast<float>(kBins) / row.reach;
   row.root = s.root;
 
-  int64_t token = index_of(best);
+  int64_t token = 0;
   float x_token = row.top;
-  bool mine = me == 0 && tid == 0;  // the thread that writes the result
-  if (!greedy) {
+  bool mine = false;  // the thread that writes the result
+  if (greedy) {
+    u64 pl = 0;
+    sc.each([&](float x, int i) {
+      if (x == row.top) pl = max(pl, place_of(x, sc.first + i));
+    });
+    token = index_of(cluster_join<false>(block_max(pl, s), 1, s, cl));
+    mine = me == 0 && tid == 0;
+  } else {
     const int64_t k = p.k_ptr ? (p.k_bits == 64 ? static_cast<const int64_t*>(p.k_ptr)[row_id]
                                                 : static_cast<int64_t>(static_cast<const int32_t*>(p.k_ptr)[row_id]))
                               : p.k;
     const double top_p = setting(p.p, row_id), min_p = setting(p.m, row_id), u = load_d(p.u, p.u_dt, row_id);
     const bool by_k = k > 0 && k < p.V, by_p = top_p < 1.0, by_m = min_p > 0.0;
-    mine = false;
     u64 cut = 0;  // kept: place >= cut
     if (by_m) {
       // the lowest score with exp((x - top) / T) >= min_p: the nearest float to the root, or a neighbour
@@ -627,39 +686,44 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     }
     // -------------------------------------------------------------- few tokens left
     bool done = false;
-    if (by_k || by_p || by_m) {
-      int last = kBins;  // the bin that holds the threshold
-      bool few = !by_k || k <= kList;
+    if (by_m || (by_k ? static_cast<u64>(k) <= min(kThreads * C / 2, kList / 2) : by_p)) {
+      float reach_x = -INFINITY;  // a score that every token which may be kept reaches
+      bool few = true;
       u64 total = 0;
-      if (few && (by_k || by_p)) {
-        const bool masses = !by_k;
-        clear_bins(masses, s);
-        sc.each([&](float x, int i) {
-          if (!row.live(x)) return;
-          const int b = row.bin(x);
-          atomicAdd(&s.count[b], 1u);
-          if (masses) s.add_mass(b, row.weight(x));
-        });
-        merge_bins(masses, s, cl);
-        if (by_k) {
-          find_bin<true>(static_cast<u64>(k), s);
-        } else {
-          total = ahead_of<false>(kBins, s);
-          find_bin<false>(nucleus(top_p, total), s);
+      if (by_k || by_p) {
+        clear_bins(false, s);
+        if (t_top != -INFINITY && row.live(t_top)) atomicAdd(&s.count[row.bin(t_top)], 1u);
+        if (!by_k) {
+          u64 w = 0;
+          sc.each([&](float x, int i) { w += row.weight(x); });
+          total = cluster_join<true>(block_sum(w, s), 2, s, cl);
         }
-        last = static_cast<int>(s.found[0]);
-        few = ahead_of<true>(min(last + 1, kBins), s) <= kList;
+        merge_bins(false, s, cl);
+        find_bin<true>(by_k ? static_cast<u64>(k) : min(256u, kThreads * C / 2), s);
+        const int b = static_cast<int>(s.found[0]);
+        // the lower end of that bin, less what rounding may have moved; fewer live threads than asked for: all that
+        // have weight
+        const float d = b < kBins - 1 ? (b + 1) / row.per_bin * 1.000001f : row.reach;
+        reach_x = score_of(max(order_of(row.top - d), order_of(-INFINITY) + 2) - 2);
+        if (by_k && b == kBins) few = false;
       }
+      if (by_m && !(by_k && by_p)) reach_x = fmaxf(reach_x, Cut(cut).x);  // (top-p after top-k weighs the first k)
       if (few) {
-        const uint32_t m = gather(sc, row, [&](float x, int i) {
-          return row.live(x) && (last < kBins ? row.bin(x) <= last : true) &&
-                 (by_k || by_p || place_of(x, sc.first + i) >= cut);
-        }, s, cl);
+        const uint32_t m = gather(sc, row, [&](float x, int i) { return x >= reach_x && row.live(x); }, s, cl);
         if (m <= kList) {
-          done = true;
-          if (me == 0)
-            choose_from_list(static_cast<int>(m), by_k, static_cast<u64>(k), by_p, top_p, total, cut, u, &token, &x_token,
-                             &mine, s);
+          const bool all = by_k || !by_p || reach_x == Cut(cut).x;
+          if (me == 0) {
+            done = choose_from_list(static_cast<int>(m), by_k, static_cast<u64>(k), by_p, top_p, total, all, cut, u, &token,
+                                    &x_token, &mine, s);
+            if (tid == 0) s.slot[3] = done;
+          }
+          if (all) {
+            done = true;
+          } else {
+            if (C > 1) cl.sync();
+            else __syncthreads();
+            done = *cl.map_shared_rank(&s.slot[3], 0) != 0;
+          }
         }
       }
     }
@@ -672,8 +736,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       constexpr int STEP = 32 * VEC;
       const int span = (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;  // scores per warp, contiguous
       const int i0 = min(sc.n, warp * span), i1 = min(sc.n, i0 + span);
+      const Cut kept(cut);
       auto kept_weight = [&](float x, int i) {
-        return x != -INFINITY && place_of(x, sc.first + i) >= cut ? row.weight(x) : 0ull;
+        const u64 w = row.weight(x);
+        return kept.keeps(x, sc.first + i) ? w : 0ull;
       };
       u64 w = 0;
       for (int i = i0 + lane * VEC; i < i1; i += STEP) {
@@ -688,11 +754,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       __syncthreads();
       u64 own = 0;
       for (int i = 0; i < kWarps; ++i) own += s.part[i];
-      if (tid == 0) s.slot[1] = own;
+      if (tid == 0) s.slot[4] = own;
       cl.sync();
       u64 ahead = 0, total = 0;
       for (unsigned c = 0; c < C; ++c) {
-        const u64 o = *cl.map_shared_rank(&s.slot[1], c);
+        const u64 o = *cl.map_shared_rank(&s.slot[4], c);
         if (c < me) ahead += o;
         total += o;
       }
@@ -737,11 +803,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     // log softmax(x / T) of the token over the whole row
     u64 w = 0;
     sc.each([&](float x, int i) { w += row.weight(x); });
-    w = block_sum(w, s);
-    if (tid == 0) s.slot[2] = w;
-    cl.sync();
-    u64 all = 0;
-    for (unsigned c = 0; c < C; ++c) all += *cl.map_shared_rank(&s.slot[2], c);
+    const u64 all = cluster_join<true>(block_sum(w, s), 5, s, cl);
     if (mine)
       p.logprob[row_id] = static_cast<float>((x_token == row.top ? 0.0 : (static_cast<double>(x_token) - row.top) * row.invT) -
                                              log(ldexp(static_cast<double>(all), -row.lg_one)));
@@ -755,9 +817,10 @@ constexpr size_t kSmemMax = 227 * 1024;
 template <typename T>
 static cudaError_t launch_t(Params p, cudaStream_t st) {
   constexpr int64_t most = static_cast<int64_t>((kSmemMax - sizeof(Shared)) / sizeof(T) / 32 * 32);
-  // the smallest cluster whose CTAs hold the row; few rows take more, to spread over the SMs
+  constexpr int64_t pair = static_cast<int64_t>((kSmemMax / 2 - 1024 - sizeof(Shared)) / sizeof(T) / 32 * 32);
+  // the smallest cluster whose CTAs hold the row, two of them an SM; few rows take more, to spread over the SMs
   int C = 1;
-  while (C < 8 && (ceil_div(p.V, C) > most || p.N * C < kNumSMsB200 / 2) && p.V > 2048 * C) C *= 2;
+  while (C < 8 && (ceil_div(p.V, C) > pair || p.N * C < kNumSMsB200 / 2) && p.V > 2048 * C) C *= 2;
   p.share = static_cast<int>(round_up(ceil_div(std::max<int64_t>(p.V, 1), C), 32));
   const bool held = p.share <= most;
   p.aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.ld * sizeof(T)) % 16 == 0;
