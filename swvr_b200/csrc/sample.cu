@@ -23,6 +23,12 @@
 // bins below the largest score and from `boundary`, which splits the threshold's bin by the order of
 // (score, index) until kList members are left; a last pass over all scores sums the kept weights per warp, in
 // index order, and the warp whose range holds u rescans it.
+//
+// Sums over all scores (the row's weight for top-p, the last pass) are first taken with fp32 weights, an eighth of the
+// instructions.  A weight 2^y, y <= 0 in octaves, is then off by |y| 3 2^-24 ln 2 + 2^-22 relatively at most, and the weighted
+// mean of |y| is at most the distribution's entropy, so no partial sum is off by more than d = 2^-18 of the
+// total (V up to 2^20).  Where what is decided lies more than that from its border (2 d: both the running weight and the
+// total may be off) the fixed-point sums would decide the same; otherwise, a few rows in a hundred, they are taken.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -41,6 +47,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
 constexpr float kReach = 30.5f;  // e^-30.5 < 2^-44
+constexpr int kRoughBits = 18;   // fp32 sums are within 2^-18 of the total
 
 struct Setting {  // one value for all rows, or one per row
   const void* ptr;
@@ -116,14 +123,14 @@ struct Cut {
   __device__ __forceinline__ bool keeps(float v, uint32_t i) const { return v > x || (v == x && i <= index); }
 };
 
-struct Shared {
+struct alignas(16) Shared {  // the scores held behind it are stored 16 bytes at a time
   u64 mass_all[kBins];
   uint32_t count_all[kBins];
   uint32_t count[kBins], mass_lo[kBins], mass_hi[kBins];
   u64 list[kList], list_w[kList];
   double root[64];        // 2^(j / 64)
   u64 part[kWarps];       // per-warp results of a block reduction or scan
-  u64 slot[12];           // values other CTAs of the cluster read, each written once
+  u64 slot[13];           // values other CTAs of the cluster read, each written once
   u64 found[3];           // boundary bin, and count or weight before it
   uint32_t n_list;
 
@@ -143,6 +150,8 @@ __device__ __forceinline__ double widen(float x) {
   return (b & 0x7f800000u) == 0 ? 0.0 : v;
 }
 
+static_assert(sizeof(Shared) % 16 == 0, "alignment of the scores behind it");
+
 struct Row {
   float top;      // the largest score
   double top_d, c64;  // top, and 64 log2(e) / T
@@ -151,7 +160,23 @@ struct Row {
   float reach;    // scores further below have no weight
   float per_bin;  // bins per unit of score
   const double* root;
+  bool rough_ok;  // fp32 weights are within their bound
+  float c32;      // log2(e) / T
 
+  __device__ __forceinline__ float rough(float x) const { return ex2((x - top) * c32); }
+  // the sum over a pack of scores
+  template <int VEC, typename S>
+  __device__ __forceinline__ double rough_pack(const S& sc, int i) const {
+    float v[VEC];
+    sc.vec(i, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = rough(v[e]);
+#pragma unroll
+    for (int o = VEC / 2; o > 0; o /= 2)
+#pragma unroll
+      for (int e = 0; e < o; ++e) v[e] += v[e + o];
+    return static_cast<double>(v[0]);
+  }
   __device__ __forceinline__ bool live(float x) const { return x == top || top - x < reach; }
   // exp((x - top) / T) 2^lg_one, rounded.  With y = 64 log2(e) (x - top) / T = n + f, |f| <= 1/2:
   // 2^(y / 64) = 2^(n / 64) e^(f ln 2 / 64), the first factor from a table of 64, the second a polynomial of
@@ -228,6 +253,14 @@ struct Scores {
 };
 
 // Sum / maximum over the block, to every thread.
+__device__ __forceinline__ uint32_t block_max32(uint32_t v, Shared& s) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) s.part[threadIdx.x / 32] = v;
+  __syncthreads();
+  const int lane = threadIdx.x % 32;
+  return __reduce_max_sync(0xffffffffu, lane < kWarps ? static_cast<uint32_t>(s.part[lane]) : 0u);
+}
 __device__ __forceinline__ u64 block_max(u64 v, Shared& s) {
   v = warp_max(v);
   __syncthreads();
@@ -257,6 +290,16 @@ __device__ __forceinline__ u64 block_scan(u64 v, Shared& s) {
   return r;
 }
 
+constexpr int kMaxCluster = 8;
+
+// One value of every CTA of the cluster: the loads are in flight together (a remote one takes some 600 cycles).
+template <typename F>
+__device__ __forceinline__ void read_all(cg::cluster_group& cl, u64 (&v)[kMaxCluster], F address) {
+  const unsigned C = cl.num_blocks();
+#pragma unroll
+  for (unsigned c = 0; c < kMaxCluster; ++c) v[c] = c < C ? *address(c) : 0;
+}
+
 // A block's value made the cluster's, through slot `at` (each used once): the largest, or the sum.
 template <bool kSum>
 __device__ __forceinline__ u64 cluster_join(u64 v, int at, Shared& s, cg::cluster_group& cl) {
@@ -281,17 +324,21 @@ __device__ __forceinline__ void merge_bins(bool masses, Shared& s, cg::cluster_g
   const unsigned C = cl.num_blocks(), me = cl.block_rank();
   cl.sync();  // every CTA's bins are complete, and nobody reads the sums of the pass before
   for (int b = me * (kBins / C) + threadIdx.x; b < static_cast<int>((me + 1) * (kBins / C)); b += kThreads) {
-    uint32_t c = 0;
-    u64 m = 0;
-    for (unsigned r = 0; r < C; ++r) {
-      const Shared* o = cl.map_shared_rank(&s, r);
-      c += o->count[b];
-      if (masses) m += o->mass(b);
-    }
-    for (unsigned r = 0; r < C; ++r) {
-      Shared* o = cl.map_shared_rank(&s, r);
-      o->count_all[b] = c;
-      if (masses) o->mass_all[b] = m;
+    u64 v[kMaxCluster];
+    read_all(cl, v, [&](unsigned r) { return cl.map_shared_rank(&s.count[b], r); });
+    u64 sum = 0;
+#pragma unroll
+    for (unsigned r = 0; r < kMaxCluster; ++r) sum += v[r];
+    for (unsigned r = 0; r < C; ++r) *cl.map_shared_rank(&s.count_all[b], r) = static_cast<uint32_t>(sum);
+    if (masses) {
+      sum = 0;
+      read_all(cl, v, [&](unsigned r) { return cl.map_shared_rank(&s.mass_lo[b], r); });
+#pragma unroll
+      for (unsigned r = 0; r < kMaxCluster; ++r) sum += v[r];
+      read_all(cl, v, [&](unsigned r) { return cl.map_shared_rank(&s.mass_hi[b], r); });
+#pragma unroll
+      for (unsigned r = 0; r < kMaxCluster; ++r) sum += v[r] << 32;
+      for (unsigned r = 0; r < C; ++r) *cl.map_shared_rank(&s.mass_all[b], r) = sum;
     }
   }
   cl.sync();
@@ -340,7 +387,8 @@ __device__ __forceinline__ u64 goal_of(double u, u64 total) {
   return at >= static_cast<double>(total) ? total : min(static_cast<u64>(at) + 1ull, total);
 }
 
-// Bitonic sort of the list's first n entries (a power of two), largest key first; weights move along.
+// Bitonic sort of the list's first n entries (a power of two), largest key first; weights move along.  A warp's
+// 32 pairs span 64 entries while the stride is at most 32: only wider steps need the block's barrier.
 __device__ __forceinline__ void sort_list(int n, Shared& s) {
   for (int size = 2; size <= n; size <<= 1)
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
@@ -355,30 +403,37 @@ __device__ __forceinline__ void sort_list(int n, Shared& s) {
           s.list_w[j] = w;
         }
       }
-      __syncthreads();
+      // the next step's stride: half of this one, or this size's after stride 1
+      if (stride > 32 || (stride == 1 ? size : stride / 2) > 32) __syncthreads();
+      else __syncwarp();
     }
+  __syncthreads();
 }
 
+enum Found { kFound = 1, kNotListed, kUnsure };
+
 // The token from a list of m places and weights that holds every token the filters may keep (one CTA).
-// total: the weight that top-p refers to, or 0 for that of the first k.  `all`: the list is known to hold the
-// whole nucleus; otherwise false is returned when it does not.
-// Up to 256 entries are ranked by comparing each with all others (512 / n threads an entry), more are sorted
-// (55 steps of a barrier each at 1024).
-__device__ __forceinline__ bool choose_from_list(int m, bool by_k, u64 k, bool by_p, double top_p, u64 total, bool all, u64 cut,
-                                                 double u, int64_t* token, float* x_token, bool* mine, Shared& s) {
+// [total_lo, total_hi] holds the weight that top-p refers to (total_hi = 0: that of the first k).  `all`: the list is
+// known to hold the whole nucleus; otherwise kNotListed is returned when it does not.  kUnsure: tokens are kept or not
+// depending on where in the range the total lies; the list is as it was.
+// Up to 64 entries are ranked by comparing each with all others (512 / n threads an entry), more are sorted.
+__device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool by_p, double top_p, u64 total_lo, u64 total_hi,
+                                                  bool all, u64 cut, double u, int64_t* token, float* x_token, bool* mine,
+                                                  Shared& s) {
   int n = 32;
   while (n < m) n <<= 1;
   for (int i = m + threadIdx.x; i < n; i += kThreads) s.list[i] = 0, s.list_w[i] = 0;
   __syncthreads();
-  if (n <= 256) {
+  if (n <= 64) {
     const int G = kThreads / n, i = threadIdx.x / G, g = threadIdx.x % G;  // G lanes of a warp share entry i
     const u64 pl = s.list[i];
     u64 w = s.list_w[i], ahead = 0;
     uint32_t rank = 0;
+#pragma unroll 4
     for (int j = g; j < n; j += G) {
-      const bool before = s.list[j] > pl;
-      rank += before;
-      ahead += before ? s.list_w[j] : 0;
+      const u64 o = s.list[j], ow = s.list_w[j];
+      rank += o > pl;
+      ahead += o > pl ? ow : 0;
     }
     for (int o = 1; o < G; o <<= 1) {
       rank += __shfl_xor_sync(0xffffffffu, rank, o);
@@ -387,9 +442,10 @@ __device__ __forceinline__ bool choose_from_list(int m, bool by_k, u64 k, bool b
     if (by_k && rank >= k) w = 0;  // what is ahead of the others is unchanged: it ranks behind them
     if (by_p) {
       const u64 sum = block_sum(g == 0 ? w : 0, s);
-      const u64 goal = nucleus(top_p, total ? total : sum);
-      if (!all && sum < goal) return false;
-      if (ahead >= goal) w = 0;
+      const u64 lo = nucleus(top_p, total_hi ? total_lo : sum), hi = nucleus(top_p, total_hi ? total_hi : sum);
+      if (!all && sum < hi) return kNotListed;
+      if (lo != hi && __syncthreads_or(w != 0 && ahead >= lo && ahead < hi)) return kUnsure;
+      if (ahead >= lo) w = 0;
     }
     if (pl < cut) w = 0;
     __syncthreads();  // everyone has read the weights
@@ -397,14 +453,18 @@ __device__ __forceinline__ bool choose_from_list(int m, bool by_k, u64 k, bool b
     const u64 goal = goal_of(u, block_sum(g == 0 ? w : 0, s));  // its barriers order the weights too
     const uint32_t low = static_cast<uint32_t>(pl);             // complemented index: a larger one comes first
     u64 run = 0;
-    for (int j = g; j < n; j += G) run += static_cast<uint32_t>(s.list[j]) > low ? s.list_w[j] : 0;
+#pragma unroll 4
+    for (int j = g; j < n; j += G) {
+      const u64 ow = s.list_w[j];
+      run += static_cast<uint32_t>(s.list[j]) > low ? ow : 0;
+    }
     for (int o = 1; o < G; o <<= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
     if (g == 0 && run < goal && goal <= run + w) {
       *token = index_of(pl);
       *x_token = score_of(static_cast<uint32_t>(pl >> 32));
       *mine = true;
     }
-    return true;
+    return kFound;
   }
   constexpr int PER = kList / kThreads;
   sort_list(n, s);
@@ -419,8 +479,19 @@ __device__ __forceinline__ bool choose_from_list(int m, bool by_k, u64 k, bool b
   u64 ahead = block_scan(sum, s), goal_p = ~0ull;
   if (by_p) {
     const u64 listed = block_sum(sum, s);
-    goal_p = nucleus(top_p, total ? total : listed);
-    if (!all && listed < goal_p) return false;
+    goal_p = nucleus(top_p, total_hi ? total_lo : listed);
+    const u64 hi = nucleus(top_p, total_hi ? total_hi : listed);
+    if (!all && listed < hi) return kNotListed;
+    if (goal_p != hi) {
+      bool unsure = false;
+      u64 at = ahead;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        unsure |= w[e] != 0 && at >= goal_p && at < hi;
+        at += w[e];
+      }
+      if (__syncthreads_or(unsure)) return kUnsure;
+    }
   }
   // kept ones, by index: the place with its halves exchanged orders by (index, score)
   u64 key[PER];
@@ -460,26 +531,44 @@ __device__ __forceinline__ bool choose_from_list(int m, bool by_k, u64 k, bool b
     }
     ahead += w[e];
   }
-  return true;
+  return kFound;
 }
 
 // Gathers in CTA 0 the places and weights of the scores that pass; returns their number, which may be over
-// kList (then the list is not complete).
+// kList (then there is no list).  Each CTA lists its own first: a remote append per token would cost a round trip each.
 template <typename T, bool kHeld, typename F>
 __device__ __forceinline__ uint32_t gather(const Scores<T, kHeld>& sc, const Row& row, F pass, Shared& s, cg::cluster_group& cl) {
-  Shared* s0 = cl.map_shared_rank(&s, 0);
   if (threadIdx.x == 0) s.n_list = 0;
-  cl.sync();
+  __syncthreads();
   sc.each([&](float x, int i) {
     if (!pass(x, i)) return;
-    const uint32_t j = atomicAdd(&s0->n_list, 1u);
-    if (j < kList) {
-      s0->list[j] = place_of(x, sc.first + i);
-      s0->list_w[j] = row.weight(x);
-    }
+    const uint32_t j = atomicAdd(&s.n_list, 1u);
+    if (j < kList) s.list[j] = place_of(x, sc.first + i);
   });
   cl.sync();
-  return s0->n_list;
+  u64 n[kMaxCluster];
+  read_all(cl, n, [&](unsigned c) { return cl.map_shared_rank(&s.n_list, c); });
+  uint32_t m = 0, before = 0;  // before: of the CTAs ahead of the one this warp copies
+  const unsigned warp = threadIdx.x / 32;
+#pragma unroll
+  for (unsigned c = 0; c < kMaxCluster; ++c) {
+    if (c == warp) before = m;
+    m += static_cast<uint32_t>(n[c]);
+  }
+  if (m <= kList && cl.block_rank() == 0) {
+    if (warp > 0 && warp < cl.num_blocks()) {
+      const Shared* o = cl.map_shared_rank(&s, warp);
+      uint32_t count = 0;
+#pragma unroll
+      for (unsigned c = 0; c < kMaxCluster; ++c)
+        if (c == warp) count = static_cast<uint32_t>(n[c]);
+      for (uint32_t j = threadIdx.x % 32; j < count; j += 32) s.list[before + j] = o->list[j];
+    }
+    __syncthreads();
+    for (uint32_t j = threadIdx.x; j < m; j += kThreads) s.list_w[j] = row.weight(score_of(static_cast<uint32_t>(s.list[j] >> 32)));
+    __syncthreads();
+  }
+  return m;
 }
 
 // The lowest kept place when tokens are kept while what is ahead of them (their number, or their weight) is
@@ -511,7 +600,7 @@ __device__ __noinline__ u64 boundary(const Scores<T, kHeld>& sc, const Row& row,
       }
       cl.sync();
       const u64 r = s0->found[0];
-      cl.sync();  // found is written again only after everyone has read it
+      cl.sync();  // found, and the lists, are written again only after everyone has read them
       return r;
     }
     // too many for the list: split [least, most] place of the members into kBins equal ranges
@@ -586,6 +675,121 @@ __device__ __noinline__ u64 thresholds(const Scores<T, kHeld>& sc, const Row& ro
   return cut;
 }
 
+// The weight of this CTA's scores, in units of 2^-lg_one of the largest: in fixed point, or from fp32 weights.
+template <typename T, bool kHeld>
+__device__ __forceinline__ u64 exact_total(const Scores<T, kHeld>& sc, const Row& row, Shared& s) {
+  u64 w = 0;
+  sc.each([&](float x, int i) { w += row.weight(x); });
+  return block_sum(w, s);
+}
+template <typename T, bool kHeld>
+__device__ __forceinline__ u64 rough_total(const Scores<T, kHeld>& sc, const Row& row, Shared& s) {
+  constexpr int VEC = Scores<T, kHeld>::VEC;
+  double w = 0;
+  for (int i = threadIdx.x * VEC; i < sc.n; i += kThreads * VEC) w += row.template rough_pack<VEC>(sc, i);
+  return block_sum(static_cast<u64>(ldexp(w, row.lg_one)), s);
+}
+
+// The token from all scores at or ahead of the cut, by sums in index order.  Rough sums: false where the border
+// is too near.
+template <bool kExact, typename T, bool kHeld>
+__device__ __forceinline__ bool sweep(const Scores<T, kHeld>& sc, const Row& row, u64 cut, double u, int slot, int64_t* token,
+                                      float* x_token, bool* mine, Shared& s, cg::cluster_group& cl) {
+  constexpr int VEC = Scores<T, kHeld>::VEC, STEP = 32 * VEC;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const unsigned me = cl.block_rank();
+  const int span = (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;  // scores per warp, contiguous
+  const int i0 = min(sc.n, warp * span), i1 = min(sc.n, i0 + span);
+  const Cut kept(cut);
+  auto kept_weight = [&](float x, int i) {
+    const u64 w = kExact ? row.weight(x) : static_cast<u64>(ldexpf(row.rough(x), row.lg_one));
+    return kept.keeps(x, sc.first + i) ? w : 0ull;
+  };
+  u64 w = 0;
+  if constexpr (kExact) {
+    for (int i = i0 + lane * VEC; i < i1; i += STEP) {
+      float v[VEC];
+      sc.vec(i, v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w += kept_weight(v[e], i + e);
+    }
+  } else {
+    double r = 0;
+    if (cut == 0) {
+      for (int i = i0 + lane * VEC; i < i1; i += STEP) r += row.template rough_pack<VEC>(sc, i);
+    } else {
+      for (int i = i0 + lane * VEC; i < i1; i += STEP) {
+        float v[VEC], t = 0.f;
+        sc.vec(i, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) t += kept.keeps(v[e], sc.first + i + e) ? row.rough(v[e]) : 0.f;
+        r += static_cast<double>(t);
+      }
+    }
+    w = static_cast<u64>(ldexp(r, row.lg_one));
+  }
+  w = warp_sum(w);
+  __syncthreads();
+  if (lane == 0) s.part[warp] = w;
+  __syncthreads();
+  u64 own = 0;
+  for (int i = 0; i < kWarps; ++i) own += s.part[i];
+  if (threadIdx.x == 0) {
+    s.slot[slot] = own;
+    s.found[2] = 0;
+  }
+  cl.sync();
+  u64 ahead = 0, total = 0, v[kMaxCluster];
+  read_all(cl, v, [&](unsigned c) { return cl.map_shared_rank(&s.slot[slot], c); });
+#pragma unroll
+  for (unsigned c = 0; c < kMaxCluster; ++c) {
+    if (c < me) ahead += v[c];
+    total += v[c];
+  }
+  const u64 goal = goal_of(u, total), margin = kExact ? 0 : (total >> (kRoughBits - 1)) + 2;
+  for (int i = 0; i < warp; ++i) ahead += s.part[i];
+  if (ahead < goal && goal <= ahead + s.part[warp]) {  // this warp's range holds it
+    for (int i = i0 + lane * VEC; i - lane * VEC < i1; i += STEP) {
+      float v[VEC];
+      u64 we[VEC], sum = 0;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = -INFINITY;
+      if (i < i1) sc.vec(i, v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        we[e] = v[e] == -INFINITY ? 0 : kept_weight(v[e], i + e);
+        sum += we[e];
+      }
+      const u64 inc = warp_scan(sum);
+      const uint32_t reached = __ballot_sync(0xffffffffu, ahead + inc >= goal);
+      if (reached) {
+        if (lane == __ffs(reached) - 1) {
+          u64 at = ahead + inc - sum;
+          bool found = false;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            if (!found && at + we[e] >= goal) {
+              found = true;
+              if (kExact || (at + margin < goal && goal + margin < at + we[e])) {
+                *mine = true;
+                *token = sc.first + i + e;
+                *x_token = v[e];
+                if (!kExact) *cl.map_shared_rank(&s.found[2], 0) = 1;
+              }
+            }
+            at += we[e];
+          }
+        }
+        break;
+      }
+      ahead += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+  if (kExact) return true;
+  cl.sync();
+  return *cl.map_shared_rank(&s.found[2], 0) != 0;
+}
+
 template <typename T, bool kHeld>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -594,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   cg::cluster_group cl = cg::this_cluster();
   const unsigned C = cl.num_blocks(), me = cl.block_rank();
   const int64_t r = blockIdx.x / C, row_id = p.row0 + r;
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int tid = threadIdx.x;
   constexpr int VEC = Scores<T, kHeld>::VEC;
   const int64_t first = static_cast<int64_t>(me) * p.share;
   Scores<T, kHeld> sc;
@@ -604,6 +808,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   sc.first = static_cast<uint32_t>(first);
   sc.n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(p.share), p.V - first)));
   if (tid < 64) s.root[tid] = exp2(tid / 64.0);
+  // settings, while the scores are on their way
+  double temp = setting(p.T, row_id);
+  const bool greedy = !(temp > 0.0);
+  if (greedy) temp = 1.0;
+  const double top_p = setting(p.p, row_id), min_p = setting(p.m, row_id), u = load_d(p.u, p.u_dt, row_id);
+  const int64_t k = p.k_ptr ? (p.k_bits == 64 ? static_cast<const int64_t*>(p.k_ptr)[row_id]
+                                              : static_cast<int64_t>(static_cast<const int32_t*>(p.k_ptr)[row_id]))
+                            : p.k;
+  const bool by_k = k > 0 && k < p.V, by_p = top_p < 1.0, by_m = min_p > 0.0;
+  const double lm = by_m && !greedy ? log(min(min_p, 1.0)) : 0.0, invT = 1.0 / temp;
 
   // ---------------------------------------------------------------- scores in, the largest
   float t_top = -INFINITY;  // of this thread (fmaxf leaves NaN out)
@@ -636,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   }
   t_top += 0.f;
   Row row;
-  row.top = score_of(static_cast<uint32_t>(cluster_join<false>(block_max(order_of(t_top), s), 0, s, cl)));
+  row.top = score_of(static_cast<uint32_t>(cluster_join<false>(block_max32(order_of(t_top), s), 0, s, cl)));
   if (p.V == 0 || row.top == -INFINITY) {  // nothing to choose from
     if (me == 0 && tid == 0) {
       p.token[row_id] = -1;
@@ -645,16 +859,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     cl.sync();
     return;
   }
-  double temp = setting(p.T, row_id);
-  const bool greedy = !(temp > 0.0);
-  if (greedy) temp = 1.0;
-  row.invT = 1.0 / temp;
+  row.invT = invT;
   row.c64 = 64 * 1.4426950408889634 * row.invT;
   row.top_d = widen(row.top);
   row.lg_one = p.lg_one;
   row.reach = kReach * static_cast<float>(temp);
   row.per_bin = static_cast<float>(kBins) / row.reach;
   row.root = s.root;
+  row.c32 = static_cast<float>(1.4426950408889634 * row.invT);
+  row.rough_ok = p.V <= (1 << 20) && row.top < INFINITY && row.c32 > 1e-30f && row.c32 < 1e30f;
 
   int64_t token = 0;
   float x_token = row.top;
@@ -667,15 +880,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     token = index_of(cluster_join<false>(block_max(pl, s), 1, s, cl));
     mine = me == 0 && tid == 0;
   } else {
-    const int64_t k = p.k_ptr ? (p.k_bits == 64 ? static_cast<const int64_t*>(p.k_ptr)[row_id]
-                                                : static_cast<int64_t>(static_cast<const int32_t*>(p.k_ptr)[row_id]))
-                              : p.k;
-    const double top_p = setting(p.p, row_id), min_p = setting(p.m, row_id), u = load_d(p.u, p.u_dt, row_id);
-    const bool by_k = k > 0 && k < p.V, by_p = top_p < 1.0, by_m = min_p > 0.0;
     u64 cut = 0;  // kept: place >= cut
     if (by_m) {
       // the lowest score with exp((x - top) / T) >= min_p: the nearest float to the root, or a neighbour
-      const double lm = log(min(min_p, 1.0)), top = row.top;
+      const double top = row.top;
       auto keeps = [&](uint32_t o) { return (static_cast<double>(score_of(o)) - top) * row.invT >= lm || score_of(o) == row.top; };
       uint32_t o = order_of(static_cast<float>(top + temp * lm));
       const uint32_t o_top = order_of(row.top), o_low = order_of(-INFINITY) + 1;
@@ -687,44 +895,55 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     // -------------------------------------------------------------- few tokens left
     bool done = false;
     if (by_m || (by_k ? static_cast<u64>(k) <= min(kThreads * C / 2, kList / 2) : by_p)) {
-      float reach_x = -INFINITY;  // a score that every token which may be kept reaches
-      bool few = true;
-      u64 total = 0;
+      u64 lo = 0, hi = 0;  // the row's weight, for top-p without top-k
+      bool exact = false;
       if (by_k || by_p) {
         clear_bins(false, s);
         if (t_top != -INFINITY && row.live(t_top)) atomicAdd(&s.count[row.bin(t_top)], 1u);
         if (!by_k) {
-          u64 w = 0;
-          sc.each([&](float x, int i) { w += row.weight(x); });
-          total = cluster_join<true>(block_sum(w, s), 2, s, cl);
+          if (row.rough_ok) {
+            const u64 w = cluster_join<true>(rough_total(sc, row, s), 2, s, cl);
+            lo = w - (w >> kRoughBits) - 1;
+            hi = w + (w >> kRoughBits) + 1;
+          } else {
+            exact = true;
+            lo = hi = cluster_join<true>(exact_total(sc, row, s), 2, s, cl);
+          }
         }
         merge_bins(false, s, cl);
-        find_bin<true>(by_k ? static_cast<u64>(k) : min(256u, kThreads * C / 2), s);
-        const int b = static_cast<int>(s.found[0]);
-        // the lower end of that bin, less what rounding may have moved; fewer live threads than asked for: all that
-        // have weight
-        const float d = b < kBins - 1 ? (b + 1) / row.per_bin * 1.000001f : row.reach;
-        reach_x = score_of(max(order_of(row.top - d), order_of(-INFINITY) + 2) - 2);
-        if (by_k && b == kBins) few = false;
       }
-      if (by_m && !(by_k && by_p)) reach_x = fmaxf(reach_x, Cut(cut).x);  // (top-p after top-k weighs the first k)
-      if (few) {
-        const uint32_t m = gather(sc, row, [&](float x, int i) { return x >= reach_x && row.live(x); }, s, cl);
-        if (m <= kList) {
-          const bool all = by_k || !by_p || reach_x == Cut(cut).x;
-          if (me == 0) {
-            done = choose_from_list(static_cast<int>(m), by_k, static_cast<u64>(k), by_p, top_p, total, all, cut, u, &token,
-                                    &x_token, &mine, s);
-            if (tid == 0) s.slot[3] = done;
-          }
-          if (all) {
-            done = true;
-          } else {
-            if (C > 1) cl.sync();
-            else __syncthreads();
-            done = *cl.map_shared_rank(&s.slot[3], 0) != 0;
-          }
+      // a nucleus is looked for among the 48 largest threads' scores, then among more
+      const u64 most = min(kThreads * C / 2, 384u);
+      for (u64 wanted = by_k ? static_cast<u64>(k) : min(48ull, most);; wanted = most) {
+        float reach_x = -INFINITY;  // a score that every token which may be kept reaches
+        if (by_k || by_p) {
+          find_bin<true>(wanted, s);
+          const int b = static_cast<int>(s.found[0]);
+          if (by_k && b == kBins) break;  // fewer threads have live scores
+          // the lower end of that bin, less what rounding may have moved
+          const float d = b < kBins - 1 ? (b + 1) / row.per_bin * 1.000001f : row.reach;
+          reach_x = score_of(max(order_of(row.top - d), order_of(-INFINITY) + 2) - 2);
         }
+        if (by_m && !(by_k && by_p)) reach_x = fmaxf(reach_x, Cut(cut).x);  // (top-p after top-k weighs the first k)
+        const uint32_t m = gather(sc, row, [&](float x, int i) { return x >= reach_x && row.live(x); }, s, cl);
+        if (m > kList) break;
+        const bool all = by_k || !by_p || reach_x == Cut(cut).x;
+        Found f = kFound;
+        for (int at = 3;; ++at) {  // slots 3, 4 in the first round, 6, 7 in the second
+          if (me == 0)
+            f = choose_from_list(static_cast<int>(m), by_k, static_cast<u64>(k), by_p, top_p, lo, hi, all, cut, u, &token,
+                                 &x_token, &mine, s);
+          if (!by_p || by_k) break;  // always found
+          const int slot = wanted == most && most > 48 ? at + 3 : at;
+          if (tid == 0 && me == 0) s.slot[slot] = f;
+          cl.sync();
+          f = static_cast<Found>(*cl.map_shared_rank(&s.slot[slot], 0));
+          if (f != kUnsure || exact) break;
+          exact = true;
+          lo = hi = cluster_join<true>(exact_total(sc, row, s), 9, s, cl);
+        }
+        if (f == kFound) done = true;
+        if (done || wanted == most) break;
       }
     }
     // -------------------------------------------------------------- many
@@ -733,77 +952,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         const u64 c = thresholds(sc, row, by_k, static_cast<u64>(k), by_p, top_p, s, cl);
         cut = c > cut ? c : cut;
       }
-      constexpr int STEP = 32 * VEC;
-      const int span = (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;  // scores per warp, contiguous
-      const int i0 = min(sc.n, warp * span), i1 = min(sc.n, i0 + span);
-      const Cut kept(cut);
-      auto kept_weight = [&](float x, int i) {
-        const u64 w = row.weight(x);
-        return kept.keeps(x, sc.first + i) ? w : 0ull;
-      };
-      u64 w = 0;
-      for (int i = i0 + lane * VEC; i < i1; i += STEP) {
-        float v[VEC];
-        sc.vec(i, v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) w += kept_weight(v[e], i + e);
-      }
-      w = warp_sum(w);
-      __syncthreads();
-      if (lane == 0) s.part[warp] = w;
-      __syncthreads();
-      u64 own = 0;
-      for (int i = 0; i < kWarps; ++i) own += s.part[i];
-      if (tid == 0) s.slot[4] = own;
-      cl.sync();
-      u64 ahead = 0, total = 0;
-      for (unsigned c = 0; c < C; ++c) {
-        const u64 o = *cl.map_shared_rank(&s.slot[4], c);
-        if (c < me) ahead += o;
-        total += o;
-      }
-      const u64 goal = goal_of(u, total);
-      for (int i = 0; i < warp; ++i) ahead += s.part[i];
-      if (ahead < goal && goal <= ahead + s.part[warp]) {  // this warp's range holds it
-        for (int i = i0 + lane * VEC; i - lane * VEC < i1; i += STEP) {
-          float v[VEC];
-          u64 we[VEC], sum = 0;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) v[e] = -INFINITY;
-          if (i < i1) sc.vec(i, v);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            we[e] = kept_weight(v[e], i + e);
-            sum += we[e];
-          }
-          const u64 inc = warp_scan(sum);
-          const uint32_t reached = __ballot_sync(0xffffffffu, ahead + inc >= goal);
-          if (reached) {
-            if (lane == __ffs(reached) - 1) {
-              u64 at = ahead + inc - sum;
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) {
-                if (!mine && at + we[e] >= goal && we[e] != 0) {
-                  mine = true;
-                  token = sc.first + i + e;
-                  x_token = v[e];
-                }
-                at += we[e];
-              }
-            }
-            break;
-          }
-          ahead += __shfl_sync(0xffffffffu, inc, 31);
-        }
-      }
+      if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 8, &token, &x_token, &mine, s, cl))
+        sweep<true>(sc, row, cut, u, 5, &token, &x_token, &mine, s, cl);
     }
   }
   if (mine) p.token[row_id] = token;
   if (p.logprob) {
     // log softmax(x / T) of the token over the whole row
-    u64 w = 0;
-    sc.each([&](float x, int i) { w += row.weight(x); });
-    const u64 all = cluster_join<true>(block_sum(w, s), 5, s, cl);
+    const u64 all = cluster_join<true>(exact_total(sc, row, s), 12, s, cl);
     if (mine)
       p.logprob[row_id] = static_cast<float>((x_token == row.top ? 0.0 : (static_cast<double>(x_token) - row.top) * row.invT) -
                                              log(ldexp(static_cast<double>(all), -row.lg_one)));
@@ -817,6 +973,7 @@ constexpr size_t kSmemMax = 227 * 1024;
 template <typename T>
 static cudaError_t launch_t(Params p, cudaStream_t st) {
   constexpr int64_t most = static_cast<int64_t>((kSmemMax - sizeof(Shared)) / sizeof(T) / 32 * 32);
+  static_assert(kMaxCluster == 8, "cluster sizes below");
   constexpr int64_t pair = static_cast<int64_t>((kSmemMax / 2 - 1024 - sizeof(Shared)) / sizeof(T) / 32 * 32);
   // the smallest cluster whose CTAs hold the row, two of them an SM; few rows take more, to spread over the SMs
   int C = 1;
