@@ -48,6 +48,8 @@ constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
 constexpr float kReach = 30.5f;  // e^-30.5 < 2^-44
 constexpr int kRoughBits = 18;   // fp32 sums are within 2^-18 of the total
+constexpr int kRoughOne = 40;    // and are kept in units of 2^-40 of the largest weight: 2^60 at most,
+constexpr u64 kRoughNan = 1ull << 60;  // what a CTA that met NaN posts instead (the fixed-point sums leave NaN out)
 
 struct Setting {  // one value for all rows, or one per row
   const void* ptr;
@@ -130,7 +132,7 @@ struct alignas(16) Shared {  // the scores held behind it are stored 16 bytes at
   u64 list[kList], list_w[kList];
   double root[64];        // 2^(j / 64)
   u64 part[kWarps];       // per-warp results of a block reduction or scan
-  u64 slot[13];           // values other CTAs of the cluster read, each written once
+  u64 slot[14];           // values other CTAs of the cluster read, each written once
   u64 found[3];           // boundary bin, and count or weight before it
   uint32_t n_list;
 
@@ -164,11 +166,11 @@ struct Row {
   float c32;      // log2(e) / T
 
   __device__ __forceinline__ float rough(float x) const { return ex2((x - top) * c32); }
-  // the sum over a pack of scores
+  // the sum over a pack of scores; NaN where one of them is
   template <int VEC, typename S>
   __device__ __forceinline__ double rough_pack(const S& sc, int i) const {
     float v[VEC];
-    sc.vec(i, v);
+    sc.raw(i, v);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = rough(v[e]);
 #pragma unroll
@@ -197,6 +199,9 @@ struct Row {
     const u64 w = static_cast<u64>(__double_as_longlong(v + 4503599627370496.0)) & 0xfffffffffffffull;
     return x == top ? 1ull << lg_one : (top - x < reach ? w : 0ull);
   }
+  // a score d below the largest, or a little further; above -inf
+  __device__ __forceinline__ float below(float d) const { return score_of(max(order_of(top - d), order_of(-INFINITY) + 3) - 2); }
+  __device__ __forceinline__ float floor_x() const { return below(reach); }  // scores below it have no weight
   // rises as x falls: subtraction, product and conversion are all monotone
   __device__ __forceinline__ int bin(float x) const {
     return x == top ? 0 : min(kBins - 1, static_cast<int>((top - x) * per_bin));
@@ -237,6 +242,18 @@ struct Scores {
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[k] = i + k < n ? at(i + k) : -INFINITY;
+    }
+  }
+  // VEC scores as they are: NaN as NaN, -0 as -0
+  __device__ __forceinline__ void raw(int i, float (&v)[VEC]) const {
+    if ((kHeld || aligned) && i + VEC <= n) {
+      struct alignas(16) P { T e[VEC]; };
+      const P p = *reinterpret_cast<const P*>((kHeld ? held : x) + i);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = to_float(p.e[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = i + k < n ? to_float(kHeld ? held[i + k] : x[i + k]) : -INFINITY;
     }
   }
   // f(score, index within the CTA) for every score, in no order
@@ -416,28 +433,32 @@ enum Found { kFound = 1, kNotListed, kUnsure };
 // [total_lo, total_hi] holds the weight that top-p refers to (total_hi = 0: that of the first k).  `all`: the list is
 // known to hold the whole nucleus; otherwise kNotListed is returned when it does not.  kUnsure: tokens are kept or not
 // depending on where in the range the total lies; the list is as it was.
-// Up to 64 entries are ranked by comparing each with all others (512 / n threads an entry), more are sorted.
+// Up to 256 entries are ranked by comparing each with all others (512 / m threads an entry), more are sorted.
 __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool by_p, double top_p, u64 total_lo, u64 total_hi,
                                                   bool all, u64 cut, double u, int64_t* token, float* x_token, bool* mine,
                                                   Shared& s) {
-  int n = 32;
-  while (n < m) n <<= 1;
-  for (int i = m + threadIdx.x; i < n; i += kThreads) s.list[i] = 0, s.list_w[i] = 0;
-  __syncthreads();
-  if (n <= 64) {
-    const int G = kThreads / n, i = threadIdx.x / G, g = threadIdx.x % G;  // G lanes of a warp share entry i
-    const u64 pl = s.list[i];
-    u64 w = s.list_w[i], ahead = 0;
+  if (m <= 256) {
+    int G = 1;  // lanes that share an entry
+    while (2 * G * m <= kThreads && G < 16) G *= 2;
+    const int i = threadIdx.x / G, g = threadIdx.x % G;
+    const bool have = i < m;
+    const u64 pl = have ? s.list[i] : ~0ull;
+    u64 w = have ? s.list_w[i] : 0, ahead = 0;
     uint32_t rank = 0;
+    if (have) {
 #pragma unroll 4
-    for (int j = g; j < n; j += G) {
-      const u64 o = s.list[j], ow = s.list_w[j];
-      rank += o > pl;
-      ahead += o > pl ? ow : 0;
+      for (int j = g; j < m; j += G) {
+        const u64 o = s.list[j];
+        if (by_p) {
+          const u64 ow = s.list_w[j];
+          ahead += o > pl ? ow : 0;
+        }
+        rank += o > pl;
+      }
     }
     for (int o = 1; o < G; o <<= 1) {
       rank += __shfl_xor_sync(0xffffffffu, rank, o);
-      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+      if (by_p) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
     }
     if (by_k && rank >= k) w = 0;  // what is ahead of the others is unchanged: it ranks behind them
     if (by_p) {
@@ -447,25 +468,37 @@ __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool 
       if (lo != hi && __syncthreads_or(w != 0 && ahead >= lo && ahead < hi)) return kUnsure;
       if (ahead >= lo) w = 0;
     }
-    if (pl < cut) w = 0;
-    __syncthreads();  // everyone has read the weights
-    if (g == 0) s.list_w[i] = w;
-    const u64 goal = goal_of(u, block_sum(g == 0 ? w : 0, s));  // its barriers order the weights too
-    const uint32_t low = static_cast<uint32_t>(pl);             // complemented index: a larger one comes first
-    u64 run = 0;
-#pragma unroll 4
-    for (int j = g; j < n; j += G) {
-      const u64 ow = s.list_w[j];
-      run += static_cast<uint32_t>(s.list[j]) > low ? ow : 0;
+    if (pl < cut || g != 0) w = 0;
+    if (threadIdx.x == 0) s.n_list = 0;
+    const u64 goal = goal_of(u, block_sum(w, s));  // its barriers: the list has been read, the count is 0
+    if (w != 0) {  // kept ones move together
+      const uint32_t j = atomicAdd(&s.n_list, 1u);
+      s.list[j] = pl;
+      s.list_w[j] = w;
     }
-    for (int o = 1; o < G; o <<= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
-    if (g == 0 && run < goal && goal <= run + w) {
-      *token = index_of(pl);
-      *x_token = score_of(static_cast<uint32_t>(pl >> 32));
-      *mine = true;
+    __syncthreads();
+    const uint32_t kept = s.n_list;
+    for (uint32_t e = threadIdx.x; e < kept; e += kThreads) {
+      const u64 mine_pl = s.list[e];
+      const uint32_t low = static_cast<uint32_t>(mine_pl);  // complemented index: a larger one comes first
+      u64 run = 0;
+#pragma unroll 4
+      for (uint32_t j = 0; j < kept; ++j) {
+        const u64 ow = s.list_w[j];
+        run += static_cast<uint32_t>(s.list[j]) > low ? ow : 0;
+      }
+      if (run < goal && goal <= run + s.list_w[e]) {
+        *token = index_of(mine_pl);
+        *x_token = score_of(static_cast<uint32_t>(mine_pl >> 32));
+        *mine = true;
+      }
     }
     return kFound;
   }
+  int n = 512;
+  while (n < m) n <<= 1;
+  for (int i = m + threadIdx.x; i < n; i += kThreads) s.list[i] = 0, s.list_w[i] = 0;
+  __syncthreads();
   constexpr int PER = kList / kThreads;
   sort_list(n, s);
   // entries of this thread: consecutive ones, so that prefix sums follow the order
@@ -534,17 +567,29 @@ __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool 
   return kFound;
 }
 
-// Gathers in CTA 0 the places and weights of the scores that pass; returns their number, which may be over
+// Gathers in CTA 0 the places and weights of the scores that reach reach_x; returns their number, which may be over
 // kList (then there is no list).  Each CTA lists its own first: a remote append per token would cost a round trip each.
+// reach_x is above -inf; `also` narrows further.
 template <typename T, bool kHeld, typename F>
-__device__ __forceinline__ uint32_t gather(const Scores<T, kHeld>& sc, const Row& row, F pass, Shared& s, cg::cluster_group& cl) {
+__device__ __forceinline__ uint32_t gather(const Scores<T, kHeld>& sc, const Row& row, float reach_x, F also, Shared& s,
+                                           cg::cluster_group& cl) {
+  constexpr int VEC = Scores<T, kHeld>::VEC;
   if (threadIdx.x == 0) s.n_list = 0;
   __syncthreads();
-  sc.each([&](float x, int i) {
-    if (!pass(x, i)) return;
-    const uint32_t j = atomicAdd(&s.n_list, 1u);
-    if (j < kList) s.list[j] = place_of(x, sc.first + i);
-  });
+  for (int i = threadIdx.x * VEC; i < sc.n; i += kThreads * VEC) {
+    float v[VEC], most = -INFINITY;
+    sc.raw(i, v);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) most = fmaxf(most, v[k]);
+    if (!(most >= reach_x)) continue;  // most packs
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      if (v[k] >= reach_x && also(v[k] + 0.f, i + k)) {
+        const uint32_t j = atomicAdd(&s.n_list, 1u);
+        if (j < kList) s.list[j] = place_of(v[k] + 0.f, sc.first + i + k);
+      }
+    }
+  }
   cl.sync();
   u64 n[kMaxCluster];
   read_all(cl, n, [&](unsigned c) { return cl.map_shared_rank(&s.n_list, c); });
@@ -584,7 +629,7 @@ __device__ __noinline__ u64 boundary(const Scores<T, kHeld>& sc, const Row& row,
     return pl >= lo && pl <= hi;
   };
   while (true) {
-    const uint32_t m = gather(sc, row, member, s, cl);
+    const uint32_t m = gather(sc, row, row.floor_x(), member, s, cl);
     if (m <= kList) {
       if (cl.block_rank() == 0) {
         u64 low = ~0ull;
@@ -614,10 +659,10 @@ __device__ __noinline__ u64 boundary(const Scores<T, kHeld>& sc, const Row& row,
     least = ~block_max(~least, s);
     most = block_max(most, s);
     cl.sync();
-    if (threadIdx.x == 0) s.slot[10] = least, s.slot[11] = most;
+    if (threadIdx.x == 0) s.slot[10] = least, s.slot[13] = most;
     cl.sync();
     for (unsigned r = 0; r < cl.num_blocks(); ++r) {
-      const u64 a = *cl.map_shared_rank(&s.slot[10], r), b = *cl.map_shared_rank(&s.slot[11], r);
+      const u64 a = *cl.map_shared_rank(&s.slot[10], r), b = *cl.map_shared_rank(&s.slot[13], r);
       least = a < least ? a : least;
       most = b > most ? b : most;
     }
@@ -682,12 +727,15 @@ __device__ __forceinline__ u64 exact_total(const Scores<T, kHeld>& sc, const Row
   sc.each([&](float x, int i) { w += row.weight(x); });
   return block_sum(w, s);
 }
+__device__ __forceinline__ u64 rough_units(double w) { return w == w ? static_cast<u64>(ldexp(w, kRoughOne)) : 0; }
 template <typename T, bool kHeld>
 __device__ __forceinline__ u64 rough_total(const Scores<T, kHeld>& sc, const Row& row, Shared& s) {
   constexpr int VEC = Scores<T, kHeld>::VEC;
   double w = 0;
   for (int i = threadIdx.x * VEC; i < sc.n; i += kThreads * VEC) w += row.template rough_pack<VEC>(sc, i);
-  return block_sum(static_cast<u64>(ldexp(w, row.lg_one)), s);
+  const bool nan = __syncthreads_or(w != w);
+  const u64 sum = block_sum(rough_units(w), s);
+  return nan ? kRoughNan : sum;
 }
 
 // The token from all scores at or ahead of the cut, by sums in index order.  Rough sums: false where the border
@@ -702,10 +750,11 @@ __device__ __forceinline__ bool sweep(const Scores<T, kHeld>& sc, const Row& row
   const int i0 = min(sc.n, warp * span), i1 = min(sc.n, i0 + span);
   const Cut kept(cut);
   auto kept_weight = [&](float x, int i) {
-    const u64 w = kExact ? row.weight(x) : static_cast<u64>(ldexpf(row.rough(x), row.lg_one));
+    const u64 w = kExact ? row.weight(x) : static_cast<u64>(ldexpf(row.rough(x), kRoughOne));
     return kept.keeps(x, sc.first + i) ? w : 0ull;
   };
   u64 w = 0;
+  bool row_nan = false;
   if constexpr (kExact) {
     for (int i = i0 + lane * VEC; i < i1; i += STEP) {
       float v[VEC];
@@ -726,14 +775,16 @@ __device__ __forceinline__ bool sweep(const Scores<T, kHeld>& sc, const Row& row
         r += static_cast<double>(t);
       }
     }
-    w = static_cast<u64>(ldexp(r, row.lg_one));
+    w = rough_units(r);
+    if (r != r) row_nan = true;
   }
   w = warp_sum(w);
-  __syncthreads();
+  const bool nan = __syncthreads_or(row_nan);
   if (lane == 0) s.part[warp] = w;
   __syncthreads();
   u64 own = 0;
   for (int i = 0; i < kWarps; ++i) own += s.part[i];
+  if (nan) own = kRoughNan;
   if (threadIdx.x == 0) {
     s.slot[slot] = own;
     s.found[2] = 0;
@@ -746,6 +797,7 @@ __device__ __forceinline__ bool sweep(const Scores<T, kHeld>& sc, const Row& row
     if (c < me) ahead += v[c];
     total += v[c];
   }
+  if (!kExact && total >= kRoughNan) return false;  // the same for every CTA
   const u64 goal = goal_of(u, total), margin = kExact ? 0 : (total >> (kRoughBits - 1)) + 2;
   for (int i = 0; i < warp; ++i) ahead += s.part[i];
   if (ahead < goal && goal <= ahead + s.part[warp]) {  // this warp's range holds it
@@ -901,13 +953,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         clear_bins(false, s);
         if (t_top != -INFINITY && row.live(t_top)) atomicAdd(&s.count[row.bin(t_top)], 1u);
         if (!by_k) {
-          if (row.rough_ok) {
-            const u64 w = cluster_join<true>(rough_total(sc, row, s), 2, s, cl);
-            lo = w - (w >> kRoughBits) - 1;
-            hi = w + (w >> kRoughBits) + 1;
+          u64 w = row.rough_ok ? cluster_join<true>(rough_total(sc, row, s), 2, s, cl) : kRoughNan;
+          if (w < kRoughNan) {
+            lo = (w - (w >> kRoughBits) - 1) << (row.lg_one - kRoughOne);
+            hi = (w + (w >> kRoughBits) + 1) << (row.lg_one - kRoughOne);
           } else {
+            row.rough_ok = false;
             exact = true;
-            lo = hi = cluster_join<true>(exact_total(sc, row, s), 2, s, cl);
+            lo = hi = cluster_join<true>(exact_total(sc, row, s), 8, s, cl);
           }
         }
         merge_bins(false, s, cl);
@@ -915,19 +968,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
       // a nucleus is looked for among the 48 largest threads' scores, then among more
       const u64 most = min(kThreads * C / 2, 384u);
       for (u64 wanted = by_k ? static_cast<u64>(k) : min(48ull, most);; wanted = most) {
-        float reach_x = -INFINITY;  // a score that every token which may be kept reaches
+        float reach_x = row.floor_x();  // a score that every token which may be kept reaches
         if (by_k || by_p) {
           find_bin<true>(wanted, s);
           const int b = static_cast<int>(s.found[0]);
           if (by_k && b == kBins) break;  // fewer threads have live scores
           // the lower end of that bin, less what rounding may have moved
-          const float d = b < kBins - 1 ? (b + 1) / row.per_bin * 1.000001f : row.reach;
-          reach_x = score_of(max(order_of(row.top - d), order_of(-INFINITY) + 2) - 2);
+          if (b < kBins - 1) reach_x = fmaxf(reach_x, row.below((b + 1) / row.per_bin * 1.000001f));
         }
         if (by_m && !(by_k && by_p)) reach_x = fmaxf(reach_x, Cut(cut).x);  // (top-p after top-k weighs the first k)
-        const uint32_t m = gather(sc, row, [&](float x, int i) { return x >= reach_x && row.live(x); }, s, cl);
+        const uint32_t m = gather(sc, row, reach_x, [](float, int) { return true; }, s, cl);
         if (m > kList) break;
-        const bool all = by_k || !by_p || reach_x == Cut(cut).x;
+        const bool all = by_k || !by_p || reach_x == row.floor_x() || reach_x == Cut(cut).x;
         Found f = kFound;
         for (int at = 3;; ++at) {  // slots 3, 4 in the first round, 6, 7 in the second
           if (me == 0)
@@ -952,7 +1004,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         const u64 c = thresholds(sc, row, by_k, static_cast<u64>(k), by_p, top_p, s, cl);
         cut = c > cut ? c : cut;
       }
-      if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 8, &token, &x_token, &mine, s, cl))
+      if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 11, &token, &x_token, &mine, s, cl))
         sweep<true>(sc, row, cut, u, 5, &token, &x_token, &mine, s, cl);
     }
   }
