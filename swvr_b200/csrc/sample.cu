@@ -10,10 +10,11 @@
 // point, 2^44 for the largest (2^(62 - log2 V) where V is past 2^18), so sums are exact in any order, by any number of
 // threads.  Weights below 2^-44 of the largest are 0 (30.5 T below the maximum).
 //
-// A row is a cluster of 1 .. 8 CTAs, each holding a contiguous share of the scores in shared memory, in
-// their own type, so the scores are read from global memory once; longer rows are read again in each
-// pass.  The usual filters leave few tokens, and those are found without a weight or a bin for every score:
-//   1. scores in, the largest, and each thread's largest;
+// A row is a cluster of 1 .. 8 CTAs, each with a contiguous share of the scores.  They are read from global memory in
+// every pass: after the first they are in L2, and shared memory full of scores would leave one CTA an SM (measured
+// on 256 rows of 128256 bf16: 92 us held, see below for what it takes now).  The usual filters leave few tokens, and
+// those are found without a weight or a bin for every score:
+//   1. the largest score, and each thread's largest;
 //   2. a score that enough tokens reach: for top-k, the k-th of the threads' largest scores (k tokens are at
 //      least that large, and few more are, as long as k is well below the number of threads); for a top-p
 //      without top-k the 256-th of them, beside the weight of the whole row; min-p knows its own;
@@ -25,10 +26,12 @@
 // index order, and the warp whose range holds u rescans it.
 //
 // Sums over all scores (the row's weight for top-p, the last pass) are first taken with fp32 weights, an eighth of the
-// instructions.  A weight 2^y, y <= 0 in octaves, is then off by |y| 3 2^-24 ln 2 + 2^-22 relatively at most, and the weighted
-// mean of |y| is at most the distribution's entropy, so no partial sum is off by more than d = 2^-18 of the
-// total (V up to 2^20).  Where what is decided lies more than that from its border (2 d: both the running weight and the
-// total may be off) the fixed-point sums would decide the same; otherwise, a few rows in a hundred, they are taken.
+// instructions.  A weight 2^y, y <= 0 in octaves, is then off by |y| 2 2^-24 ln 2 (difference and product rounded, the
+// factor in two parts) + 2^-22 (ex2) + 3 2^-24 (sums) relatively at most, and the weighted mean of |y| is at most the
+// distribution's entropy, log2 V: no partial sum is off by more than d = 2^-19 of the total up to V = 200000,
+// 2^-18 up to 2^20.  Where what is decided lies more than that from its border (2 d: both the running
+// weight and the total may be off) the fixed-point sums would decide the same; otherwise, a few rows in a
+// hundred, they are taken.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -47,8 +50,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
 constexpr float kReach = 30.5f;  // e^-30.5 < 2^-44
-constexpr int kRoughBits = 18;   // fp32 sums are within 2^-18 of the total
-constexpr int kRoughOne = 40;    // and are kept in units of 2^-40 of the largest weight: 2^60 at most,
+constexpr int kRoughOne = 40;    // fp32 sums are kept in units of 2^-40 of the largest weight: 2^60 at most,
 constexpr u64 kRoughNan = 1ull << 60;  // what a CTA that met NaN posts instead (the fixed-point sums leave NaN out)
 
 struct Setting {  // one value for all rows, or one per row
@@ -125,7 +127,7 @@ struct Cut {
   __device__ __forceinline__ bool keeps(float v, uint32_t i) const { return v > x || (v == x && i <= index); }
 };
 
-struct alignas(16) Shared {  // the scores held behind it are stored 16 bytes at a time
+struct Shared {
   u64 mass_all[kBins];
   uint32_t count_all[kBins];
   uint32_t count[kBins], mass_lo[kBins], mass_hi[kBins];
@@ -152,8 +154,6 @@ __device__ __forceinline__ double widen(float x) {
   return (b & 0x7f800000u) == 0 ? 0.0 : v;
 }
 
-static_assert(sizeof(Shared) % 16 == 0, "alignment of the scores behind it");
-
 struct Row {
   float top;      // the largest score
   double top_d, c64;  // top, and 64 log2(e) / T
@@ -163,9 +163,13 @@ struct Row {
   float per_bin;  // bins per unit of score
   const double* root;
   bool rough_ok;  // fp32 weights are within their bound
-  float c32;      // log2(e) / T
+  int rough_bits; // 18 or 19
+  float c32, c32_lo;  // log2(e) / T in two parts
 
-  __device__ __forceinline__ float rough(float x) const { return ex2((x - top) * c32); }
+  __device__ __forceinline__ float rough(float x) const {
+    const float d = x - top;
+    return ex2(fmaf(d, c32, d * c32_lo));
+  }
   // the sum over a pack of scores; NaN where one of them is
   template <int VEC, typename S>
   __device__ __forceinline__ double rough_pack(const S& sc, int i) const {
@@ -221,22 +225,21 @@ __device__ __forceinline__ float to_score(T v) {
   return f != f ? -INFINITY : f + 0.f;
 }
 
-// This CTA's scores: in shared memory (kHeld), or where they are.
-template <typename T, bool kHeld>
+// This CTA's scores.
+template <typename T>
 struct Scores {
   static constexpr int VEC = 16 / sizeof(T);
   const T* x;      // this CTA's first score
-  const T* held;
   bool aligned;
   int n;
   uint32_t first;  // its index in the row
 
-  __device__ __forceinline__ float at(int i) const { return to_score(kHeld ? held[i] : x[i]); }
+  __device__ __forceinline__ float at(int i) const { return to_score(x[i]); }
   // VEC scores from i on (i a multiple of VEC); -inf past the end
   __device__ __forceinline__ void vec(int i, float (&v)[VEC]) const {
-    if ((kHeld || aligned) && i + VEC <= n) {
+    if (aligned && i + VEC <= n) {
       struct alignas(16) P { T e[VEC]; };
-      const P p = *reinterpret_cast<const P*>((kHeld ? held : x) + i);
+      const P p = *reinterpret_cast<const P*>(x + i);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[k] = to_score(p.e[k]);
     } else {
@@ -246,14 +249,14 @@ struct Scores {
   }
   // VEC scores as they are: NaN as NaN, -0 as -0
   __device__ __forceinline__ void raw(int i, float (&v)[VEC]) const {
-    if ((kHeld || aligned) && i + VEC <= n) {
+    if (aligned && i + VEC <= n) {
       struct alignas(16) P { T e[VEC]; };
-      const P p = *reinterpret_cast<const P*>((kHeld ? held : x) + i);
+      const P p = *reinterpret_cast<const P*>(x + i);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[k] = to_float(p.e[k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = i + k < n ? to_float(kHeld ? held[i + k] : x[i + k]) : -INFINITY;
+      for (int k = 0; k < VEC; ++k) v[k] = i + k < n ? to_float(x[i + k]) : -INFINITY;
     }
   }
   // f(score, index within the CTA) for every score, in no order
@@ -570,10 +573,10 @@ __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool 
 // Gathers in CTA 0 the places and weights of the scores that reach reach_x; returns their number, which may be over
 // kList (then there is no list).  Each CTA lists its own first: a remote append per token would cost a round trip each.
 // reach_x is above -inf; `also` narrows further.
-template <typename T, bool kHeld, typename F>
-__device__ __forceinline__ uint32_t gather(const Scores<T, kHeld>& sc, const Row& row, float reach_x, F also, Shared& s,
+template <typename T, typename F>
+__device__ __forceinline__ uint32_t gather(const Scores<T>& sc, const Row& row, float reach_x, F also, Shared& s,
                                            cg::cluster_group& cl) {
-  constexpr int VEC = Scores<T, kHeld>::VEC;
+  constexpr int VEC = Scores<T>::VEC;
   if (threadIdx.x == 0) s.n_list = 0;
   __syncthreads();
   for (int i = threadIdx.x * VEC; i < sc.n; i += kThreads * VEC) {
@@ -618,8 +621,8 @@ __device__ __forceinline__ uint32_t gather(const Scores<T, kHeld>& sc, const Row
 
 // The lowest kept place when tokens are kept while what is ahead of them (their number, or their weight) is
 // below goal; `bin` holds the boundary and `before` is ahead of it.
-template <bool kByCount, typename T, bool kHeld>
-__device__ __noinline__ u64 boundary(const Scores<T, kHeld>& sc, const Row& row, int bin, u64 before, u64 goal, Shared& s,
+template <bool kByCount, typename T>
+__device__ __noinline__ u64 boundary(const Scores<T>& sc, const Row& row, int bin, u64 before, u64 goal, Shared& s,
                                      cg::cluster_group& cl) {
   u64 lo = 0, hi = ~0ull;  // places of the members still in question
   Shared* s0 = cl.map_shared_rank(&s, 0);
@@ -686,8 +689,8 @@ __device__ __noinline__ u64 boundary(const Scores<T, kHeld>& sc, const Row& row,
 }
 
 // The lowest kept place of top-k and top-p, whatever they leave.
-template <typename T, bool kHeld>
-__device__ __noinline__ u64 thresholds(const Scores<T, kHeld>& sc, const Row& row, bool by_k, u64 k, bool by_p, double top_p,
+template <typename T>
+__device__ __noinline__ u64 thresholds(const Scores<T>& sc, const Row& row, bool by_k, u64 k, bool by_p, double top_p,
                                        Shared& s, cg::cluster_group& cl) {
   u64 cut = 0;
   if (by_k) {
@@ -721,50 +724,46 @@ __device__ __noinline__ u64 thresholds(const Scores<T, kHeld>& sc, const Row& ro
 }
 
 // The weight of this CTA's scores, in units of 2^-lg_one of the largest: in fixed point, or from fp32 weights.
-template <typename T, bool kHeld>
-__device__ __forceinline__ u64 exact_total(const Scores<T, kHeld>& sc, const Row& row, Shared& s) {
+template <typename T>
+__device__ __forceinline__ u64 exact_total(const Scores<T>& sc, const Row& row, Shared& s) {
   u64 w = 0;
   sc.each([&](float x, int i) { w += row.weight(x); });
   return block_sum(w, s);
 }
 __device__ __forceinline__ u64 rough_units(double w) { return w == w ? static_cast<u64>(ldexp(w, kRoughOne)) : 0; }
-template <typename T, bool kHeld>
-__device__ __forceinline__ u64 rough_total(const Scores<T, kHeld>& sc, const Row& row, Shared& s) {
-  constexpr int VEC = Scores<T, kHeld>::VEC;
+template <typename T>
+__device__ __forceinline__ u64 rough_total(const Scores<T>& sc, const Row& row, Shared& s) {
+  constexpr int VEC = Scores<T>::VEC;
   double w = 0;
+#pragma unroll 2
   for (int i = threadIdx.x * VEC; i < sc.n; i += kThreads * VEC) w += row.template rough_pack<VEC>(sc, i);
   const bool nan = __syncthreads_or(w != w);
   const u64 sum = block_sum(rough_units(w), s);
   return nan ? kRoughNan : sum;
 }
 
-// The token from all scores at or ahead of the cut, by sums in index order.  Rough sums: false where the border
-// is too near.
-template <bool kExact, typename T, bool kHeld>
-__device__ __forceinline__ bool sweep(const Scores<T, kHeld>& sc, const Row& row, u64 cut, double u, int slot, int64_t* token,
-                                      float* x_token, bool* mine, Shared& s, cg::cluster_group& cl) {
-  constexpr int VEC = Scores<T, kHeld>::VEC, STEP = 32 * VEC;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const unsigned me = cl.block_rank();
-  const int span = (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;  // scores per warp, contiguous
-  const int i0 = min(sc.n, warp * span), i1 = min(sc.n, i0 + span);
-  const Cut kept(cut);
-  auto kept_weight = [&](float x, int i) {
-    const u64 w = kExact ? row.weight(x) : static_cast<u64>(ldexpf(row.rough(x), kRoughOne));
-    return kept.keeps(x, sc.first + i) ? w : 0ull;
-  };
-  u64 w = 0;
-  bool row_nan = false;
+// Weights of the scores [i0, i1) of this CTA at or ahead of the cut, summed over the warp (to lane 0); i0 a multiple
+// of VEC.  Rough sums: *nan where a score is NaN.
+template <bool kExact, typename T>
+__device__ __forceinline__ u64 span_weight(const Scores<T>& sc, const Row& row, const Cut& kept, bool cut, int i0, int i1, bool* nan) {
+  constexpr int VEC = Scores<T>::VEC, STEP = 32 * VEC;
+  const int lane = threadIdx.x % 32;
   if constexpr (kExact) {
+    u64 w = 0;
     for (int i = i0 + lane * VEC; i < i1; i += STEP) {
       float v[VEC];
       sc.vec(i, v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) w += kept_weight(v[e], i + e);
+      for (int e = 0; e < VEC; ++e) {
+        const u64 we = row.weight(v[e]);
+        w += kept.keeps(v[e], sc.first + i + e) ? we : 0ull;
+      }
     }
+    return warp_sum(w);
   } else {
     double r = 0;
-    if (cut == 0) {
+    if (!cut) {
+#pragma unroll 2
       for (int i = i0 + lane * VEC; i < i1; i += STEP) r += row.template rough_pack<VEC>(sc, i);
     } else {
       for (int i = i0 + lane * VEC; i < i1; i += STEP) {
@@ -775,11 +774,24 @@ __device__ __forceinline__ bool sweep(const Scores<T, kHeld>& sc, const Row& row
         r += static_cast<double>(t);
       }
     }
-    w = rough_units(r);
-    if (r != r) row_nan = true;
+    if (r != r) *nan = true;
+    return warp_sum(rough_units(r));
   }
-  w = warp_sum(w);
-  const bool nan = __syncthreads_or(row_nan);
+}
+
+// The token from all scores at or ahead of the cut, by sums in index order: of each warp's sixteenth of the share; where
+// the goal falls, of sixteenths of that; then of single scores.  Rough sums: false where the border is too near.
+template <bool kExact, typename T>
+__device__ __forceinline__ bool sweep(const Scores<T>& sc, const Row& row, u64 cut, double u, int slot, int64_t* token,
+                                      float* x_token, bool* mine, Shared& s, cg::cluster_group& cl) {
+  constexpr int VEC = Scores<T>::VEC, STEP = 32 * VEC;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const unsigned me = cl.block_rank();
+  const int span = (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;  // scores per warp, contiguous
+  const Cut kept(cut);
+  bool nan = false;
+  u64 w = span_weight<kExact>(sc, row, kept, cut != 0, min(sc.n, warp * span), min(sc.n, (warp + 1) * span), &nan);
+  nan = __syncthreads_or(nan);
   if (lane == 0) s.part[warp] = w;
   __syncthreads();
   u64 own = 0;
@@ -798,43 +810,54 @@ __device__ __forceinline__ bool sweep(const Scores<T, kHeld>& sc, const Row& row
     total += v[c];
   }
   if (!kExact && total >= kRoughNan) return false;  // the same for every CTA
-  const u64 goal = goal_of(u, total), margin = kExact ? 0 : (total >> (kRoughBits - 1)) + 2;
-  for (int i = 0; i < warp; ++i) ahead += s.part[i];
-  if (ahead < goal && goal <= ahead + s.part[warp]) {  // this warp's range holds it
-    for (int i = i0 + lane * VEC; i - lane * VEC < i1; i += STEP) {
-      float v[VEC];
-      u64 we[VEC], sum = 0;
+  const u64 goal = goal_of(u, total), margin = kExact ? 0 : (total >> (row.rough_bits - 1)) + 2;
+  if (ahead < goal && goal <= ahead + own) {  // this CTA's share holds it
+    int part = 0;
+    while (part < kWarps - 1 && ahead + s.part[part] < goal) ahead += s.part[part++];
+    const int sub = (span + STEP * kWarps - 1) / (STEP * kWarps) * STEP, end = min(sc.n, (part + 1) * span);
+    const int i0 = min(end, part * span + warp * sub), i1 = min(end, i0 + sub);
+    w = span_weight<kExact>(sc, row, kept, cut != 0, i0, i1, &nan);
+    __syncthreads();
+    if (lane == 0) s.part[warp] = w;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) ahead += s.part[i];
+    if (ahead < goal && goal <= ahead + s.part[warp]) {
+      for (int i = i0 + lane * VEC; i - lane * VEC < i1; i += STEP) {
+        float x[VEC];
+        u64 we[VEC], sum = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = -INFINITY;
-      if (i < i1) sc.vec(i, v);
+        for (int e = 0; e < VEC; ++e) x[e] = -INFINITY;
+        if (i < i1) sc.vec(i, x);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        we[e] = v[e] == -INFINITY ? 0 : kept_weight(v[e], i + e);
-        sum += we[e];
-      }
-      const u64 inc = warp_scan(sum);
-      const uint32_t reached = __ballot_sync(0xffffffffu, ahead + inc >= goal);
-      if (reached) {
-        if (lane == __ffs(reached) - 1) {
-          u64 at = ahead + inc - sum;
-          bool found = false;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            if (!found && at + we[e] >= goal) {
-              found = true;
-              if (kExact || (at + margin < goal && goal + margin < at + we[e])) {
-                *mine = true;
-                *token = sc.first + i + e;
-                *x_token = v[e];
-                if (!kExact) *cl.map_shared_rank(&s.found[2], 0) = 1;
-              }
-            }
-            at += we[e];
-          }
+        for (int e = 0; e < VEC; ++e) {
+          const u64 wx = kExact ? row.weight(x[e]) : static_cast<u64>(ldexpf(row.rough(x[e]), kRoughOne));
+          we[e] = x[e] != -INFINITY && kept.keeps(x[e], sc.first + i + e) ? wx : 0;
+          sum += we[e];
         }
-        break;
+        const u64 inc = warp_scan(sum);
+        const uint32_t reached = __ballot_sync(0xffffffffu, ahead + inc >= goal);
+        if (reached) {
+          if (lane == __ffs(reached) - 1) {
+            u64 at = ahead + inc - sum;
+            bool found = false;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              if (!found && at + we[e] >= goal) {
+                found = true;
+                if (kExact || (at + margin < goal && goal + margin < at + we[e])) {
+                  *mine = true;
+                  *token = sc.first + i + e;
+                  *x_token = x[e];
+                  if (!kExact) *cl.map_shared_rank(&s.found[2], 0) = 1;
+                }
+              }
+              at += we[e];
+            }
+          }
+          break;
+        }
+        ahead += __shfl_sync(0xffffffffu, inc, 31);
       }
-      ahead += __shfl_sync(0xffffffffu, inc, 31);
     }
   }
   if (kExact) return true;
@@ -842,20 +865,18 @@ __device__ __forceinline__ bool sweep(const Scores<T, kHeld>& sc, const Row& row
   return *cl.map_shared_rank(&s.found[2], 0) != 0;
 }
 
-template <typename T, bool kHeld>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
-  T* held = reinterpret_cast<T*>(smem_raw + sizeof(Shared));
   cg::cluster_group cl = cg::this_cluster();
   const unsigned C = cl.num_blocks(), me = cl.block_rank();
   const int64_t r = blockIdx.x / C, row_id = p.row0 + r;
   const int tid = threadIdx.x;
-  constexpr int VEC = Scores<T, kHeld>::VEC;
+  constexpr int VEC = Scores<T>::VEC;
   const int64_t first = static_cast<int64_t>(me) * p.share;
-  Scores<T, kHeld> sc;
+  Scores<T> sc;
   sc.x = static_cast<const T*>(p.x) + r * p.ld + first;
-  sc.held = held;
   sc.aligned = p.aligned;
   sc.first = static_cast<uint32_t>(first);
   sc.n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(p.share), p.V - first)));
@@ -871,7 +892,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   const bool by_k = k > 0 && k < p.V, by_p = top_p < 1.0, by_m = min_p > 0.0;
   const double lm = by_m && !greedy ? log(min(min_p, 1.0)) : 0.0, invT = 1.0 / temp;
 
-  // ---------------------------------------------------------------- scores in, the largest
+  // ---------------------------------------------------------------- the largest score
   float t_top = -INFINITY;  // of this thread (fmaxf leaves NaN out)
   {
     struct alignas(16) P { T e[VEC]; };
@@ -892,9 +913,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int at = i + j * kThreads * VEC;
-        if constexpr (kHeld)
-          if (at < sc.n) *reinterpret_cast<P*>(held + at) = q[j];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) t_top = fmaxf(t_top, to_float(q[j].e[k]));
       }
@@ -919,6 +937,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   row.per_bin = static_cast<float>(kBins) / row.reach;
   row.root = s.root;
   row.c32 = static_cast<float>(1.4426950408889634 * row.invT);
+  row.c32_lo = static_cast<float>(1.4426950408889634 * row.invT - row.c32);
+  row.rough_bits = p.V <= 200000 ? 19 : 18;
   row.rough_ok = p.V <= (1 << 20) && row.top < INFINITY && row.c32 > 1e-30f && row.c32 < 1e30f;
 
   int64_t token = 0;
@@ -955,8 +975,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         if (!by_k) {
           u64 w = row.rough_ok ? cluster_join<true>(rough_total(sc, row, s), 2, s, cl) : kRoughNan;
           if (w < kRoughNan) {
-            lo = (w - (w >> kRoughBits) - 1) << (row.lg_one - kRoughOne);
-            hi = (w + (w >> kRoughBits) + 1) << (row.lg_one - kRoughOne);
+            lo = (w - (w >> row.rough_bits) - 1) << (row.lg_one - kRoughOne);
+            hi = (w + (w >> row.rough_bits) + 1) << (row.lg_one - kRoughOne);
           } else {
             row.rough_ok = false;
             exact = true;
@@ -1020,23 +1040,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ host
-constexpr size_t kSmemMax = 227 * 1024;
-
 template <typename T>
 static cudaError_t launch_t(Params p, cudaStream_t st) {
-  constexpr int64_t most = static_cast<int64_t>((kSmemMax - sizeof(Shared)) / sizeof(T) / 32 * 32);
   static_assert(kMaxCluster == 8, "cluster sizes below");
-  constexpr int64_t pair = static_cast<int64_t>((kSmemMax / 2 - 1024 - sizeof(Shared)) / sizeof(T) / 32 * 32);
-  // the smallest cluster whose CTAs hold the row, two of them an SM; few rows take more, to spread over the SMs
+  // two CTAs an SM and about two rounds of them, so that a row that needs its fixed-point sums does not hold up the rest
   int C = 1;
-  while (C < 8 && (ceil_div(p.V, C) > pair || p.N * C < kNumSMsB200 / 2) && p.V > 2048 * C) C *= 2;
+  while (C < 8 && 2 * C * p.N <= 4 * kNumSMsB200 && p.V > 2048 * C) C *= 2;
   p.share = static_cast<int>(round_up(ceil_div(std::max<int64_t>(p.V, 1), C), 32));
-  const bool held = p.share <= most;
   p.aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.ld * sizeof(T)) % 16 == 0;
   int lg = 0;
   while ((1ll << lg) < p.V) ++lg;
   p.lg_one = std::min(44, 62 - lg);
-  auto kern = held ? sample_kernel<T, true> : sample_kernel<T, false>;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1047,11 +1061,10 @@ static cudaError_t launch_t(Params p, cudaStream_t st) {
   cfg.numAttrs = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(p.N * C), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = sizeof(Shared) + (held ? static_cast<size_t>(p.share) * sizeof(T) : 0);
+  cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = st;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
-  if (e != cudaSuccess) return e;
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  static_assert(sizeof(Shared) <= 48 * 1024, "more needs cudaFuncSetAttribute");
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
 }
 
 static cudaError_t launch(const Params& p, cudaStream_t st) {
