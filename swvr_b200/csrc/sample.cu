@@ -17,7 +17,7 @@
 //   1. the largest score, and each thread's largest;
 //   2. a score that enough tokens reach: for top-k, the k-th of the threads' largest scores (k tokens are at
 //      least that large, and few more are, as long as k is well below the number of threads); for a top-p
-//      without top-k the 256-th of them, beside the weight of the whole row; min-p knows its own;
+//      without top-k the 128-th of them, beside the weight of the whole row; min-p knows its own;
 //   3. the tokens that reach it are gathered in one CTA, ordered by (score, index), cut by prefix sums, and u is
 //      looked up in the running weight by index.
 // Otherwise (no filter, a wide nucleus, long runs of equal scores) thresholds come from a histogram over kBins
@@ -50,8 +50,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
 constexpr float kReach = 30.5f;  // e^-30.5 < 2^-44
-constexpr int kRoughOne = 40;    // fp32 sums are kept in units of 2^-40 of the largest weight: 2^60 at most,
-constexpr u64 kRoughNan = 1ull << 60;  // what a CTA that met NaN posts instead (the fixed-point sums leave NaN out)
+constexpr int kRoughOne = 40;    // fp32 sums are kept in units of 2^-40 of the largest weight
 
 struct Setting {  // one value for all rows, or one per row
   const void* ptr;
@@ -154,6 +153,19 @@ __device__ __forceinline__ double widen(float x) {
   return (b & 0x7f800000u) == 0 ? 0.0 : v;
 }
 
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ void set_lowest(float* v) { *v = -INFINITY; }
+__device__ __forceinline__ void set_lowest(__nv_bfloat16* v) { *v = __ushort_as_bfloat16(0xff80); }
+__device__ __forceinline__ void set_lowest(__half* v) { *v = __ushort_as_half(0xfc00); }
+// NaN never wins; -0 equals +0
+template <typename T>
+__device__ __forceinline__ float to_score(T v) {
+  const float f = to_float(v);
+  return f != f ? -INFINITY : f + 0.f;
+}
+
 struct Row {
   float top;      // the largest score
   double top_d, c64;  // top, and 64 log2(e) / T
@@ -166,17 +178,17 @@ struct Row {
   int rough_bits; // 18 or 19
   float c32, c32_lo;  // log2(e) / T in two parts
 
+  // -inf and NaN: 2^-88, nothing
   __device__ __forceinline__ float rough(float x) const {
-    const float d = x - top;
+    const float d = fmaxf(x - top, -2.f * reach);
     return ex2(fmaf(d, c32, d * c32_lo));
   }
-  // the sum over a pack of scores; NaN where one of them is
-  template <int VEC, typename S>
-  __device__ __forceinline__ double rough_pack(const S& sc, int i) const {
+  // the sum over a pack of scores
+  template <int VEC, typename P>
+  __device__ __forceinline__ double rough_pack(const P& p) const {
     float v[VEC];
-    sc.raw(i, v);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = rough(v[e]);
+    for (int e = 0; e < VEC; ++e) v[e] = rough(to_float(p.e[e]));
 #pragma unroll
     for (int o = VEC / 2; o > 0; o /= 2)
 #pragma unroll
@@ -212,19 +224,6 @@ struct Row {
   }
 };
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ void set_lowest(float* v) { *v = -INFINITY; }
-__device__ __forceinline__ void set_lowest(__nv_bfloat16* v) { *v = __ushort_as_bfloat16(0xff80); }
-__device__ __forceinline__ void set_lowest(__half* v) { *v = __ushort_as_half(0xfc00); }
-// NaN never wins; -0 equals +0
-template <typename T>
-__device__ __forceinline__ float to_score(T v) {
-  const float f = to_float(v);
-  return f != f ? -INFINITY : f + 0.f;
-}
-
 // This CTA's scores.
 template <typename T>
 struct Scores {
@@ -235,40 +234,45 @@ struct Scores {
   uint32_t first;  // its index in the row
 
   __device__ __forceinline__ float at(int i) const { return to_score(x[i]); }
-  // VEC scores from i on (i a multiple of VEC); -inf past the end
-  __device__ __forceinline__ void vec(int i, float (&v)[VEC]) const {
-    if (aligned && i + VEC <= n) {
-      struct alignas(16) P { T e[VEC]; };
-      const P p = *reinterpret_cast<const P*>(x + i);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = to_score(p.e[k]);
+  struct alignas(16) Pack {
+    T e[VEC];
+  };
+  // VEC scores from i on (i a multiple of VEC), as they are; -inf past `end`
+  __device__ __forceinline__ Pack load(int i, int end) const {
+    Pack p;
+    if (aligned && i + VEC <= end) {
+      p = *reinterpret_cast<const Pack*>(x + i);
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = i + k < n ? at(i + k) : -INFINITY;
+      for (int k = 0; k < VEC; ++k) {
+        if (i + k < end) p.e[k] = x[i + k];
+        else set_lowest(&p.e[k]);
+      }
+    }
+    return p;
+  }
+  // f(pack, index) for the packs at i0, i0 + step, ... before end, U loads at a time (an L2 round trip is some 700
+  // cycles; more than f has registers for costs more than it hides)
+  template <int U, typename F>
+  __device__ __forceinline__ void packs(int i0, int end, int step, F f) const {
+    for (int i = i0; i < end; i += U * step) {
+      Pack q[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) q[j] = load(i + j * step, end);
+#pragma unroll
+      for (int j = 0; j < U; ++j) f(q[j], i + j * step);
     }
   }
-  // VEC scores as they are: NaN as NaN, -0 as -0
-  __device__ __forceinline__ void raw(int i, float (&v)[VEC]) const {
-    if (aligned && i + VEC <= n) {
-      struct alignas(16) P { T e[VEC]; };
-      const P p = *reinterpret_cast<const P*>(x + i);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = to_float(p.e[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = i + k < n ? to_float(x[i + k]) : -INFINITY;
-    }
-  }
-  // f(score, index within the CTA) for every score, in no order
+  // f(score, index within the CTA) for every score, in no order; NaN and -inf are left out, -0 is +0
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    for (int i = threadIdx.x * VEC; i < n; i += kThreads * VEC) {
-      float v[VEC];
-      vec(i, v);
+    packs<1>(threadIdx.x * VEC, n, kThreads * VEC, [&](const Pack& p, int i) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k)
-        if (v[k] != -INFINITY) f(v[k], i + k);
-    }
+      for (int k = 0; k < VEC; ++k) {
+        const float v = to_score(p.e[k]);
+        if (v != -INFINITY) f(v, i + k);
+      }
+    });
   }
 };
 
@@ -579,20 +583,20 @@ __device__ __forceinline__ uint32_t gather(const Scores<T>& sc, const Row& row, 
   constexpr int VEC = Scores<T>::VEC;
   if (threadIdx.x == 0) s.n_list = 0;
   __syncthreads();
-  for (int i = threadIdx.x * VEC; i < sc.n; i += kThreads * VEC) {
-    float v[VEC], most = -INFINITY;
-    sc.raw(i, v);
+  sc.template packs<2>(threadIdx.x * VEC, sc.n, kThreads * VEC, [&](const typename Scores<T>::Pack& p, int i) {
+    float most = to_float(p.e[0]);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) most = fmaxf(most, v[k]);
-    if (!(most >= reach_x)) continue;  // most packs
+    for (int k = 1; k < VEC; ++k) most = fmaxf(most, to_float(p.e[k]));
+    if (!(most >= reach_x)) return;  // most packs
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      if (v[k] >= reach_x && also(v[k] + 0.f, i + k)) {
+      const float v = to_float(p.e[k]) + 0.f;
+      if (v >= reach_x && also(v, i + k)) {
         const uint32_t j = atomicAdd(&s.n_list, 1u);
-        if (j < kList) s.list[j] = place_of(v[k] + 0.f, sc.first + i + k);
+        if (j < kList) s.list[j] = place_of(v, sc.first + i + k);
       }
     }
-  }
+  });
   cl.sync();
   u64 n[kMaxCluster];
   read_all(cl, n, [&](unsigned c) { return cl.map_shared_rank(&s.n_list, c); });
@@ -730,51 +734,48 @@ __device__ __forceinline__ u64 exact_total(const Scores<T>& sc, const Row& row, 
   sc.each([&](float x, int i) { w += row.weight(x); });
   return block_sum(w, s);
 }
-__device__ __forceinline__ u64 rough_units(double w) { return w == w ? static_cast<u64>(ldexp(w, kRoughOne)) : 0; }
+__device__ __forceinline__ u64 rough_units(double w) { return static_cast<u64>(ldexp(w, kRoughOne)); }
 template <typename T>
 __device__ __forceinline__ u64 rough_total(const Scores<T>& sc, const Row& row, Shared& s) {
   constexpr int VEC = Scores<T>::VEC;
   double w = 0;
-#pragma unroll 2
-  for (int i = threadIdx.x * VEC; i < sc.n; i += kThreads * VEC) w += row.template rough_pack<VEC>(sc, i);
-  const bool nan = __syncthreads_or(w != w);
-  const u64 sum = block_sum(rough_units(w), s);
-  return nan ? kRoughNan : sum;
+  sc.template packs<2>(threadIdx.x * VEC, sc.n, kThreads * VEC,
+                       [&](const typename Scores<T>::Pack& p, int) { w += row.template rough_pack<VEC>(p); });
+  return block_sum(rough_units(w), s);
 }
 
-// Weights of the scores [i0, i1) of this CTA at or ahead of the cut, summed over the warp (to lane 0); i0 a multiple
-// of VEC.  Rough sums: *nan where a score is NaN.
+// Weights of the scores [i0, i1) of this CTA at or ahead of the cut, summed over the warp; i0 a multiple of VEC.
 template <bool kExact, typename T>
-__device__ __forceinline__ u64 span_weight(const Scores<T>& sc, const Row& row, const Cut& kept, bool cut, int i0, int i1, bool* nan) {
+__device__ __forceinline__ u64 span_weight(const Scores<T>& sc, const Row& row, const Cut& kept, bool cut, int i0, int i1) {
   constexpr int VEC = Scores<T>::VEC, STEP = 32 * VEC;
   const int lane = threadIdx.x % 32;
+  using Pack = typename Scores<T>::Pack;
   if constexpr (kExact) {
     u64 w = 0;
-    for (int i = i0 + lane * VEC; i < i1; i += STEP) {
-      float v[VEC];
-      sc.vec(i, v);
+    sc.template packs<1>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int i) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const u64 we = row.weight(v[e]);
-        w += kept.keeps(v[e], sc.first + i + e) ? we : 0ull;
+        const float x = to_score(p.e[e]);
+        const u64 we = row.weight(x);
+        w += kept.keeps(x, sc.first + i + e) ? we : 0ull;
       }
-    }
+    });
     return warp_sum(w);
   } else {
     double r = 0;
     if (!cut) {
-#pragma unroll 2
-      for (int i = i0 + lane * VEC; i < i1; i += STEP) r += row.template rough_pack<VEC>(sc, i);
+      sc.template packs<2>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int) { r += row.template rough_pack<VEC>(p); });
     } else {
-      for (int i = i0 + lane * VEC; i < i1; i += STEP) {
-        float v[VEC], t = 0.f;
-        sc.vec(i, v);
+      sc.template packs<2>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int i) {
+        float t = 0.f;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) t += kept.keeps(v[e], sc.first + i + e) ? row.rough(v[e]) : 0.f;
+        for (int e = 0; e < VEC; ++e) {
+          const float x = to_score(p.e[e]);
+          t += kept.keeps(x, sc.first + i + e) ? row.rough(x) : 0.f;
+        }
         r += static_cast<double>(t);
-      }
+      });
     }
-    if (r != r) *nan = true;
     return warp_sum(rough_units(r));
   }
 }
@@ -789,14 +790,12 @@ __device__ __forceinline__ bool sweep(const Scores<T>& sc, const Row& row, u64 c
   const unsigned me = cl.block_rank();
   const int span = (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;  // scores per warp, contiguous
   const Cut kept(cut);
-  bool nan = false;
-  u64 w = span_weight<kExact>(sc, row, kept, cut != 0, min(sc.n, warp * span), min(sc.n, (warp + 1) * span), &nan);
-  nan = __syncthreads_or(nan);
+  u64 w = span_weight<kExact>(sc, row, kept, cut != 0, min(sc.n, warp * span), min(sc.n, (warp + 1) * span));
+  __syncthreads();
   if (lane == 0) s.part[warp] = w;
   __syncthreads();
   u64 own = 0;
   for (int i = 0; i < kWarps; ++i) own += s.part[i];
-  if (nan) own = kRoughNan;
   if (threadIdx.x == 0) {
     s.slot[slot] = own;
     s.found[2] = 0;
@@ -809,27 +808,25 @@ __device__ __forceinline__ bool sweep(const Scores<T>& sc, const Row& row, u64 c
     if (c < me) ahead += v[c];
     total += v[c];
   }
-  if (!kExact && total >= kRoughNan) return false;  // the same for every CTA
   const u64 goal = goal_of(u, total), margin = kExact ? 0 : (total >> (row.rough_bits - 1)) + 2;
   if (ahead < goal && goal <= ahead + own) {  // this CTA's share holds it
     int part = 0;
     while (part < kWarps - 1 && ahead + s.part[part] < goal) ahead += s.part[part++];
     const int sub = (span + STEP * kWarps - 1) / (STEP * kWarps) * STEP, end = min(sc.n, (part + 1) * span);
     const int i0 = min(end, part * span + warp * sub), i1 = min(end, i0 + sub);
-    w = span_weight<kExact>(sc, row, kept, cut != 0, i0, i1, &nan);
+    w = span_weight<kExact>(sc, row, kept, cut != 0, i0, i1);
     __syncthreads();
     if (lane == 0) s.part[warp] = w;
     __syncthreads();
     for (int i = 0; i < warp; ++i) ahead += s.part[i];
     if (ahead < goal && goal <= ahead + s.part[warp]) {
       for (int i = i0 + lane * VEC; i - lane * VEC < i1; i += STEP) {
+        const typename Scores<T>::Pack p = sc.load(i, i1);
         float x[VEC];
         u64 we[VEC], sum = 0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[e] = -INFINITY;
-        if (i < i1) sc.vec(i, x);
-#pragma unroll
         for (int e = 0; e < VEC; ++e) {
+          x[e] = to_score(p.e[e]);
           const u64 wx = kExact ? row.weight(x[e]) : static_cast<u64>(ldexpf(row.rough(x[e]), kRoughOne));
           we[e] = x[e] != -INFINITY && kept.keeps(x[e], sc.first + i + e) ? wx : 0;
           sum += we[e];
@@ -865,7 +862,8 @@ __device__ __forceinline__ bool sweep(const Scores<T>& sc, const Row& row, u64 c
   return *cl.map_shared_rank(&s.found[2], 0) != 0;
 }
 
-template <typename T>
+// kFilters: some row may have top-k, top-p or min-p; without, the kernel needs fewer registers and more of it fits an SM.
+template <typename T, bool kFilters>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
@@ -889,35 +887,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   const int64_t k = p.k_ptr ? (p.k_bits == 64 ? static_cast<const int64_t*>(p.k_ptr)[row_id]
                                               : static_cast<int64_t>(static_cast<const int32_t*>(p.k_ptr)[row_id]))
                             : p.k;
-  const bool by_k = k > 0 && k < p.V, by_p = top_p < 1.0, by_m = min_p > 0.0;
+  const bool by_k = kFilters && k > 0 && k < p.V, by_p = kFilters && top_p < 1.0, by_m = kFilters && min_p > 0.0;
   const double lm = by_m && !greedy ? log(min(min_p, 1.0)) : 0.0, invT = 1.0 / temp;
 
   // ---------------------------------------------------------------- the largest score
   float t_top = -INFINITY;  // of this thread (fmaxf leaves NaN out)
-  {
-    struct alignas(16) P { T e[VEC]; };
-    constexpr int U = 4;  // packs in flight per thread
-    for (int i = tid * VEC; i < sc.n; i += U * kThreads * VEC) {
-      P q[U];
+  sc.template packs<4>(tid * VEC, sc.n, kThreads * VEC, [&](const typename Scores<T>::Pack& q, int) {
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int at = i + j * kThreads * VEC;
-        if (p.aligned && at + VEC <= sc.n) {
-          q[j] = *reinterpret_cast<const P*>(sc.x + at);
-        } else {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k)
-            if (at + k < sc.n) q[j].e[k] = sc.x[at + k];
-            else set_lowest(&q[j].e[k]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) t_top = fmaxf(t_top, to_float(q[j].e[k]));
-      }
-    }
-  }
+    for (int k = 0; k < VEC; ++k) t_top = fmaxf(t_top, to_float(q.e[k]));
+  });
   t_top += 0.f;
   Row row;
   row.top = score_of(static_cast<uint32_t>(cluster_join<false>(block_max32(order_of(t_top), s), 0, s, cl)));
@@ -973,21 +951,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         clear_bins(false, s);
         if (t_top != -INFINITY && row.live(t_top)) atomicAdd(&s.count[row.bin(t_top)], 1u);
         if (!by_k) {
-          u64 w = row.rough_ok ? cluster_join<true>(rough_total(sc, row, s), 2, s, cl) : kRoughNan;
-          if (w < kRoughNan) {
+          if (row.rough_ok) {
+            const u64 w = cluster_join<true>(rough_total(sc, row, s), 2, s, cl);
             lo = (w - (w >> row.rough_bits) - 1) << (row.lg_one - kRoughOne);
             hi = (w + (w >> row.rough_bits) + 1) << (row.lg_one - kRoughOne);
           } else {
-            row.rough_ok = false;
             exact = true;
-            lo = hi = cluster_join<true>(exact_total(sc, row, s), 8, s, cl);
+            lo = hi = cluster_join<true>(exact_total(sc, row, s), 2, s, cl);
           }
         }
         merge_bins(false, s, cl);
       }
-      // a nucleus is looked for among the 48 largest threads' scores, then among more
+      // a nucleus is looked for among the 128 largest threads' scores, then among more
       const u64 most = min(kThreads * C / 2, 384u);
-      for (u64 wanted = by_k ? static_cast<u64>(k) : min(48ull, most);; wanted = most) {
+      for (u64 wanted = by_k ? static_cast<u64>(k) : min(128ull, most);; wanted = most) {
         float reach_x = row.floor_x();  // a score that every token which may be kept reaches
         if (by_k || by_p) {
           find_bin<true>(wanted, s);
@@ -1006,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
             f = choose_from_list(static_cast<int>(m), by_k, static_cast<u64>(k), by_p, top_p, lo, hi, all, cut, u, &token,
                                  &x_token, &mine, s);
           if (!by_p || by_k) break;  // always found
-          const int slot = wanted == most && most > 48 ? at + 3 : at;
+          const int slot = wanted == most && most > 128 ? at + 3 : at;
           if (tid == 0 && me == 0) s.slot[slot] = f;
           cl.sync();
           f = static_cast<Found>(*cl.map_shared_rank(&s.slot[slot], 0));
@@ -1064,7 +1041,8 @@ static cudaError_t launch_t(Params p, cudaStream_t st) {
   cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = st;
   static_assert(sizeof(Shared) <= 48 * 1024, "more needs cudaFuncSetAttribute");
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+  const bool filters = p.k_ptr || p.k > 0 || p.p.ptr || p.p.value < 1.0 || p.m.ptr || p.m.value > 0.0;
+  return cudaLaunchKernelEx(&cfg, filters ? sample_kernel<T, true> : sample_kernel<T, false>, p);
 }
 
 static cudaError_t launch(const Params& p, cudaStream_t st) {
