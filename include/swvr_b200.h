@@ -262,9 +262,9 @@ int swvr_embed_bwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tok
  * logit above -inf) makes its token's loss and gradient NaN and sets SWVR_TOKEN_CODE.
  *
  * teacher_ids [N, teacher] (id_bits 32 or 64) and teacher_logits [N, teacher] (any dtype) are
- * contiguous; teacher_lse and weight ([N] or NULL), out, lse, qsum, each [N], slogq and z
- * [N, teacher] and stats [2] are in the accumulation dtype, sid [N, teacher] in int32.  sid, slogq,
- * z, lse, qsum, each and stats are written by the forward and read by the backward: the
+ * contiguous; teacher_lse and weight ([N] or NULL), out, lse, lse_lo (what rounding took from lse), qsum,
+ * each [N], slogq and z [N, teacher] and stats [2] are in the accumulation dtype, sid [N, teacher] in
+ * int32.  sid, slogq, z, lse, lse_lo, qsum, each and stats are written by the forward and read by the backward: the
  * caller keeps them, and h, W, bias, weight and the sizes unchanged, in between.  W and h as in
  * swvr_problem.  At most 1024 teacher entries.  [N, vocab] is never materialised on the
  * tensor-core path; the fp32 / fp64 path stages `chunk` vocabulary rows of it.
@@ -288,6 +288,7 @@ typedef struct swvr_distill {
   void* slogq;
   void* z;
   void* lse;
+  void* lse_lo;
   void* qsum;
   void* each;
   void* stats;                /* SUM / MEAN */

@@ -6,6 +6,7 @@ codes and the current CUDA stream; the library allocates nothing.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -63,8 +64,8 @@ class Distill(ctypes.Structure):
         ("chunk", c_int64),
         ("teacher_ids", c_void_p), ("teacher_logits", c_void_p), ("teacher_lse", c_void_p), ("weight", c_void_p),
         ("reduction", c_int32),
-        ("sid", c_void_p), ("slogq", c_void_p), ("z", c_void_p), ("lse", c_void_p), ("qsum", c_void_p),
-        ("each", c_void_p), ("stats", c_void_p),
+        ("sid", c_void_p), ("slogq", c_void_p), ("z", c_void_p), ("lse", c_void_p), ("lse_lo", c_void_p),
+        ("qsum", c_void_p), ("each", c_void_p), ("stats", c_void_p),
     ]
 
 
@@ -183,8 +184,21 @@ def check_device_error() -> None:
         raise RuntimeError(f"swvr_b200 kernel gave up waiting (device error site 0x{code.value:x})")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None:  # the handle alone: no Stream object
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context with ``device`` current; nothing to enter when it already is."""
+    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(t):

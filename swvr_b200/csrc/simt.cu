@@ -434,11 +434,11 @@ cudaError_t gemm(cudaStream_t st, int64_t M, int64_t N, int64_t K, T alpha, cons
 template <typename T>
 cudaError_t gemm_split(cudaStream_t st, int64_t M, int64_t N, int64_t K, T alpha, const T* A, int64_t sam,
                         int64_t sak, const T* B, int64_t sbk, int64_t sbn, T beta, void* C, int cdt, int64_t scm,
-                        int64_t scn, float* part) {
+                        int64_t scn, float* part, int64_t k_least = 256) {
   if constexpr (sizeof(T) == 4) {
     if (M > 0 && N > 0 && part && tf32x3_ok(A, sam, sak, M, B, sbk, sbn, N, K)) {
       const int64_t tiles = ceil_div(M, tf32x3::TM) * ceil_div(N, tf32x3::TN);
-      int64_t splits = std::min<int64_t>({int64_t(16), ceil_div(4 * kNumSMsB200, tiles), K / 256,
+      int64_t splits = std::min<int64_t>({int64_t(16), ceil_div(4 * kNumSMsB200, tiles), K / k_least,
                                           splitk_floats(M, N) / (M * N)});
       if (splits >= 2) {
         const int64_t kper = round_up(ceil_div(K, splits), tf32x3::TK);

@@ -3,10 +3,35 @@
 
 #include <cuda.h>
 
+#include <map>
+#include <mutex>
+#include <utility>
+
 #include "common.cuh"
 
 namespace swvr {
 namespace tc {
+
+// How many clusters of `cfg` (of two CTAs) of this kernel can be resident on the current device, with its
+// dynamic shared memory allowed: asked of the runtime once per kernel and device (the two calls take some
+// 10 us of host time, more than a launch).
+inline cudaError_t resident_clusters(const void* kern, const cudaLaunchConfig_t& cfg, int* clusters) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, int> known;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto it = known.find({dev, kern});
+  if (it != known.end()) {
+    *clusters = it->second;
+    return cudaSuccess;
+  }
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cfg.dynamicSmemBytes));
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(clusters, kern, &cfg);
+  if (e == cudaSuccess) known[{dev, kern}] = *clusters;
+  return e;
+}
 
 // ------------------------------------------------------------------ forward
 struct FwdParams {

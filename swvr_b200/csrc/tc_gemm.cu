@@ -292,8 +292,6 @@ template <bool kBF16, int NS, bool kScaled>
 static cudaError_t launch(const GemmMaps& m, const GemmParams& prm, int max_pairs, bool pdl, cudaStream_t st) {
   using Cfg = GemmCfg<NS>;
   auto kern = gemm_kernel<kBF16, NS, kScaled>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_ALLOC);
-  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -307,7 +305,7 @@ static cudaError_t launch(const GemmMaps& m, const GemmParams& prm, int max_pair
   cfg.stream = st;
   cfg.gridDim = dim3(2 * 74, 1, 1);
   int clusters = 0;
-  e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+  const cudaError_t e = resident_clusters(reinterpret_cast<const void*>(kern), cfg, &clusters);
   if (e != cudaSuccess) return e;
   const int tiles = prm.dw_tiles + prm.dh_tiles;
   int pairs = std::min(std::min(clusters, max_pairs), tiles);

@@ -374,8 +374,6 @@ template <bool kBF16, int MODE, int BN, int NS>
 static cudaError_t launch_head(const HeadMaps& m, const HeadParams& prm, int max_pairs, bool pdl, cudaStream_t st) {
   using Cfg = HeadCfg<BN, NS>;
   auto kern = head_kernel<kBF16, MODE, BN, NS>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_ALLOC);
-  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -389,7 +387,7 @@ static cudaError_t launch_head(const HeadMaps& m, const HeadParams& prm, int max
   cfg.stream = st;
   cfg.gridDim = dim3(2 * 74, 1, 1);
   int clusters = 0;
-  e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+  const cudaError_t e = resident_clusters(reinterpret_cast<const void*>(kern), cfg, &clusters);
   if (e != cudaSuccess) return e;
   int pairs = std::min(std::min(clusters, max_pairs), prm.units);
   if (pairs < 1) pairs = 1;

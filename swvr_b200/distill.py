@@ -19,6 +19,7 @@ from torch import nn
 
 from . import _native as nat
 from .api import _compute_dtype, _weight_of
+from .embedding import _eager
 from .ops import (_REDUCTIONS, _grad_buffer, _ld, _no_grad_marker, _prepare_k, _require_cuda, _tensor_core, _workspace,
                   acc_dtype, default_chunk_size)
 
@@ -26,12 +27,15 @@ _ID_BITS = {torch.int64: 64, torch.int32: 32}
 MAX_TEACHER = 1024
 
 
-def _problem(hc, Wc, bias, ids, logits, t_lse, weight, saved, temperature, logit_scale, chunk, cdt, reduction):
+def _problem(hc, Wc, bias, ids, logits, t_lse, weight, sid, saved, temperature, logit_scale, chunk, cdt, reduction):
     """The C struct of one call.  It holds raw pointers only: the caller keeps every tensor referenced
-    until the launch has been issued."""
+    until the launch has been issued.  ``saved`` holds the forward's fp32 / fp64 results one after another
+    (``_saved_numel``): log q and scores by sorted entry, then lse, its remainder, sum of q and loss by token, then the
+    reduction's two numbers."""
+    N, Kt = ids.shape
     p = nat.Distill()
     p.n_tokens, p.hidden = hc.shape
-    p.vocab, p.teacher = Wc.shape[0], ids.shape[1]
+    p.vocab, p.teacher = Wc.shape[0], Kt
     p.compute_dtype = nat.dtype_code(cdt)
     p.bias_dtype = nat.dtype_code(bias.dtype) if bias is not None else 0
     p.teacher_dtype, p.id_bits = nat.dtype_code(logits.dtype), _ID_BITS[ids.dtype]
@@ -40,71 +44,56 @@ def _problem(hc, Wc, bias, ids, logits, t_lse, weight, saved, temperature, logit
     p.logit_scale, p.temperature, p.chunk, p.reduction = logit_scale, temperature, chunk, reduction
     p.teacher_ids, p.teacher_logits = ids.data_ptr(), logits.data_ptr()
     p.teacher_lse, p.weight = nat.ptr(t_lse), nat.ptr(weight)
-    p.sid, p.slogq, p.z, p.lse, p.qsum, p.each, p.stats = (t.data_ptr() for t in saved)
+    p.sid = sid.data_ptr()
+    at, es = saved.data_ptr(), saved.element_size()
+    p.slogq, p.z = at, at + es * N * Kt
+    at += es * 2 * N * Kt
+    p.lse, p.lse_lo, p.qsum, p.each, p.stats = at, at + es * N, at + es * 2 * N, at + es * 3 * N, at + es * 4 * N
     return p
+
+
+def _saved_numel(N, Kt):
+    return 2 * N * Kt + 4 * N + 2
 
 
 def _operands(h, W, bias, cdt):
     return _prepare_k(h, cdt), _prepare_k(W, cdt), bias.contiguous() if bias is not None else None
 
 
-# Custom-op pair, like the readout's own (ops.py).  The outputs after the loss are what the
-# backward needs of the forward: sorted teacher ids, their log q and scores, and per token lse,
-# sum of q, loss; they take no gradient.
-
-@torch.library.custom_op("swvr_b200::distill", mutates_args=())
-def _distill_op(h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], ids: torch.Tensor, logits: torch.Tensor,
-                t_lse: Optional[torch.Tensor], weight: Optional[torch.Tensor], temperature: float, logit_scale: float,
-                chunk: int, cdt: torch.dtype, reduction: int) -> Tuple[
-                    torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
-                    torch.Tensor]:
+def _distill_fwd(h, W, bias, ids, logits, t_lse, weight, temperature, logit_scale, chunk, cdt, reduction):
     dev = _require_cuda(h, W, bias, ids, logits, t_lse, weight)
     adt = acc_dtype(cdt)
     N, Kt = ids.shape
-    new = lambda *s, dtype=adt: torch.empty(*s, dtype=dtype, device=dev)  # noqa: E731
-    out = new(N) if reduction == nat.REDUCE_NONE else new(())
-    saved = (new(N, Kt, dtype=torch.int32), new(N, Kt), new(N, Kt), new(N), new(N), new(N), new(2))
+    out = torch.empty((N,) if reduction == nat.REDUCE_NONE else (), dtype=adt, device=dev)
+    sid = torch.empty(N, Kt, dtype=torch.int32, device=dev)
+    saved = torch.empty(_saved_numel(N, Kt), dtype=adt, device=dev)
     hc, Wc, b = _operands(h, W, bias, cdt)
-    p = _problem(hc, Wc, b, ids, logits, t_lse, weight, saved, temperature, logit_scale, chunk, cdt, reduction)
+    p = _problem(hc, Wc, b, ids, logits, t_lse, weight, sid, saved, temperature, logit_scale, chunk, cdt, reduction)
     lib = nat.lib()
     nbytes = nat.c_size_t(0)
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         nat.check(lib.swvr_distill_fwd_workspace_size(p, nat.ctypes.byref(nbytes)), "swvr_distill_fwd_workspace_size")
         ws = _workspace(nbytes.value, dev)
         nat.check(lib.swvr_distill_fwd(p, out.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_ptr(dev)),
                   "swvr_distill_fwd")
-    return (out, *saved)
+    return out, sid, saved
 
 
-@_distill_op.register_fake
-def _(h, W, bias, ids, logits, t_lse, weight, temperature, logit_scale, chunk, cdt, reduction):
-    adt = acc_dtype(cdt)
-    N, Kt = ids.shape
-    new = lambda *s, dtype=adt: h.new_empty(s, dtype=dtype)  # noqa: E731
-    out = new(N) if reduction == nat.REDUCE_NONE else new()
-    return out, new(N, Kt, dtype=torch.int32), new(N, Kt), new(N, Kt), new(N), new(N), new(N), new(2)
-
-
-@torch.library.custom_op("swvr_b200::distill_bwd", mutates_args=())
-def _distill_bwd_op(grad: torch.Tensor, h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor],
-                    ids: torch.Tensor, logits: torch.Tensor, t_lse: Optional[torch.Tensor],
-                    weight: Optional[torch.Tensor], sid: torch.Tensor, slogq: torch.Tensor, z: torch.Tensor,
-                    lse: torch.Tensor, qsum: torch.Tensor, each: torch.Tensor, stats: torch.Tensor, temperature: float,
-                    logit_scale: float, chunk: int, cdt: torch.dtype, reduction: int, need_h: bool, need_W: bool,
-                    need_b: bool, need_w: bool) -> List[torch.Tensor]:
+def _distill_bwd(grad, h, W, bias, ids, logits, t_lse, weight, sid, saved, temperature, logit_scale, chunk, cdt, reduction,
+                 need_h, need_W, need_b, need_w):
+    """(dh, dW, db, dweight), None where not asked for."""
     dev = _require_cuda(h, W, bias, ids, grad, weight)
     (N, K), V = h.shape, W.shape[0]
     hc, Wc, b = _operands(h, W, bias, cdt)
     K8 = hc.shape[1]
-    grad = grad.to(lse.dtype).contiguous()
+    grad = grad.to(saved.dtype).contiguous()
     gh = torch.empty(N, K8, dtype=h.dtype, device=dev) if need_h else None
     gW_buf, gW = _grad_buffer(W, cdt, _tensor_core(cdt)) if need_W else (None, None)
     if need_W and K8 != K:
         gW_buf = torch.empty(V, K8, dtype=gW_buf.dtype, device=dev)
     gb = torch.empty(V, dtype=bias.dtype, device=dev) if need_b and bias is not None else None
-    gw = torch.empty(N, dtype=lse.dtype, device=dev) if need_w and weight is not None else None
-    p = _problem(hc, Wc, b, ids, logits, t_lse, weight, (sid, slogq, z, lse, qsum, each, stats), temperature, logit_scale,
-                 chunk, cdt, reduction)
+    gw = torch.empty(N, dtype=saved.dtype, device=dev) if need_w and weight is not None else None
+    p = _problem(hc, Wc, b, ids, logits, t_lse, weight, sid, saved, temperature, logit_scale, chunk, cdt, reduction)
     g = nat.DistillGrads()
     g.grad_out = grad.data_ptr()
     if gh is not None:
@@ -116,7 +105,7 @@ def _distill_bwd_op(grad: torch.Tensor, h: torch.Tensor, W: torch.Tensor, bias: 
     g.grad_weight = nat.ptr(gw)
     lib = nat.lib()
     nbytes = nat.c_size_t(0)
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         nat.check(lib.swvr_distill_bwd_workspace_size(p, g, nat.ctypes.byref(nbytes)), "swvr_distill_bwd_workspace_size")
         ws = _workspace(nbytes.value, dev)
         nat.check(lib.swvr_distill_bwd(p, g, ws.data_ptr(), ws.numel(), nat.stream_ptr(dev)), "swvr_distill_bwd")
@@ -124,36 +113,82 @@ def _distill_bwd_op(grad: torch.Tensor, h: torch.Tensor, W: torch.Tensor, bias: 
         gh = gh[:, :K].contiguous()
     if gW is not None and gW_buf is not gW:
         gW.copy_(gW_buf[:, :K])
-    return [t if t is not None else _no_grad_marker(h) for t in (gh, gW, gb, gw)]
+    return gh, gW, gb, gw
+
+
+# Custom-op pair, like the readout's own (ops.py), for torch.compile and other tracing.  The outputs after
+# the loss are what the backward needs of the forward: the sorted teacher ids and the values of
+# ``_problem``; they take no gradient.
+
+@torch.library.custom_op("swvr_b200::distill", mutates_args=())
+def _distill_op(h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], ids: torch.Tensor, logits: torch.Tensor,
+                t_lse: Optional[torch.Tensor], weight: Optional[torch.Tensor], temperature: float, logit_scale: float,
+                chunk: int, cdt: torch.dtype, reduction: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _distill_fwd(h, W, bias, ids, logits, t_lse, weight, temperature, logit_scale, chunk, cdt, reduction)
+
+
+@_distill_op.register_fake
+def _(h, W, bias, ids, logits, t_lse, weight, temperature, logit_scale, chunk, cdt, reduction):
+    adt = acc_dtype(cdt)
+    N, Kt = ids.shape
+    return (h.new_empty((N,) if reduction == nat.REDUCE_NONE else (), dtype=adt), h.new_empty((N, Kt), dtype=torch.int32),
+            h.new_empty((_saved_numel(N, Kt),), dtype=adt))
+
+
+@torch.library.custom_op("swvr_b200::distill_bwd", mutates_args=())
+def _distill_bwd_op(grad: torch.Tensor, h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor],
+                    ids: torch.Tensor, logits: torch.Tensor, t_lse: Optional[torch.Tensor],
+                    weight: Optional[torch.Tensor], sid: torch.Tensor, saved: torch.Tensor, temperature: float,
+                    logit_scale: float, chunk: int, cdt: torch.dtype, reduction: int, need_h: bool, need_W: bool,
+                    need_b: bool, need_w: bool) -> List[torch.Tensor]:
+    got = _distill_bwd(grad, h, W, bias, ids, logits, t_lse, weight, sid, saved, temperature, logit_scale, chunk, cdt,
+                       reduction, need_h, need_W, need_b, need_w)
+    return [t if t is not None else _no_grad_marker(h) for t in got]
 
 
 @_distill_bwd_op.register_fake
-def _(grad, h, W, bias, ids, logits, t_lse, weight, sid, slogq, z, lse, qsum, each, stats, temperature, logit_scale, chunk,
-      cdt, reduction, need_h, need_W, need_b, need_w):
+def _(grad, h, W, bias, ids, logits, t_lse, weight, sid, saved, temperature, logit_scale, chunk, cdt, reduction, need_h,
+      need_W, need_b, need_w):
     out = []
-    for wanted, like in ((need_h, h), (need_W, W), (need_b and bias is not None, bias),
-                         (need_w and weight is not None, lse)):
+    for wanted, like in ((need_h, h), (need_W, W), (need_b and bias is not None, bias)):
         out.append(like.new_empty(like.shape) if wanted else _no_grad_marker(h))
-    return out
+    return out + [saved.new_empty(h.shape[0]) if need_w and weight is not None else _no_grad_marker(h)]
 
 
-def _distill_setup(ctx, inputs, output):
+def _save(ctx, inputs, sid, saved):
     h, W, bias, ids, logits, t_lse, weight, *consts = inputs
-    ctx.save_for_backward(h, W, bias, ids, logits, t_lse, weight, *output[1:])
+    ctx.save_for_backward(h, W, bias, ids, logits, t_lse, weight, sid, saved)
     ctx.consts = consts
+    ctx.set_materialize_grads(False)
 
 
-def _distill_backward(ctx, grad, *_):
-    h, W, bias, ids, logits, t_lse, weight, *saved = ctx.saved_tensors
+def _grads(ctx, grad, run):
+    h, W, bias, ids, logits, t_lse, weight, sid, saved = ctx.saved_tensors
+    if grad is None:  # the loss did not reach what is differentiated
+        return (None,) * (7 + len(ctx.consts))
     want = [bool(ctx.needs_input_grad[i]) and t is not None for i, t in ((0, h), (1, W), (2, bias), (6, weight))]
-    if grad is None:
-        grad = torch.zeros(h.shape[0] if ctx.consts[4] == nat.REDUCE_NONE else (), dtype=saved[3].dtype, device=h.device)
-    got = _distill_bwd_op(grad, h, W, bias, ids, logits, t_lse, weight, *saved, *ctx.consts, *want)
+    got = run(grad, h, W, bias, ids, logits, t_lse, weight, sid, saved, *ctx.consts, *want)
     gh, gW, gb, gw = (t if w else None for t, w in zip(got, want))
     return (gh, gW, gb, None, None, None, gw) + (None,) * len(ctx.consts)
 
 
-_distill_op.register_autograd(_distill_backward, setup_context=_distill_setup)
+_distill_op.register_autograd(lambda ctx, grad, *_: _grads(ctx, grad, _distill_bwd_op),
+                              setup_context=lambda ctx, inputs, output: _save(ctx, inputs, *output[1:]))
+
+
+class _Distill(torch.autograd.Function):
+    """The custom op's forward and backward without its dispatch, for eager calls."""
+
+    @staticmethod
+    def forward(ctx, *inputs):
+        out, sid, saved = _distill_fwd(*inputs)
+        _save(ctx, inputs, sid, saved)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _grads(ctx, grad, _distill_bwd)
 
 
 def softmax_distill(h, W, teacher_ids, teacher_logits, bias=None, *, temperature=1.0, teacher_lse=None, weight=None,
@@ -210,11 +245,14 @@ def softmax_distill(h, W, teacher_ids, teacher_logits, bias=None, *, temperature
     adt = acc_dtype(cdt)
     N = math.prod(lead)
     row = lambda t: None if t is None else t.to(adt).reshape(N).contiguous()  # noqa: E731
-    with torch.autocast(h.device.type, enabled=False):
-        out = _distill_op(h.reshape(N, h.shape[-1]), W, bias, teacher_ids.reshape(N, Kt).contiguous(),
-                          teacher_logits.detach().reshape(N, Kt).contiguous(),
-                          None if teacher_lse is None else row(teacher_lse.detach()), row(weight), temperature,
-                          float(logit_scale), chunk, cdt, _REDUCTIONS[reduction])[0]
+    args = (h.reshape(N, h.shape[-1]), W, bias, teacher_ids.reshape(N, Kt).contiguous(),
+            teacher_logits.detach().reshape(N, Kt).contiguous(), None if teacher_lse is None else row(teacher_lse.detach()),
+            row(weight), temperature, float(logit_scale), chunk, cdt, _REDUCTIONS[reduction])
+    if _eager(*args[:7]):
+        out = _Distill.apply(*args)
+    else:
+        with torch.autocast(h.device.type, enabled=False):
+            out = _distill_op(*args)[0]
     return out.view(lead) if reduction == "none" else out
 
 

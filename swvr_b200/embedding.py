@@ -33,7 +33,7 @@ def _embed_fwd(tokens: torch.Tensor, E: torch.Tensor, scale: float) -> torch.Ten
     E = _unit_rows(E)
     tokens = tokens.contiguous()
     out = torch.empty(tokens.shape[0], E.shape[1], dtype=E.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         nat.check(nat.lib().swvr_embed_fwd(tokens.shape[0], E.shape[0], E.shape[1], tokens.data_ptr(),
                                            _TOKEN_BITS[tokens.dtype], E.data_ptr(), nat.dtype_code(E.dtype), _pitch(E),
                                            scale, out.data_ptr(), nat.stream_ptr(dev)), "swvr_embed_fwd")
@@ -48,7 +48,7 @@ def _embed_bwd(g: torch.Tensor, tokens: torch.Tensor, V: int, scale: float, padd
     dE = torch.empty(V, D, dtype=g.dtype, device=dev)
     lib = nat.lib()
     nbytes = nat.c_size_t(0)
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         nat.check(lib.swvr_embed_bwd_workspace_size(N, V, D, dt, nat.ctypes.byref(nbytes)),
                   "swvr_embed_bwd_workspace_size")
         ws = _workspace(nbytes.value, dev)
@@ -94,12 +94,27 @@ def _embed_backward(ctx, g):
 _embed_op.register_autograd(_embed_backward, setup_context=_embed_setup)
 
 
-def _plain_call(*tensors) -> bool:
-    """True where an op may be run without its custom op: no gradient, no tracing, plain tensors.  It
-    saves the dispatcher's host time, most of a call on a few tokens."""
-    grad = torch.is_grad_enabled()
+class _Embed(torch.autograd.Function):
+    """The custom op's forward and backward without its dispatch, for eager calls."""
+
+    @staticmethod
+    def forward(ctx, tokens, E, scale, padding):
+        ctx.save_for_backward(tokens)
+        ctx.consts = (E.shape[0], scale, padding)
+        return _embed_fwd(tokens, E, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (tokens,) = ctx.saved_tensors
+        return None, _embed_bwd(g, tokens, *ctx.consts), None, None
+
+
+def _eager(*tensors) -> bool:
+    """True where an op may be run without its custom op: no tracing, plain tensors.  It saves the
+    dispatcher's host time, most of a call on a few tokens."""
     return not torch.compiler.is_compiling() and all(
-        t is None or type(t) in (torch.Tensor, torch.nn.Parameter) and not (grad and t.requires_grad) for t in tensors)
+        t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
 
 
 def embedding_lookup(tokens, E, *, scale=1.0, padding_idx=None):
@@ -124,8 +139,5 @@ def embedding_lookup(tokens, E, *, scale=1.0, padding_idx=None):
             raise ValueError(f"padding_idx {padding_idx} is outside a table of {V} rows")
         padding += V if padding < 0 else 0
     flat = tokens.reshape(-1)
-    if _plain_call(flat, E):
-        out = _embed_fwd(flat, E, float(scale))
-    else:
-        out = _embed_op(flat, E, float(scale), padding)
+    out = (_Embed.apply if _eager(flat, E) else _embed_op)(flat, E, float(scale), padding)
     return out.view(*tokens.shape, E.shape[1])

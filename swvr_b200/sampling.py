@@ -17,7 +17,7 @@ import torch
 
 from . import _native as nat
 from .api import _compute_dtype
-from .embedding import _pitch, _plain_call, _unit_rows
+from .embedding import _pitch, _eager, _unit_rows
 from .ops import _ld, _prepare_k, _require_cuda, _workspace
 
 _INT_BITS = {torch.int64: 64, torch.int32: 32}
@@ -49,7 +49,7 @@ def _sample_logits(logits, u, T, top_k, top_p, min_p, Ts, ks, ps, ms, want_logpr
     logits = _unit_rows(logits)
     N, V = logits.shape
     s, keep, tokens, logprobs = _sampling(N, dev, u, T, top_k, top_p, min_p, Ts, ks, ps, ms, want_logprobs)
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         nat.check(nat.lib().swvr_sample_logits(N, V, logits.data_ptr(), nat.dtype_code(logits.dtype), _pitch(logits), s,
                                                nat.stream_ptr(dev)), "swvr_sample_logits")
     return tokens, logprobs
@@ -69,7 +69,7 @@ def _sample_head(h, W, bias, u, logit_scale, cdt, T, top_k, top_p, min_p, Ts, ks
     s, keep, tokens, logprobs = _sampling(hc.shape[0], dev, u, T, top_k, top_p, min_p, Ts, ks, ps, ms, want_logprobs)
     lib = nat.lib()
     nbytes = nat.c_size_t(0)
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         nat.check(lib.swvr_sample_workspace_size(p, nat.ctypes.byref(nbytes)), "swvr_sample_workspace_size")
         ws = _workspace(nbytes.value, dev)
         nat.check(lib.swvr_sample(p, s, ws.data_ptr(), ws.numel(), nat.stream_ptr(dev)), "swvr_sample")
@@ -166,7 +166,7 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     lead = logits.shape[:-1]
     args = _settings(lead, u, temperature, top_k, top_p, min_p)
     x, uu = logits.detach().reshape(math.prod(lead), logits.shape[-1]), u.detach().reshape(-1)
-    run = _sample_logits if _plain_call(x, uu) else _sample_logits_op
+    run = _sample_logits if _eager(x, uu) else _sample_logits_op
     return _shaped(run(x, uu, *args, bool(return_logprobs)), lead, return_logprobs)
 
 
@@ -192,7 +192,7 @@ def softmax_sample(h, W, u, bias=None, *, temperature=1.0, top_k=None, top_p=Non
     args = _settings(lead, u, temperature, top_k, top_p, min_p)
     h2, W2 = h.detach().reshape(math.prod(lead), h.shape[-1]), W.detach()
     b, uu = None if bias is None else bias.detach(), u.detach().reshape(-1)
-    run = _sample_head if _plain_call(h2, W2, b, uu) else _sample_op
+    run = _sample_head if _eager(h2, W2, b, uu) else _sample_op
     with torch.autocast(h.device.type, enabled=False):
         out = run(h2, W2, b, uu, float(logit_scale), cdt, *args, bool(return_logprobs))
     return _shaped(out, lead, return_logprobs)

@@ -64,7 +64,7 @@ def _problem(N=256, K=64, V=1000, Kt=8, dt=nat.BF16, buf=1 << 20, **kw):
     p = nat.Distill()
     p.n_tokens, p.hidden, p.vocab, p.teacher = N, K, V, Kt
     p.compute_dtype, p.bias_dtype, p.teacher_dtype, p.id_bits = dt, nat.F32, nat.F32, 64
-    p.h = p.W = p.teacher_ids = p.teacher_logits = p.slogq = p.z = p.lse = p.qsum = p.each = p.stats = p.sid = buf
+    p.h = p.W = p.teacher_ids = p.teacher_logits = p.slogq = p.z = p.lse = p.lse_lo = p.qsum = p.each = p.stats = p.sid = buf
     p.ldh = p.ldw = K
     p.logit_scale = p.temperature = 1.0
     p.chunk, p.reduction = 8192, nat.REDUCE_MEAN
@@ -130,7 +130,7 @@ def test_distill_fake_impls_give_shapes(dtype, adt):
     h, W, b, ids, t, w = m(6, 16), m(100, 16), m(100), m(6, 5, dt=torch.int64), m(6, 5, dt=torch.float32), m(6, dt=adt)
     out, *saved = torch.ops.swvr_b200.distill(h, W, b, ids, t, None, w, 2.0, 1.0, 8192, dtype, nat.REDUCE_MEAN)
     assert out.shape == () and out.dtype == adt
-    assert [tuple(s.shape) for s in saved] == [(6, 5)] * 3 + [(6,)] * 3 + [(2,)] and saved[0].dtype == torch.int32
+    assert [tuple(s.shape) for s in saved] == [(6, 5), (2 * 30 + 4 * 6 + 2,)] and saved[0].dtype == torch.int32
     none = torch.ops.swvr_b200.distill(h, W, b, ids, t, None, w, 2.0, 1.0, 8192, dtype, nat.REDUCE_NONE)[0]
     assert none.shape == (6,)
     grads = torch.ops.swvr_b200.distill_bwd(out, h, W, b, ids, t, None, w, *saved, 2.0, 1.0, 8192, dtype, nat.REDUCE_MEAN,
