@@ -45,29 +45,42 @@ __device__ __forceinline__ int64_t load_token(const void* tokens, int bits, int6
 }
 
 // ------------------------------------------------------------------ lookup
-// One thread per pack of a row: consecutive threads copy consecutive packs.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) lookup_kernel(int64_t total, int packs, int64_t V, const void* __restrict__ tokens,
+// blockDim.x threads own packs of a row, blockDim.y rows share a block; ROWS rows a thread, loaded before any is
+// stored.  Bound by HBM: 16384 rows of 2560 bf16 (168 MB in and out) in 27 us (31 us with one row a thread).
+template <typename T, int VEC, int ROWS>
+__global__ void __launch_bounds__(256) lookup_kernel(int64_t n, int packs, int64_t V, const void* __restrict__ tokens,
                                                      int bits, const T* __restrict__ E, int64_t lde,
                                                      typename Acc<T>::type scale, T* __restrict__ out) {
   using A = typename Acc<T>::type;
   using P = Pack<T, VEC>;
-  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= total) return;
-  const int64_t n = i / packs;
-  const int64_t c = (i - n * packs) * VEC;
-  const int64_t tok = load_token(tokens, bits, n);
-  P p;
-  if (tok >= 0 && tok < V) {
-    p = *reinterpret_cast<const P*>(E + tok * lde + c);
+  const int pk = blockIdx.y * blockDim.x + threadIdx.x;
+  if (pk >= packs) return;
+  const int64_t c = static_cast<int64_t>(pk) * VEC, D = static_cast<int64_t>(packs) * VEC;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (blockDim.y * ROWS) + threadIdx.y;
+  int64_t tok[ROWS];
+  P p[ROWS];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) from_acc(to_acc(p.v[k]) * scale, &p.v[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) from_acc(static_cast<A>(NAN), &p.v[k]);
-    atomicCAS(&g_device_error, 0u, kErrToken | 1u);
+  for (int r = 0; r < ROWS; ++r) {
+    const int64_t i = row0 + r * static_cast<int>(blockDim.y);
+    tok[r] = i < n ? load_token(tokens, bits, i) : -1;
   }
-  *reinterpret_cast<P*>(out + i * VEC) = p;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+    if (tok[r] >= 0 && tok[r] < V) p[r] = *reinterpret_cast<const P*>(E + tok[r] * lde + c);
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int64_t i = row0 + r * static_cast<int>(blockDim.y);
+    if (i >= n) return;
+    if (tok[r] >= 0 && tok[r] < V) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) from_acc(to_acc(p[r].v[k]) * scale, &p[r].v[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) from_acc(static_cast<A>(NAN), &p[r].v[k]);
+      atomicCAS(&g_device_error, 0u, kErrToken | 1u);
+    }
+    *reinterpret_cast<P*>(out + i * D + c) = p[r];
+  }
 }
 
 // ------------------------------------------------------------------ stable sort by token
@@ -211,6 +224,115 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(int64_t n, S
   }
 }
 
+// Up to kSmallSort pairs: one block sorts them in shared memory while the other blocks of the launch clear dE, which takes
+// longer where it matters (778 MB: 125 us; the sort of 16384 pairs with 18-bit keys: 14 us).  Pairs stay in registers, `digit`
+// bits a pass; warp w owns items [w * 32 * ITEMS, ...), so ranks follow the list order as above.
+constexpr int kSmallThreads = 1024, kSmallSort = 16 * kSmallThreads, kSmallDigits = 512;
+
+struct SmallSmem {
+  uint16_t cnt[kSmallThreads / 32][kSmallDigits];  // pairs per warp and digit, then where each warp's go
+  uint32_t warp_sum[kSmallThreads / 32];
+};
+
+template <int ITEMS>
+__device__ __forceinline__ void small_sort(int n, const SortIn& in, int bits, int digit, unsigned char* smem, uint32_t* key_out,
+                                           uint32_t* pos_out) {
+  SmallSmem& s = *reinterpret_cast<SmallSmem*>(smem);
+  uint32_t* sk = reinterpret_cast<uint32_t*>(smem + sizeof(SmallSmem));
+  uint32_t* sp = sk + ITEMS * kSmallThreads;
+  const int t = threadIdx.x, lane = t % 32, warp = t / 32, base = warp * 32 * ITEMS;
+  const int digits = 1 << digit;
+  uint32_t key[ITEMS], pos[ITEMS], rank[ITEMS];
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    const int i = base + r * 32 + lane;
+    key[r] = i < n ? sort_key(in, i) : 0u;
+    pos[r] = i;
+  }
+  for (int shift = 0;; shift += digit) {
+    for (int i = t; i < (kSmallThreads / 32) * digits; i += kSmallThreads) s.cnt[i / digits][i % digits] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+      const bool have = base + r * 32 + lane < n;
+      uint32_t same = __ballot_sync(0xffffffffu, have);
+      const uint32_t d = (key[r] >> shift) & (digits - 1u);
+      for (int b = 0; b < digit; ++b) {
+        const uint32_t ones = __ballot_sync(0xffffffffu, (d >> b) & 1u);
+        same &= ((d >> b) & 1u) ? ones : ~ones;
+      }
+      rank[r] = 0;
+      if (have) rank[r] = s.cnt[warp][d] + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+      if (have && (same >> lane) == 1u) s.cnt[warp][d] = static_cast<uint16_t>(rank[r] + 1u);  // the group's last lane
+      __syncwarp();
+    }
+    __syncthreads();
+    // digit t's total over the warps, its exclusive prefix over the digits, then each warp's start
+    uint32_t total = 0;
+    if (t < digits)
+#pragma unroll 8
+      for (int w = 0; w < kSmallThreads / 32; ++w) total += s.cnt[w][t];
+    uint32_t inc = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) s.warp_sum[warp] = inc;
+    __syncthreads();
+    uint32_t run = inc - total;
+    for (int w = 0; w < warp; ++w) run += s.warp_sum[w];
+    if (t < digits)
+#pragma unroll 8
+      for (int w = 0; w < kSmallThreads / 32; ++w) {
+        const uint32_t c = s.cnt[w][t];
+        s.cnt[w][t] = static_cast<uint16_t>(run);  // below n, which fits
+        run += c;
+      }
+    __syncthreads();
+    const bool last = shift + digit >= bits;
+    uint32_t* ko = last ? key_out : sk;
+    uint32_t* po = last ? pos_out : sp;
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+      if (base + r * 32 + lane < n) {
+        const uint32_t o = s.cnt[warp][(key[r] >> shift) & (digits - 1u)] + rank[r];
+        ko[o] = key[r];
+        po[o] = pos[r];
+      }
+    }
+    if (last) return;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+      const int i = base + r * 32 + lane;
+      if (i < n) {
+        key[r] = sk[i];
+        pos[r] = sp[i];
+      }
+    }
+  }
+}
+
+// Block 0 sorts; the others clear `bytes` bytes from dE (16-byte aligned) on.
+template <int ITEMS>
+__global__ void __launch_bounds__(kSmallThreads)
+    sort_fill_kernel(int n, SortIn in, int bits, int digit, uint32_t* key, uint32_t* pos, unsigned char* dE, int64_t bytes) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  if (blockIdx.x == 0) {
+    small_sort<ITEMS>(n, in, bits, digit, smem_raw, key, pos);
+    return;
+  }
+  const int64_t step = static_cast<int64_t>(gridDim.x - 1) * kSmallThreads;
+  const int64_t at = static_cast<int64_t>(blockIdx.x - 1) * kSmallThreads + threadIdx.x;
+  uint4* d = reinterpret_cast<uint4*>(dE);
+  const int64_t vecs = bytes / 16;
+#pragma unroll 4
+  for (int64_t i = at; i < vecs; i += step) d[i] = make_uint4(0, 0, 0, 0);
+  if (at < bytes % 16) dE[vecs * 16 + at] = 0;
+}
+
 // ------------------------------------------------------------------ sums by token
 // A chunk is `len` consecutive sorted pairs.  TX threads own the packs of a row, TY chunks share a
 // block.  A token that begins and ends inside a chunk is written to dE at once; the part of
@@ -281,48 +403,72 @@ __global__ void __launch_bounds__(256) sum_kernel(int64_t n, int len, int chunks
   }
 }
 
-// Adds the pieces of each token that spans chunks, in chunk order: one block (row of threads) per
-// chunk in which such a token begins.
+// Adds the pieces of each token that spans chunks, in a fixed order: a block for each chunk in which such a token
+// begins, 32 threads wide; 16 groups of threads take every 16th of the pieces that follow, and the groups'
+// sums are added in group order (one row of threads adding them all took 38 us for a token of 82 pieces).
+constexpr int kJoinGroups = 16;
+
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) join_kernel(int64_t n, int len, int chunks, int packs, uint32_t V,
-                                                   const uint32_t* __restrict__ key,
-                                                   typename Acc<T>::type scale, T* __restrict__ dE, int64_t lde,
-                                                   const typename Acc<T>::type* __restrict__ part) {
+__global__ void __launch_bounds__(32 * kJoinGroups)
+    join_kernel(int64_t n, int len, int chunks, int packs, uint32_t V, const uint32_t* __restrict__ key,
+                typename Acc<T>::type scale, T* __restrict__ dE, int64_t lde,
+                const typename Acc<T>::type* __restrict__ part) {
   using A = typename Acc<T>::type;
   using P = Pack<T, VEC>;
-  const int64_t chunk = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  const int pk = blockIdx.y * blockDim.x + threadIdx.x;
-  if (chunk >= chunks || pk >= packs) return;
+  __shared__ A sums[kJoinGroups][32][VEC + 1];
+  const int64_t chunk = blockIdx.x;
   const int64_t i0 = chunk * len, i1 = min(n, i0 + len);
   if (i1 >= n) return;
   const uint32_t cur = key[i1 - 1];
   if (cur >= V || key[i1] != cur) return;                       // nothing goes on
   if (i0 > 0 && key[i0] == cur && key[i0 - 1] == cur) return;   // it began earlier
-  const int64_t c = static_cast<int64_t>(pk) * VEC, D = static_cast<int64_t>(packs) * VEC;
-  A acc[VEC];
+  const int64_t D = static_cast<int64_t>(packs) * VEC;
+  for (int pk0 = blockIdx.y * 32; pk0 < packs; pk0 += gridDim.y * 32) {
+    const int pk = pk0 + threadIdx.x;
+    const int64_t c = static_cast<int64_t>(pk) * VEC;
+    A acc[VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] = part[(chunk * 2 + 1) * D + c + k];
-  for (int64_t j = chunk + 1; j < chunks && key[j * len] == cur; ++j)
+    for (int k = 0; k < VEC; ++k) acc[k] = A(0);
+    if (pk < packs) {
+      if (threadIdx.y == 0)
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += part[j * 2 * D + c + k];
-  P o;
+        for (int k = 0; k < VEC; ++k) acc[k] = part[(chunk * 2 + 1) * D + c + k];
+#pragma unroll 2
+      for (int64_t j = chunk + 1 + threadIdx.y; j < chunks && key[j * len] == cur; j += kJoinGroups)
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) from_acc(acc[k] * scale, &o.v[k]);
-  *reinterpret_cast<P*>(dE + static_cast<int64_t>(cur) * lde + c) = o;
+        for (int k = 0; k < VEC; ++k) acc[k] += part[j * 2 * D + c + k];
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sums[threadIdx.y][threadIdx.x][k] = acc[k];
+    __syncthreads();
+    if (threadIdx.y == 0 && pk < packs) {
+#pragma unroll
+      for (int g = 1; g < kJoinGroups; ++g)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += sums[g][threadIdx.x][k];
+      P o;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) from_acc(acc[k] * scale, &o.v[k]);
+      *reinterpret_cast<P*>(dE + static_cast<int64_t>(cur) * lde + c) = o;
+    }
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------------------ host
 struct BwdPlan {
-  int tiles, passes, len, chunks;
+  int tiles, bits, passes, len, chunks;
+  bool small;  // one block sorts
   size_t off_key[2], off_pos[2], off_counts, off_part, bytes;
 };
 
 static BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D, int dt) {
   BwdPlan b{};
   b.tiles = static_cast<int>(ceil_div(std::max<int64_t>(n, 1), kSortTile));
-  int bits = 1;
-  while ((V >> bits) != 0) ++bits;  // keys 0 .. V
-  b.passes = (bits + 7) / 8;
+  b.bits = 1;
+  while ((V >> b.bits) != 0) ++b.bits;  // keys 0 .. V
+  b.passes = (b.bits + 7) / 8;
+  b.small = n <= kSmallSort;
   // chunks of 16 pairs, longer where that gives more than 2048 of them
   b.len = static_cast<int>(std::min<int64_t>(512, std::max<int64_t>(16, ceil_div(n, 2048))));
   b.chunks = static_cast<int>(ceil_div(std::max<int64_t>(n, 1), b.len));
@@ -345,13 +491,28 @@ static bool rows16(const void* p, int64_t ld, int64_t D, size_t es) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * es) % 16 == 0 && (D * es) % 16 == 0;
 }
 
+// Threads across a row: the widest of 256, 128, 64, 32 that leaves the fewest of them idle.
+static int row_threads(int packs) {
+  int best = 32;
+  for (int tx : {64, 128, 256})
+    if (round_up(packs, tx) <= round_up(packs, best)) best = tx;
+  return best;
+}
+
 template <typename T, int VEC>
 static cudaError_t lookup(int64_t n, int64_t V, int64_t D, const void* tokens, int bits, const void* E, int64_t lde,
                           double scale, void* out, cudaStream_t st) {
-  const int64_t packs = D / VEC, total = n * packs;
-  lookup_kernel<T, VEC><<<static_cast<unsigned>(ceil_div(total, 256)), 256, 0, st>>>(
-      total, static_cast<int>(packs), V, tokens, bits, static_cast<const T*>(E), lde,
-      static_cast<typename Acc<T>::type>(scale), static_cast<T*>(out));
+  using A = typename Acc<T>::type;
+  const int packs = static_cast<int>(D / VEC), tx = row_threads(packs);
+  const dim3 block(tx, 256 / tx);
+  const unsigned gy = static_cast<unsigned>(ceil_div(packs, tx));
+  // several rows a thread once one each would be over eight blocks an SM
+  if (ceil_div(n, block.y) * gy > 8 * kNumSMsB200)
+    lookup_kernel<T, VEC, 4><<<dim3(static_cast<unsigned>(ceil_div(n, block.y * 4)), gy), block, 0, st>>>(
+        n, packs, V, tokens, bits, static_cast<const T*>(E), lde, static_cast<A>(scale), static_cast<T*>(out));
+  else
+    lookup_kernel<T, VEC, 1><<<dim3(static_cast<unsigned>(ceil_div(n, block.y)), gy), block, 0, st>>>(
+        n, packs, V, tokens, bits, static_cast<const T*>(E), lde, static_cast<A>(scale), static_cast<T*>(out));
   return cudaGetLastError();
 }
 
@@ -368,9 +529,7 @@ template <typename T, int VEC>
 static cudaError_t sums(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const uint32_t* key, const uint32_t* pos,
                         const void* g, int64_t ldg, double scale, void* dE, int64_t lde, void* part, cudaStream_t st) {
   using A = typename Acc<T>::type;
-  const int packs = static_cast<int>(D / VEC);
-  int tx = 8;
-  while (tx < packs && tx < 256) tx *= 2;
+  const int packs = static_cast<int>(D / VEC), tx = row_threads(packs);
   const dim3 block(tx, 256 / tx);
   const dim3 grid(static_cast<unsigned>(ceil_div(b.chunks, block.y)), static_cast<unsigned>(ceil_div(packs, tx)));
   sum_kernel<T, VEC><<<grid, block, 0, st>>>(n, b.len, b.chunks, packs, static_cast<uint32_t>(V), key, pos,
@@ -378,7 +537,8 @@ static cudaError_t sums(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const
                                              lde, static_cast<A*>(part));
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  join_kernel<T, VEC><<<grid, block, 0, st>>>(n, b.len, b.chunks, packs, static_cast<uint32_t>(V), key,
+  join_kernel<T, VEC><<<dim3(static_cast<unsigned>(b.chunks), static_cast<unsigned>(std::min<int64_t>(ceil_div(packs, 32), 64))),
+                        dim3(32, kJoinGroups), 0, st>>>(n, b.len, b.chunks, packs, static_cast<uint32_t>(V), key,
                                               static_cast<A>(scale), static_cast<T*>(dE), lde,
                                               static_cast<const A*>(part));
   return cudaGetLastError();
@@ -388,20 +548,42 @@ template <typename T>
 static cudaError_t bwd(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const void* tokens, int bits, const void* g,
                        int64_t ldg, double scale, int64_t padding, void* dE, int64_t lde, char* ws, cudaStream_t st) {
   constexpr int VEC = 16 / sizeof(T);
-  cudaError_t e = lde == D ? cudaMemsetAsync(dE, 0, sizeof(T) * V * D, st)
-                           : cudaMemset2DAsync(dE, lde * sizeof(T), 0, D * sizeof(T), V, st);
-  if (e != cudaSuccess || n == 0) return e;
-  uint32_t* counts = reinterpret_cast<uint32_t*>(ws + b.off_counts);
+  cudaError_t e = cudaSuccess;
   SortIn in{tokens, bits, V, padding, nullptr, nullptr};
-  for (int p = 0; p < b.passes; ++p) {
-    uint32_t* ko = reinterpret_cast<uint32_t*>(ws + b.off_key[p & 1]);
-    uint32_t* po = reinterpret_cast<uint32_t*>(ws + b.off_pos[p & 1]);
-    sort_hist_kernel<<<b.tiles, kSortThreads, 0, st>>>(n, in, 8 * p, b.tiles, counts);
-    sort_scan_kernel<<<1, 1024, 0, st>>>(static_cast<int64_t>(b.tiles) * kDigits, counts);
-    sort_scatter_kernel<<<b.tiles, kSortThreads, 0, st>>>(n, in, 8 * p, b.tiles, counts, ko, po);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    in.key = ko;
-    in.pos = po;
+  uint32_t* key[2] = {reinterpret_cast<uint32_t*>(ws + b.off_key[0]), reinterpret_cast<uint32_t*>(ws + b.off_key[1])};
+  uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + b.off_pos[0]), reinterpret_cast<uint32_t*>(ws + b.off_pos[1])};
+  if (b.small && n > 0 && lde == D && (reinterpret_cast<uintptr_t>(dE) & 15u) == 0) {
+    const int passes = (b.bits + 8) / 9, digit = (b.bits + passes - 1) / passes;  // at most 9 bits each
+    const int64_t bytes = V * D * static_cast<int64_t>(sizeof(T));
+    auto launch = [&](auto kern, int items) {
+      const int smem = static_cast<int>(sizeof(SmallSmem)) + items * kSmallThreads * 8;
+      cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (r != cudaSuccess) return r;
+      const int64_t fill = std::min<int64_t>(kNumSMsB200 - 1, ceil_div(bytes, 16 * kSmallThreads));
+      kern<<<static_cast<unsigned>(1 + fill), kSmallThreads, smem, st>>>(static_cast<int>(n), in, b.bits, digit, key[0], pos[0],
+                                                                         static_cast<unsigned char*>(dE), bytes);
+      return cudaGetLastError();
+    };
+    e = n <= 2 * kSmallThreads   ? launch(sort_fill_kernel<2>, 2)
+        : n <= 8 * kSmallThreads ? launch(sort_fill_kernel<8>, 8)
+                                 : launch(sort_fill_kernel<16>, 16);
+    if (e != cudaSuccess) return e;
+    in.key = key[0];
+    in.pos = pos[0];
+  } else {
+    e = lde == D ? cudaMemsetAsync(dE, 0, sizeof(T) * V * D, st)
+                 : cudaMemset2DAsync(dE, lde * sizeof(T), 0, D * sizeof(T), V, st);
+    if (e != cudaSuccess || n == 0) return e;
+    uint32_t* counts = reinterpret_cast<uint32_t*>(ws + b.off_counts);
+    for (int p = 0; p < b.passes; ++p) {
+      uint32_t *ko = key[p & 1], *po = pos[p & 1];
+      sort_hist_kernel<<<b.tiles, kSortThreads, 0, st>>>(n, in, 8 * p, b.tiles, counts);
+      sort_scan_kernel<<<1, 1024, 0, st>>>(static_cast<int64_t>(b.tiles) * kDigits, counts);
+      sort_scatter_kernel<<<b.tiles, kSortThreads, 0, st>>>(n, in, 8 * p, b.tiles, counts, ko, po);
+      if ((e = cudaGetLastError()) != cudaSuccess) return e;
+      in.key = ko;
+      in.pos = po;
+    }
   }
   char* part = ws + b.off_part;
   if (rows16(g, ldg, D, sizeof(T)) && rows16(dE, lde, D, sizeof(T)))
@@ -416,7 +598,7 @@ static int check_sizes(int64_t n, int64_t V, int64_t D, int bits, int dt, int64_
   if (bits != 32 && bits != 64) return fail(SWVR_ERR_INVALID_ARGUMENT, "tokens must be 32- or 64-bit integers");
   if (dt < SWVR_F32 || dt > SWVR_F16) return fail(SWVR_ERR_INVALID_ARGUMENT, "unknown dtype %d", dt);
   if (lde < D) return fail(SWVR_ERR_INVALID_ARGUMENT, "row stride smaller than the row length");
-  if (ceil_div(n * D, 256) >= (1ll << 31)) return fail(SWVR_ERR_UNSUPPORTED, "n_tokens x dim too large");
+  if (ceil_div(n, 8) * ceil_div(D, 32) >= (1ll << 40) || ceil_div(D, 32) > 65535) return fail(SWVR_ERR_UNSUPPORTED, "n_tokens x dim too large");
   return SWVR_OK;
 }
 
@@ -463,7 +645,7 @@ int swvr_embed_bwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tok
     return fail(SWVR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, b.bytes);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  ProfScope ps(kProfEmbed, st, n_tokens > 0 ? 3 * b.passes + 2 : 0);
+  ProfScope ps(kProfEmbed, st, n_tokens > 0 ? (b.small ? 1 : 3 * b.passes) + 2 : 0);
   switch (dtype) {
     case SWVR_F32:
       SWVR_CUDA(embed::bwd<float>(b, n_tokens, vocab, dim, tokens, token_bits, grad_out, ld_grad_out, scale, padding_idx,
