@@ -497,8 +497,7 @@ template <typename A>
 static cudaError_t teacher_rows(const swvr_distill& p, cudaStream_t st) {
   const size_t smem = static_cast<size_t>(kWarps) * p.teacher * (sizeof(A) + 4);
   auto kern = teacher_kernel<A>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kWarps * kMaxTeacher * (static_cast<int>(sizeof(A)) + 4));
+  const cudaError_t e = tc::allow_smem(reinterpret_cast<const void*>(kern), kWarps * kMaxTeacher * (static_cast<int>(sizeof(A)) + 4));
   if (e != cudaSuccess) return e;
   kern<<<static_cast<unsigned>(ceil_div(p.n_tokens, kWarps)), 32 * kWarps, smem, st>>>(
       p.n_tokens, p.vocab, static_cast<int>(p.teacher), p.teacher_ids, p.id_bits, p.teacher_logits, p.teacher_dtype,

@@ -12,6 +12,7 @@
 
 #include "common.cuh"
 #include "ptx.cuh"
+#include "tc.cuh"
 
 namespace swvr {
 namespace embed {
@@ -318,9 +319,11 @@ __device__ __forceinline__ void small_sort(int n, const SortIn& in, int bits, in
 // Block 0 sorts; the others clear `bytes` bytes from dE (16-byte aligned) on.
 template <int ITEMS>
 __global__ void __launch_bounds__(kSmallThreads)
-    sort_fill_kernel(int n, SortIn in, int bits, int digit, uint32_t* key, uint32_t* pos, unsigned char* dE, int64_t bytes) {
+    sort_fill_kernel(int n, SortIn in, int bits, int digit, uint32_t* key, uint32_t* pos, uint32_t* joins,
+                     unsigned char* dE, int64_t bytes) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *joins = 0;
     small_sort<ITEMS>(n, in, bits, digit, smem_raw, key, pos);
     return;
   }
@@ -337,13 +340,14 @@ __global__ void __launch_bounds__(kSmallThreads)
 // A chunk is `len` consecutive sorted pairs.  TX threads own the packs of a row, TY chunks share a
 // block.  A token that begins and ends inside a chunk is written to dE at once; the part of
 // the chunk's first token that began earlier goes to part[chunk][0], the part of its last token
-// that goes on (and began here) to part[chunk][1].
+// that goes on (and began here) to part[chunk][1], and the chunk to the list of those that join_kernel starts from (in any
+// order: each is joined by itself).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) sum_kernel(int64_t n, int len, int chunks, int packs, uint32_t V,
                                                   const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
                                                   const T* __restrict__ g, int64_t ldg,
                                                   typename Acc<T>::type scale, T* __restrict__ dE, int64_t lde,
-                                                  typename Acc<T>::type* __restrict__ part) {
+                                                  typename Acc<T>::type* __restrict__ part, uint32_t* joins) {
   using A = typename Acc<T>::type;
   using P = Pack<T, VEC>;
   const int64_t chunk = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
@@ -392,6 +396,7 @@ __global__ void __launch_bounds__(256) sum_kernel(int64_t n, int len, int chunks
   const bool goes_on = i1 < n && key[i1] == cur;
   if (first || goes_on) {
     // a token that fills the whole chunk and goes on is a middle piece: slot 0
+    if (goes_on && !first && pk == 0) joins[1 + atomicAdd(joins, 1u)] = static_cast<uint32_t>(chunk);
     A* dst = part + (chunk * 2 + (first ? 0 : 1)) * D + c;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) dst[k] = acc[k];
@@ -403,28 +408,25 @@ __global__ void __launch_bounds__(256) sum_kernel(int64_t n, int len, int chunks
   }
 }
 
-// Adds the pieces of each token that spans chunks, in a fixed order: a block for each chunk in which such a token
-// begins, 32 threads wide; 16 groups of threads take every 16th of the pieces that follow, and the groups'
-// sums are added in group order (one row of threads adding them all took 38 us for a token of 82 pieces).
+// Adds the pieces of each token that spans chunks, in a fixed order: a block (32 packs wide) for each chunk in which
+// such a token begins; 16 groups of threads take every 16th of the pieces that follow, and the groups' sums are added in
+// group order.  16384 tokens, one of 82 pieces: 38 us by one row of threads per chunk.
 constexpr int kJoinGroups = 16;
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(32 * kJoinGroups)
-    join_kernel(int64_t n, int len, int chunks, int packs, uint32_t V, const uint32_t* __restrict__ key,
+    join_kernel(int len, int chunks, int packs, const uint32_t* __restrict__ key,
                 typename Acc<T>::type scale, T* __restrict__ dE, int64_t lde,
-                const typename Acc<T>::type* __restrict__ part) {
+                const typename Acc<T>::type* __restrict__ part, const uint32_t* __restrict__ joins) {
   using A = typename Acc<T>::type;
   using P = Pack<T, VEC>;
   __shared__ A sums[kJoinGroups][32][VEC + 1];
-  const int64_t chunk = blockIdx.x;
-  const int64_t i0 = chunk * len, i1 = min(n, i0 + len);
-  if (i1 >= n) return;
-  const uint32_t cur = key[i1 - 1];
-  if (cur >= V || key[i1] != cur) return;                       // nothing goes on
-  if (i0 > 0 && key[i0] == cur && key[i0 - 1] == cur) return;   // it began earlier
   const int64_t D = static_cast<int64_t>(packs) * VEC;
-  for (int pk0 = blockIdx.y * 32; pk0 < packs; pk0 += gridDim.y * 32) {
-    const int pk = pk0 + threadIdx.x;
+  const uint32_t wide = (packs + 31) / 32, work = joins[0] * wide;  // (chunk, 32 packs) pairs
+  for (uint32_t u = blockIdx.x; u < work; u += gridDim.x) {
+    const int64_t chunk = joins[1 + u / wide];
+    const uint32_t cur = key[chunk * len + len - 1];  // it goes on, so the chunk is full
+    const int pk = u % wide * 32 + threadIdx.x;
     const int64_t c = static_cast<int64_t>(pk) * VEC;
     A acc[VEC];
 #pragma unroll
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(32 * kJoinGroups)
 struct BwdPlan {
   int tiles, bits, passes, len, chunks;
   bool small;  // one block sorts
-  size_t off_key[2], off_pos[2], off_counts, off_part, bytes;
+  size_t off_key[2], off_pos[2], off_counts, off_joins, off_part, bytes;
 };
 
 static BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D, int dt) {
@@ -481,6 +483,8 @@ static BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D, int dt) {
   }
   b.off_counts = off;
   off += align_up(static_cast<size_t>(b.tiles) * kDigits * 4, 256);
+  b.off_joins = off;
+  off += align_up((static_cast<size_t>(b.chunks) + 1) * 4, 256);
   b.off_part = off;
   off += align_up(static_cast<size_t>(b.chunks) * 2 * D * (dt == SWVR_F64 ? 8 : 4), 256);
   b.bytes = off + 256;
@@ -527,20 +531,20 @@ static cudaError_t fwd(int64_t n, int64_t V, int64_t D, const void* tokens, int 
 
 template <typename T, int VEC>
 static cudaError_t sums(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const uint32_t* key, const uint32_t* pos,
-                        const void* g, int64_t ldg, double scale, void* dE, int64_t lde, void* part, cudaStream_t st) {
+                        const void* g, int64_t ldg, double scale, void* dE, int64_t lde, void* part, uint32_t* joins,
+                        cudaStream_t st) {
   using A = typename Acc<T>::type;
   const int packs = static_cast<int>(D / VEC), tx = row_threads(packs);
   const dim3 block(tx, 256 / tx);
   const dim3 grid(static_cast<unsigned>(ceil_div(b.chunks, block.y)), static_cast<unsigned>(ceil_div(packs, tx)));
   sum_kernel<T, VEC><<<grid, block, 0, st>>>(n, b.len, b.chunks, packs, static_cast<uint32_t>(V), key, pos,
                                              static_cast<const T*>(g), ldg, static_cast<A>(scale), static_cast<T*>(dE),
-                                             lde, static_cast<A*>(part));
+                                             lde, static_cast<A*>(part), joins);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  join_kernel<T, VEC><<<dim3(static_cast<unsigned>(b.chunks), static_cast<unsigned>(std::min<int64_t>(ceil_div(packs, 32), 64))),
-                        dim3(32, kJoinGroups), 0, st>>>(n, b.len, b.chunks, packs, static_cast<uint32_t>(V), key,
-                                              static_cast<A>(scale), static_cast<T*>(dE), lde,
-                                              static_cast<const A*>(part));
+  const int64_t work = ceil_div(packs, 32) * b.chunks;
+  join_kernel<T, VEC><<<static_cast<unsigned>(std::min<int64_t>(work, 4 * kNumSMsB200)), dim3(32, kJoinGroups), 0, st>>>(
+      b.len, b.chunks, packs, key, static_cast<A>(scale), static_cast<T*>(dE), lde, static_cast<const A*>(part), joins);
   return cudaGetLastError();
 }
 
@@ -550,6 +554,7 @@ static cudaError_t bwd(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const 
   constexpr int VEC = 16 / sizeof(T);
   cudaError_t e = cudaSuccess;
   SortIn in{tokens, bits, V, padding, nullptr, nullptr};
+  uint32_t* joins = reinterpret_cast<uint32_t*>(ws + b.off_joins);
   uint32_t* key[2] = {reinterpret_cast<uint32_t*>(ws + b.off_key[0]), reinterpret_cast<uint32_t*>(ws + b.off_key[1])};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + b.off_pos[0]), reinterpret_cast<uint32_t*>(ws + b.off_pos[1])};
   if (b.small && n > 0 && lde == D && (reinterpret_cast<uintptr_t>(dE) & 15u) == 0) {
@@ -557,10 +562,10 @@ static cudaError_t bwd(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const 
     const int64_t bytes = V * D * static_cast<int64_t>(sizeof(T));
     auto launch = [&](auto kern, int items) {
       const int smem = static_cast<int>(sizeof(SmallSmem)) + items * kSmallThreads * 8;
-      cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      const cudaError_t r = tc::allow_smem(reinterpret_cast<const void*>(kern), smem);
       if (r != cudaSuccess) return r;
       const int64_t fill = std::min<int64_t>(kNumSMsB200 - 1, ceil_div(bytes, 16 * kSmallThreads));
-      kern<<<static_cast<unsigned>(1 + fill), kSmallThreads, smem, st>>>(static_cast<int>(n), in, b.bits, digit, key[0], pos[0],
+      kern<<<static_cast<unsigned>(1 + fill), kSmallThreads, smem, st>>>(static_cast<int>(n), in, b.bits, digit, key[0], pos[0], joins,
                                                                          static_cast<unsigned char*>(dE), bytes);
       return cudaGetLastError();
     };
@@ -574,6 +579,7 @@ static cudaError_t bwd(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const 
     e = lde == D ? cudaMemsetAsync(dE, 0, sizeof(T) * V * D, st)
                  : cudaMemset2DAsync(dE, lde * sizeof(T), 0, D * sizeof(T), V, st);
     if (e != cudaSuccess || n == 0) return e;
+    if ((e = cudaMemsetAsync(joins, 0, 4, st)) != cudaSuccess) return e;
     uint32_t* counts = reinterpret_cast<uint32_t*>(ws + b.off_counts);
     for (int p = 0; p < b.passes; ++p) {
       uint32_t *ko = key[p & 1], *po = pos[p & 1];
@@ -587,8 +593,8 @@ static cudaError_t bwd(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const 
   }
   char* part = ws + b.off_part;
   if (rows16(g, ldg, D, sizeof(T)) && rows16(dE, lde, D, sizeof(T)))
-    return sums<T, VEC>(b, n, V, D, in.key, in.pos, g, ldg, scale, dE, lde, part, st);
-  return sums<T, 1>(b, n, V, D, in.key, in.pos, g, ldg, scale, dE, lde, part, st);
+    return sums<T, VEC>(b, n, V, D, in.key, in.pos, g, ldg, scale, dE, lde, part, joins, st);
+  return sums<T, 1>(b, n, V, D, in.key, in.pos, g, ldg, scale, dE, lde, part, joins, st);
 }
 
 static int check_sizes(int64_t n, int64_t V, int64_t D, int bits, int dt, int64_t lde) {

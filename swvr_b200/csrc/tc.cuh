@@ -33,6 +33,21 @@ inline cudaError_t resident_clusters(const void* kern, const cudaLaunchConfig_t&
   return e;
 }
 
+// Dynamic shared memory beyond 48 KiB allowed for a kernel, once per kernel and device.
+inline cudaError_t allow_smem(const void* kern, int bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, int> known;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lk(mu);
+  int& most = known[{dev, kern}];
+  if (most >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) most = bytes;
+  return e;
+}
+
 // ------------------------------------------------------------------ forward
 struct FwdParams {
   int N, K, V, D;
