@@ -57,12 +57,13 @@ constexpr int kMaxTeacher = 1024;  // entries per token: the sort's shared memor
 template <typename A>
 __global__ void __launch_bounds__(32 * kWarps)
     teacher_kernel(int64_t N, int64_t V, int Kt, const void* __restrict__ ids, int bits, const void* __restrict__ t,
-                   int t_dt, const A* __restrict__ t_lse, A inv_T, int32_t* sid, A* slogq, A* qsum) {
+                   int t_dt, const A* __restrict__ t_lse, A inv_T, int32_t* sid, A* slogq, A* qsum, uint32_t* done) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   A* tv = reinterpret_cast<A*>(smem_raw) + warp * Kt;
   int32_t* id = reinterpret_cast<int32_t*>(reinterpret_cast<A*>(smem_raw) + kWarps * Kt) + warp * Kt;
   const int64_t n = blockIdx.x * static_cast<int64_t>(kWarps) + warp;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0;
   if (n >= N) return;
   A mx = -INFINITY;
   bool bad = false;
@@ -102,128 +103,143 @@ __global__ void __launch_bounds__(32 * kWarps)
   }
 }
 
-// ------------------------------------------------------------------ loss of each token
-// Sources of (m, l): `splits` partial slots of head_kernel in log2 units (slot (n / 256 * splits + s) * 256
-// + n % 256), or one natural-unit pair per token (splits = 0).
-template <typename A>
-__global__ void __launch_bounds__(32 * kWarps)
-    each_kernel(int64_t N, int Kt, int splits, const A* __restrict__ m, const A* __restrict__ l,
-                const int32_t* __restrict__ sid, const A* __restrict__ slogq, const A* __restrict__ z,
-                const A* __restrict__ qsum, A T2, A* lse, A* lse_lo, A* each) {
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int64_t n = blockIdx.x * static_cast<int64_t>(kWarps) + warp;
-  if (n >= N) return;
-  double L;
-  if (splits == 0) {
-    L = static_cast<double>(m[n]) + log(static_cast<double>(l[n]));
-  } else {
-    const int64_t base = (n / 256) * splits * 256 + n % 256;
-    A mx = -INFINITY;
-    for (int s = lane; s < splits; s += 32) mx = m[base + s * 256ll] > mx ? m[base + s * 256ll] : mx;
-    mx = warp_max(mx);
-    double sum = 0;
-    if (mx != -static_cast<A>(INFINITY))
-      for (int s = lane; s < splits; s += 32) {
-        const A w = exp2f(static_cast<float>(m[base + s * 256ll] - mx));
-        sum += static_cast<double>(l[base + s * 256ll]) * w;
-      }
-    sum = warp_sum(sum);
-    L = (static_cast<double>(mx) + log2(sum)) * 0.6931471805599453;
-  }
-  const A hi = static_cast<A>(L), lo = isfinite(L) ? static_cast<A>(L - static_cast<double>(hi)) : A(0);
-  // (log q - z) + lse: z and lse are near each other, so the difference is taken first
-  A s = 0;
-  for (int k = lane; k < Kt; k += 32) {
-    if (sid[n * Kt + k] == INT_MAX) continue;
-    const A lq = slogq[n * Kt + k], q = exp_a(lq);
-    if (q > 0) s += q * (lq - ((z[n * Kt + k] - hi) - lo));
-    else if (q != q) s = q;
-  }
-  s = warp_sum(s);
-  if (lane == 0) {
-    lse[n] = hi;
-    lse_lo[n] = lo;
-    each[n] = qsum[n] != qsum[n] ? qsum[n] : T2 * s;
-  }
-}
-
+// ------------------------------------------------------------------ loss
 template <typename A>
 __device__ __forceinline__ A weighted(A w, A e) {
   return w == A(0) ? A(0) : w * e;  // a zero weight drops the token, whatever its loss
 }
 
-template <typename A>
-__global__ void none_kernel(int64_t N, const A* __restrict__ each, const A* __restrict__ w, A* out) {
-  const int64_t n = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-  if (n < N) out[n] = w ? weighted(w[n], each[n]) : each[n];
-}
-
 // Sum or mean over the tokens by one block in a fixed order, in double.  stats: loss, denominator.
 template <typename A>
-__global__ void __launch_bounds__(1024) total_kernel(int64_t N, bool mean, const A* __restrict__ each,
-                                                     const A* __restrict__ w, A* out, A* stats) {
-  __shared__ double sh[2][32];
+__device__ __forceinline__ void total_loss(int64_t N, bool mean, const A* each, const A* __restrict__ w, A* out, A* stats) {
+  __shared__ double sh[2][32 * kWarps / 32];
   double s = 0, d = 0;
-  for (int64_t n = threadIdx.x; n < N; n += 1024) {
+#pragma unroll 4
+  for (int64_t n = threadIdx.x; n < N; n += blockDim.x) {
     const A wn = w ? w[n] : A(1);
-    s += static_cast<double>(weighted(wn, each[n]));
+    s += static_cast<double>(weighted(wn, __ldcg(each + n)));
     d += static_cast<double>(wn);
   }
   s = warp_sum(s);
   d = warp_sum(d);
   if (threadIdx.x % 32 == 0) sh[0][threadIdx.x / 32] = s, sh[1][threadIdx.x / 32] = d;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    s = warp_sum(sh[0][threadIdx.x]);
-    d = warp_sum(sh[1][threadIdx.x]);
-    if (threadIdx.x == 0) {
-      if (!mean) d = 1.0;
-      *out = static_cast<A>(s / d);
-      stats[0] = static_cast<A>(s / d);
-      stats[1] = static_cast<A>(d);
+  if (threadIdx.x == 0) {
+    s = d = 0;
+    for (int i = 0; i < kWarps; ++i) s += sh[0][i], d += sh[1][i];
+    if (!mean) d = 1.0;
+    *out = static_cast<A>(s / d);
+    stats[0] = static_cast<A>(s / d);
+    stats[1] = static_cast<A>(d);
+  }
+}
+
+// Sources of (m, l): `splits` partial slots of head_kernel in log2 units (slot (n / 256 * splits + s) * 256
+// + n % 256), or one natural-unit pair per token (splits = 0).  The block that finishes last sums the tokens (all of
+// them, in a fixed order); `done` counts finished blocks and is cleared by teacher_kernel.
+template <typename A>
+__global__ void __launch_bounds__(32 * kWarps)
+    each_kernel(int64_t N, int Kt, int splits, const A* __restrict__ m, const A* __restrict__ l,
+                const int32_t* __restrict__ sid, const A* __restrict__ slogq, const A* __restrict__ z,
+                const A* __restrict__ qsum, A T2, A* lse, A* lse_lo, A* each, int red, const A* __restrict__ w, A* out, A* stats,
+                uint32_t* done) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t n = blockIdx.x * static_cast<int64_t>(kWarps) + warp;
+  if (n < N) {
+    double L;
+    if (splits == 0) {
+      L = static_cast<double>(m[n]) + log(static_cast<double>(l[n]));
+    } else {
+      const int64_t base = (n / 256) * splits * 256 + n % 256;
+      A mx = -INFINITY;
+      for (int s = lane; s < splits; s += 32) mx = m[base + s * 256ll] > mx ? m[base + s * 256ll] : mx;
+      mx = warp_max(mx);
+      double sum = 0;
+      if (mx != -static_cast<A>(INFINITY))
+        for (int s = lane; s < splits; s += 32) {
+          const A w = exp2f(static_cast<float>(m[base + s * 256ll] - mx));
+          sum += static_cast<double>(l[base + s * 256ll]) * w;
+        }
+      sum = warp_sum(sum);
+      L = (static_cast<double>(mx) + log2(sum)) * 0.6931471805599453;
     }
+    const A hi = static_cast<A>(L), lo = isfinite(L) ? static_cast<A>(L - static_cast<double>(hi)) : A(0);
+    // (log q - z) + lse: z and lse are near each other, so the difference is taken first
+    A s = 0;
+    for (int k = lane; k < Kt; k += 32) {
+      if (sid[n * Kt + k] == INT_MAX) continue;
+      const A lq = slogq[n * Kt + k], q = exp_a(lq);
+      if (q > 0) s += q * (lq - ((z[n * Kt + k] - hi) - lo));
+      else if (q != q) s = q;
+    }
+    s = warp_sum(s);
+    if (lane == 0) {
+      const A e = qsum[n] != qsum[n] ? qsum[n] : T2 * s;
+      lse[n] = hi;
+      lse_lo[n] = lo;
+      each[n] = e;
+      if (red == SWVR_REDUCE_NONE) out[n] = w ? weighted(w[n], e) : e;
+    }
+  }
+  if (red == SWVR_REDUCE_NONE) return;
+  __shared__ bool last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(done, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (last) {
+    __threadfence();
+    total_loss(N, red == SWVR_REDUCE_MEAN, each, w, out, stats);
   }
 }
 
 // ------------------------------------------------------------------ backward
-// Per token: gT = g_n T (g_n: upstream, weight and denominator), coef = gT sum q, and the weight's
-// gradient.  amax: the largest |gT| max(1, sum q) as fp32 bits, for the ranges below.
-template <typename A>
-__global__ void token_grad_kernel(int64_t N, int red, A T, const A* __restrict__ gout, const A* __restrict__ w,
-                                  const A* __restrict__ each, const A* __restrict__ qsum, const A* __restrict__ stats,
-                                  A* gT, A* coef, A* grad_w, uint32_t* amax) {
-  const int64_t n = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-  if (n >= N) return;
-  const A up = red == SWVR_REDUCE_NONE ? gout[n] : gout[0];
-  const A den = red == SWVR_REDUCE_MEAN ? stats[1] : A(1);
-  const A wn = w ? w[n] : A(1);
-  const A q = qsum[n];
-  // a row with no teacher left, and one of zero weight, take no part: 0, not 0 x inf
-  const A g = wn == A(0) || q == A(0) ? A(0) : up * wn / den * T;
-  gT[n] = g;
-  coef[n] = g == A(0) ? A(0) : g * q;
-  if (grad_w) grad_w[n] = red == SWVR_REDUCE_MEAN ? up * (each[n] - stats[0]) / den : up * each[n];
-  if (amax) {
-    const float a = fabsf(static_cast<float>(g)) * fmaxf(1.f, static_cast<float>(q));
-    if (a > 0.f && a < INFINITY) atomicMax(amax, __float_as_uint(a));  // positive floats order as integers
-  }
-}
+// One block.  Per token: gT = g_n T (g_n: upstream, weight and denominator), coef = gT sum q, and the weight's
+// gradient.  Then the ranges, from the largest |gT| max(1, sum q), a:
+// f[0] what dS is multiplied by when stored, f[1] its undoing (dh, dW), f[2] the binary exponent of db's fixed point.
+// fp16 dS is scaled by a power of two that puts its largest value near 2^13, so that small gradients (1 / N of a
+// mean) do not fall below fp16's range; bf16 has fp32's.
+constexpr int kGradThreads = 1024;
 
-// factors: [0] what dS is multiplied by when stored, [1] its undoing (dh, dW), [2] fixed-point scale of db,
-// [3] its undoing.  fp16 dS is scaled by a power of two that puts its largest value near 2^13, so that
-// small gradients (1 / N of a mean) do not fall below fp16's range; bf16 has fp32's.
-__global__ void factors_kernel(const uint32_t* amax, float s, bool fp16, float* f) {
-  const float a = __uint_as_float(*amax);
-  int e = 0, x = 0;
-  if (a > 0.f) {
-    const float as = a * fabsf(s);
-    if (fp16 && as > 0.f && as < INFINITY) e = max(-100, min(100, 13 - ilogbf(as)));
-    x = max(-100, min(140, 40 - ilogbf(a)));
+template <typename A>
+__global__ void __launch_bounds__(kGradThreads)
+    token_grad_kernel(int64_t N, int red, A T, const A* __restrict__ gout, const A* __restrict__ w, const A* __restrict__ each,
+                      const A* __restrict__ qsum, const A* __restrict__ stats, A* gT, A* coef, A* grad_w, float s, bool fp16,
+                      float* f) {
+  __shared__ float most[kGradThreads / 32];
+  float a = 0.f;
+#pragma unroll 4
+  for (int64_t n = threadIdx.x; n < N; n += kGradThreads) {
+    const A up = red == SWVR_REDUCE_NONE ? gout[n] : gout[0];
+    const A den = red == SWVR_REDUCE_MEAN ? stats[1] : A(1);
+    const A wn = w ? w[n] : A(1);
+    const A q = qsum[n];
+    // a row with no teacher left, and one of zero weight, take no part: 0, not 0 x inf
+    const A g = wn == A(0) || q == A(0) ? A(0) : up * wn / den * T;
+    gT[n] = g;
+    coef[n] = g == A(0) ? A(0) : g * q;
+    if (grad_w) grad_w[n] = red == SWVR_REDUCE_MEAN ? up * (each[n] - stats[0]) / den : up * each[n];
+    const float b = fabsf(static_cast<float>(g)) * fmaxf(1.f, static_cast<float>(q));
+    if (b < INFINITY) a = fmaxf(a, b);  // neither inf nor NaN
   }
-  f[0] = ldexpf(s, e);
-  f[1] = ldexpf(1.f, -e);
-  f[2] = static_cast<float>(x);
-  f[3] = 0.f;
+  if (!f) return;
+  a = warp_max(a);
+  if (threadIdx.x % 32 == 0) most[threadIdx.x / 32] = a;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    a = warp_max(most[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      int e = 0, x = 0;
+      if (a > 0.f) {
+        const float as = a * fabsf(s);
+        if (fp16 && as > 0.f && as < INFINITY) e = max(-100, min(100, 13 - ilogbf(as)));
+        x = max(-100, min(140, 40 - ilogbf(a)));
+      }
+      f[0] = ldexpf(s, e);
+      f[1] = ldexpf(1.f, -e);
+      f[2] = static_cast<float>(x);
+    }
+  }
 }
 
 // The sum of q over the entries of sorted position j's id, when j is the first of them; -1 otherwise.
@@ -274,11 +290,16 @@ __global__ void db_kernel(int rows, int v0, int TS, const float* __restrict__ pa
   store_d(gb, gb_dt, v0 + i, s);
 }
 
-__global__ void cast_scaled_kernel(const float* __restrict__ src, const float* __restrict__ f, void* dst, int dt, int64_t n) {
+// dh from its slices of accumulators, added in slice order.
+__global__ void cast_scaled_kernel(const float* __restrict__ src, int slices, int64_t slice, const float* __restrict__ f,
+                                   void* dst, int dt, int64_t n) {
   const float k = f[1];
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < n;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x)
-    store_f(dst, dt, i, src[i] * k);
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    float v = src[i];
+    for (int s = 1; s < slices; ++s) v += src[s * slice + i];
+    store_f(dst, dt, i, v * k);
+  }
 }
 
 // ------------------------------------------------------------------ exact path (fp32 / fp64)
@@ -286,12 +307,6 @@ template <typename A>
 __global__ void scaled_bias_kernel(int64_t V, const void* bias, int dt, A inv_T, A* out) {
   const int64_t v = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
   if (v < V) out[v] = static_cast<A>(load_d(bias, dt, v)) * inv_T;
-}
-
-template <typename A>
-__global__ void exact_init_kernel(int64_t N, A* m, A* l) {
-  const int64_t n = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-  if (n < N) m[n] = -INFINITY, l[n] = A(0);
 }
 
 // One block per token: picks the teacher's scores of the chunk, then updates (m, l) with the row.
@@ -309,41 +324,36 @@ __global__ void __launch_bounds__(256)
   A mx = -INFINITY;
   for (int64_t c = threadIdx.x; c < C; c += blockDim.x) mx = row[c] > mx ? row[c] : mx;
   mx = simt::block_reduce<A>(mx, true, sh);
-  const A m_old = m[n], m_new = m_old > mx ? m_old : mx;
+  const A m_old = v0 == 0 ? -static_cast<A>(INFINITY) : m[n], m_new = m_old > mx ? m_old : mx;
   const A shift = isinf(m_new) ? A(0) : m_new;
   A sum = 0;
   for (int64_t c = threadIdx.x; c < C; c += blockDim.x) sum += exp_a(row[c] - shift);
   sum = simt::block_reduce<A>(sum, false, sh);
   if (threadIdx.x == 0) {
-    l[n] = l[n] * exp_a(m_old - shift) + sum;
+    l[n] = (v0 == 0 ? A(0) : l[n] * exp_a(m_old - shift)) + sum;
     m[n] = m_new;
   }
 }
 
+// dS of a chunk in place of S: a block per token writes the dense row, then the teacher's entries over it.
 template <typename A>
-__global__ void exact_dense_kernel(A* S, const A* __restrict__ lse, const A* __restrict__ lse_lo,
-                                   const A* __restrict__ coef, int64_t N, int64_t C) {
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < N * C;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const A c = coef[i / C];
-    S[i] = c == A(0) ? A(0) : exp_a((S[i] - lse[i / C]) - lse_lo[i / C]) * c;
-  }
-}
-
-template <typename A>
-__global__ void exact_entries_kernel(int64_t N, int Kt, int64_t C, int v0, const int32_t* __restrict__ sid,
-                                     const A* __restrict__ slogq, const A* __restrict__ z, const A* __restrict__ lse, const A* __restrict__ lse_lo,
-                                     const A* __restrict__ gT, const A* __restrict__ coef, A* G) {
-  const int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-  if (i >= N * Kt) return;
-  const int32_t v = sid[i];
-  if (v < v0 || v >= v0 + C) return;
-  const int64_t n = i / Kt;
-  const A g = gT[n];
+__global__ void __launch_bounds__(256)
+    exact_grad_kernel(int64_t C, int Kt, int v0, const int32_t* __restrict__ sid, const A* __restrict__ slogq,
+                      const A* __restrict__ z, const A* __restrict__ lse, const A* __restrict__ lse_lo,
+                      const A* __restrict__ gT, const A* __restrict__ coef, A* S) {
+  const int64_t n = blockIdx.x;
+  const A c = coef[n], g = gT[n], hi = lse[n], lo = lse_lo[n];
+  A* row = S + n * C;
+  for (int64_t i = threadIdx.x; i < C; i += blockDim.x) row[i] = c == A(0) ? A(0) : exp_a((row[i] - hi) - lo) * c;
   if (g == A(0)) return;
-  const A q = merged_q(sid + n * Kt, slogq + n * Kt, static_cast<int>(i - n * Kt), Kt);
-  if (q < A(0)) return;
-  G[n * C + v - v0] = exp_a((z[i] - lse[n]) - lse_lo[n]) * coef[n] - g * q;
+  __syncthreads();
+  for (int j = threadIdx.x; j < Kt; j += blockDim.x) {
+    const int32_t v = sid[n * Kt + j];
+    if (v < v0 || v >= v0 + C) continue;
+    const A q = merged_q(sid + n * Kt, slogq + n * Kt, j, Kt);
+    if (q < A(0)) continue;
+    row[v - v0] = exp_a((z[n * Kt + j] - hi) - lo) * c - g * q;
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -390,7 +400,7 @@ static int check(const swvr_distill* p) {
 
 struct LsePlan {
   int MT, BT, splits, per, units, pairs;
-  size_t off_l, bytes;
+  size_t off_l, off_done, bytes;
 };
 
 // Splits of the vocabulary per 256-token tile: the rounds over the pairs times the tiles of a unit, least.
@@ -410,7 +420,8 @@ static LsePlan plan_lse(const swvr_distill& p) {
   f.units = f.MT * f.splits;
   const size_t rows = static_cast<size_t>(f.units) * 256;
   f.off_l = align_up(rows * 4, 256);
-  f.bytes = f.off_l + align_up(rows * 4, 256) + 256;
+  f.off_done = f.off_l + align_up(rows * 4, 256);
+  f.bytes = f.off_done + 256;
   return f;
 }
 
@@ -418,7 +429,7 @@ static size_t acc_size(const swvr_distill& p) { return p.compute_dtype == SWVR_F
 
 struct ExactPlan {
   int64_t C;
-  size_t off_bias, off_m, off_l, off_dh, off_part, bytes;
+  size_t off_bias, off_m, off_l, off_done, off_dh, off_part, bytes;
 };
 
 static ExactPlan plan_exact(const swvr_distill& p, bool bwd, bool need_h) {
@@ -432,6 +443,8 @@ static ExactPlan plan_exact(const swvr_distill& p, bool bwd, bool need_h) {
   off += align_up(es * p.n_tokens, 256);
   e.off_l = off;
   off += align_up(es * p.n_tokens, 256);
+  e.off_done = off;
+  off += 256;
   e.off_dh = off;
   if (bwd && need_h) off += align_up(es * p.n_tokens * p.hidden, 256);
   // slices of a product split along its sum, where its 128 x 128 tiles would leave SMs idle (simt::gemm_split)
@@ -449,7 +462,8 @@ struct GradPlan {
   int NT, C, pairs, max_units;
   int64_t Npad;
   bool need_h, need_W, need_b;
-  size_t off_gT, off_coef, off_amax, off_f, off_fix, off_db, off_ds, off_dh, bytes;
+  int slices;     // of dh's accumulators
+  size_t off_gT, off_coef, off_f, off_fix, off_dh, off_db, off_ds, clear, bytes;
 };
 
 static GradPlan plan_grad(const swvr_distill& p, const swvr_distill_grads& g) {
@@ -476,25 +490,31 @@ static GradPlan plan_grad(const swvr_distill& p, const swvr_distill_grads& g) {
   off += align_up(p.n_tokens * acc_size(p), 256);
   b.off_coef = off;
   off += align_up(p.n_tokens * acc_size(p), 256);
-  b.off_amax = off;
-  b.off_f = off + 64;
+  b.off_f = off;
   off += 256;
+  b.slices = 1;
   if (is_tc(p.compute_dtype)) {
+    // few tokens: dh has few tiles and each sums over the whole chunk, so the sum is dealt over slices while that
+    // fills pairs that would be idle (517 tokens, K = 512, V = 10007: the GEMMs 57 -> 22 us)
+    const int64_t tiles = b.NT * ceil_div(p.hidden, 256), kblocks = b.C / 128;
+    if (b.need_h && tiles > 0)
+      b.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({b.pairs / tiles, kblocks / 4, 16})));
     b.off_fix = off;
     if (b.need_b) off += align_up(p.vocab * 8, 256);
+    b.off_dh = off;
+    if (b.need_h) off += align_up(static_cast<size_t>(b.slices > 1 ? b.slices * b.Npad : p.n_tokens) * p.hidden * 4, 256);
+    b.clear = off - b.off_fix;
     b.off_db = off;
     if (b.need_b) off += align_up(static_cast<size_t>(b.max_units) * 256 * 4, 256);
     b.off_ds = off;
     off += align_up(static_cast<size_t>(b.C) * b.Npad * 2, 256);
-    b.off_dh = off;
-    if (b.need_h) off += align_up(static_cast<size_t>(p.n_tokens) * p.hidden * 4, 256);
   }
   b.bytes = off + 256;
   return b;
 }
 
 template <typename A>
-static cudaError_t teacher_rows(const swvr_distill& p, cudaStream_t st) {
+static cudaError_t teacher_rows(const swvr_distill& p, uint32_t* done, cudaStream_t st) {
   const size_t smem = static_cast<size_t>(kWarps) * p.teacher * (sizeof(A) + 4);
   auto kern = teacher_kernel<A>;
   const cudaError_t e = tc::allow_smem(reinterpret_cast<const void*>(kern), kWarps * kMaxTeacher * (static_cast<int>(sizeof(A)) + 4));
@@ -502,24 +522,27 @@ static cudaError_t teacher_rows(const swvr_distill& p, cudaStream_t st) {
   kern<<<static_cast<unsigned>(ceil_div(p.n_tokens, kWarps)), 32 * kWarps, smem, st>>>(
       p.n_tokens, p.vocab, static_cast<int>(p.teacher), p.teacher_ids, p.id_bits, p.teacher_logits, p.teacher_dtype,
       static_cast<const A*>(p.teacher_lse), static_cast<A>(1.0 / p.temperature), p.sid, static_cast<A*>(p.slogq),
-      static_cast<A*>(p.qsum));
+      static_cast<A*>(p.qsum), done);
   return cudaGetLastError();
 }
 
 template <typename A>
-static cudaError_t losses(const swvr_distill& p, int splits, const A* m, const A* l, void* out, cudaStream_t st) {
+__global__ void empty_kernel(bool mean, A* out, A* stats) {  // no tokens: a sum of 0, a mean of 0 / 0
+  *out = stats[0] = mean ? static_cast<A>(NAN) : A(0);
+  stats[1] = mean ? A(0) : A(1);
+}
+
+template <typename A>
+static cudaError_t losses(const swvr_distill& p, int splits, const A* m, const A* l, void* out, uint32_t* done, cudaStream_t st) {
   const int64_t N = p.n_tokens;
   if (N > 0)
     each_kernel<A><<<static_cast<unsigned>(ceil_div(N, kWarps)), 32 * kWarps, 0, st>>>(
         N, static_cast<int>(p.teacher), splits, m, l, p.sid, static_cast<const A*>(p.slogq), static_cast<const A*>(p.z),
         static_cast<const A*>(p.qsum), static_cast<A>(p.temperature * p.temperature), static_cast<A*>(p.lse),
-        static_cast<A*>(p.lse_lo), static_cast<A*>(p.each));
-  if (p.reduction != SWVR_REDUCE_NONE)
-    total_kernel<A><<<1, 1024, 0, st>>>(N, p.reduction == SWVR_REDUCE_MEAN, static_cast<const A*>(p.each),
-                                        static_cast<const A*>(p.weight), static_cast<A*>(out), static_cast<A*>(p.stats));
-  else if (N > 0)
-    none_kernel<A><<<static_cast<unsigned>(ceil_div(N, 256)), 256, 0, st>>>(
-        N, static_cast<const A*>(p.each), static_cast<const A*>(p.weight), static_cast<A*>(out));
+        static_cast<A*>(p.lse_lo), static_cast<A*>(p.each), p.reduction, static_cast<const A*>(p.weight),
+        static_cast<A*>(out), static_cast<A*>(p.stats), done);
+  else if (p.reduction != SWVR_REDUCE_NONE)
+    empty_kernel<A><<<1, 1, 0, st>>>(p.reduction == SWVR_REDUCE_MEAN, static_cast<A*>(out), static_cast<A*>(p.stats));
   return cudaGetLastError();
 }
 
@@ -537,13 +560,14 @@ static int tc_fwd_distill(const swvr_distill& p, void* out, void* ws, size_t wsb
   if (wsb < f.bytes) return fail(SWVR_ERR_WORKSPACE, "workspace %zu < required %zu", wsb, f.bytes);
   float* m2 = static_cast<float*>(ws);
   float* l = reinterpret_cast<float*>(static_cast<char*>(ws) + f.off_l);
+  uint32_t* done = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + f.off_done);
   if (p.n_tokens > 0) {
     tc::HeadMaps maps;
     SWVR_TRY(make_map(&maps.a, p.h, p.compute_dtype, p.hidden, p.n_tokens, p.ldh * 2, 64, 128));
     SWVR_TRY(make_map(&maps.b, p.W, p.compute_dtype, p.hidden, p.vocab, p.ldw * 2, 64, 128));
     {
       ProfScope ps(kProfDistill, st);
-      SWVR_CUDA(teacher_rows<float>(p, st));
+      SWVR_CUDA(teacher_rows<float>(p, done, st));
     }
     tc::HeadParams h{};
     head_scores(p, &h);
@@ -564,8 +588,8 @@ static int tc_fwd_distill(const swvr_distill& p, void* out, void* ws, size_t wsb
                   ? tc::launch_head_any<true>(tc::kHeadLse, 256, maps, h, f.pairs, false, st)
                   : tc::launch_head_any<false>(tc::kHeadLse, 256, maps, h, f.pairs, false, st));
   }
-  ProfScope ps(kProfDistill, st, 2);
-  SWVR_CUDA(losses<float>(p, f.splits, m2, l, out, st));
+  ProfScope ps(kProfDistill, st);
+  SWVR_CUDA(losses<float>(p, f.splits, m2, l, out, done, st));
   return SWVR_OK;
 }
 
@@ -593,11 +617,11 @@ static int exact_fwd(const swvr_distill& p, void* out, void* ws, size_t wsb, cud
   A *S = reinterpret_cast<A*>(w), *bias = p.bias ? reinterpret_cast<A*>(w + x.off_bias) : nullptr;
   A *m = reinterpret_cast<A*>(w + x.off_m), *l = reinterpret_cast<A*>(w + x.off_l);
   const int64_t N = p.n_tokens;
+  uint32_t* done = reinterpret_cast<uint32_t*>(w + x.off_done);
   ProfScope ps(kProfDistill, st);
   if (N > 0) {
-    SWVR_CUDA(teacher_rows<A>(p, st));
+    SWVR_CUDA(teacher_rows<A>(p, done, st));
     if (bias) SWVR_CUDA(exact_bias<A>(p, bias, st));
-    exact_init_kernel<A><<<static_cast<unsigned>(ceil_div(N, 256)), 256, 0, st>>>(N, m, l);
     for (int64_t v0 = 0; v0 < p.vocab; v0 += x.C) {
       const int64_t c = std::min(x.C, p.vocab - v0);
       SWVR_CUDA(exact_scores<A>(p, x, v0, c, S, bias, st));
@@ -606,17 +630,17 @@ static int exact_fwd(const swvr_distill& p, void* out, void* ws, size_t wsb, cud
       SWVR_CUDA(cudaGetLastError());
     }
   }
-  SWVR_CUDA(losses<A>(p, 0, m, l, out, st));
+  SWVR_CUDA(losses<A>(p, 0, m, l, out, done, st));
   return SWVR_OK;
 }
 
 template <typename A>
-static cudaError_t token_grads(const swvr_distill& p, const swvr_distill_grads& g, A* gT, A* coef, uint32_t* amax,
-                               cudaStream_t st) {
-  token_grad_kernel<A><<<static_cast<unsigned>(ceil_div(p.n_tokens, 256)), 256, 0, st>>>(
+static cudaError_t token_grads(const swvr_distill& p, const swvr_distill_grads& g, A* gT, A* coef, float* f, cudaStream_t st) {
+  token_grad_kernel<A><<<1, kGradThreads, 0, st>>>(
       p.n_tokens, p.reduction, static_cast<A>(p.temperature), static_cast<const A*>(g.grad_out),
       static_cast<const A*>(p.weight), static_cast<const A*>(p.each), static_cast<const A*>(p.qsum),
-      static_cast<const A*>(p.stats), gT, coef, static_cast<A*>(g.grad_weight), amax);
+      static_cast<const A*>(p.stats), gT, coef, static_cast<A*>(g.grad_weight), static_cast<float>(p.logit_scale),
+      p.compute_dtype == SWVR_F16, f);
   return cudaGetLastError();
 }
 
@@ -624,22 +648,17 @@ static int tc_bwd_distill(const swvr_distill& p, const swvr_distill_grads& g, co
   const int64_t N = p.n_tokens, K = p.hidden, V = p.vocab;
   const bool bf16 = p.compute_dtype == SWVR_BF16;
   float *gT = reinterpret_cast<float*>(w + b.off_gT), *coef = reinterpret_cast<float*>(w + b.off_coef);
-  uint32_t* amax = reinterpret_cast<uint32_t*>(w + b.off_amax);
   float* f = reinterpret_cast<float*>(w + b.off_f);
   unsigned long long* fix = b.need_b ? reinterpret_cast<unsigned long long*>(w + b.off_fix) : nullptr;
   float* part_db = b.need_b ? reinterpret_cast<float*>(w + b.off_db) : nullptr;
   void* ds = w + b.off_ds;
   float* dh = b.need_h ? reinterpret_cast<float*>(w + b.off_dh) : nullptr;
-  SWVR_CUDA(cudaMemsetAsync(amax, 0, 4, st));
   {
-    ProfScope ps(kProfDistill, st, 2);
-    SWVR_CUDA(token_grads<float>(p, g, gT, coef, amax, st));
-    factors_kernel<<<1, 1, 0, st>>>(amax, static_cast<float>(p.logit_scale), !bf16, f);
-    SWVR_CUDA(cudaGetLastError());
+    ProfScope ps(kProfDistill, st);
+    SWVR_CUDA(token_grads<float>(p, g, gT, coef, f, st));
   }
   if (!(b.need_h || b.need_W || b.need_b)) return SWVR_OK;
-  if (fix) SWVR_CUDA(cudaMemsetAsync(fix, 0, V * 8, st));
-  if (dh) SWVR_CUDA(cudaMemsetAsync(dh, 0, static_cast<size_t>(N) * K * 4, st));
+  if (b.clear) SWVR_CUDA(cudaMemsetAsync(w + b.off_fix, 0, b.clear, st));  // db's fixed point and dh, side by side
   tc::HeadMaps maps;
   SWVR_TRY(make_map(&maps.a, p.W, p.compute_dtype, K, V, p.ldw * 2, 64, 128));
   SWVR_TRY(make_map(&maps.b, p.h, p.compute_dtype, K, N, p.ldh * 2, 64, 128));
@@ -653,7 +672,7 @@ static int tc_bwd_distill(const swvr_distill& p, const swvr_distill_grads& g, co
     else
       SWVR_TRY(make_map(&gm.gw, g.grad_W, p.compute_dtype, K, V, g.ld_grad_W * 2, 64, 128));
   }
-  if (dh) SWVR_TRY(make_map(&gm.dh, dh, SWVR_F32, K, N, K * 4, 32, 128));
+  if (dh) SWVR_TRY(make_map(&gm.dh, dh, SWVR_F32, K, b.slices > 1 ? b.slices * b.Npad : N, K * 4, 32, 128));
   for (int64_t v0 = 0; v0 < V; v0 += b.C) {
     const int64_t v1 = std::min<int64_t>(v0 + b.C, V);
     const int rows = static_cast<int>(v1 - v0), VTc = static_cast<int>(ceil_div(rows, 256));
@@ -707,7 +726,10 @@ static int tc_bwd_distill(const swvr_distill& p, const swvr_distill_grads& g, co
       gp.dh_mt = b.NT;
       gp.dh_nt = nt;
       gp.dh_kb = static_cast<int>(ceil_div(rows, 64));
-      gp.dh_tiles = dh ? gp.dh_mt * nt : 0;
+      gp.dh_splits = std::max(1, std::min<int>(b.slices, static_cast<int>(ceil_div(gp.dh_kb, 2))));
+      gp.dh_splits = static_cast<int>(ceil_div(ceil_div(gp.dh_kb, 2), ceil_div(ceil_div(gp.dh_kb, 2), gp.dh_splits)));  // none empty
+      gp.dh_slice_rows = static_cast<int>(b.Npad);
+      gp.dh_tiles = dh ? gp.dh_mt * nt * gp.dh_splits : 0;
       gp.v_begin = static_cast<int>(v0);
       gp.gw_f32 = g.grad_W_dtype == SWVR_F32 ? 1 : 0;
       gp.gw_scale = bf16 ? nullptr : f + 1;
@@ -719,7 +741,7 @@ static int tc_bwd_distill(const swvr_distill& p, const swvr_distill_grads& g, co
     ProfScope ps(kProfCast, st);
     const int64_t n = N * K;
     cast_scaled_kernel<<<static_cast<unsigned>(std::min<int64_t>(ceil_div(n, 256), 8 * kNumSMsB200)), 256, 0, st>>>(
-        dh, f, g.grad_h, g.grad_h_dtype, n);
+        dh, b.slices, b.Npad * K, f, g.grad_h, g.grad_h_dtype, n);
     SWVR_CUDA(cudaGetLastError());
   }
   return SWVR_OK;
@@ -737,32 +759,29 @@ static int exact_bwd(const swvr_distill& p, const swvr_distill_grads& g, const G
   A* dh = reinterpret_cast<A*>(w + x.off_dh);
   float* part = sizeof(A) == 4 ? reinterpret_cast<float*>(w + x.off_part) : nullptr;
   ProfScope ps(kProfDistill, st);
-  SWVR_CUDA(token_grads<A>(p, g, gT, coef, nullptr, st));
+  SWVR_CUDA(token_grads<A>(p, g, gT, coef, static_cast<float*>(nullptr), st));
   if (!(b.need_h || b.need_W || b.need_b)) return SWVR_OK;
   if (bias) SWVR_CUDA(exact_bias<A>(p, bias, st));
-  if (b.need_h) SWVR_CUDA(cudaMemsetAsync(dh, 0, sizeof(A) * N * K, st));
+  const bool one = x.C >= V;  // one chunk: dh goes straight to its place
   for (int64_t v0 = 0; v0 < V; v0 += x.C) {
     const int64_t c = std::min(x.C, V - v0);
     SWVR_CUDA(exact_scores<A>(p, x, v0, c, S, bias, st));
-    exact_dense_kernel<A><<<simt::grid_for(N * c), 256, 0, st>>>(S, static_cast<const A*>(p.lse),
-                                                                static_cast<const A*>(p.lse_lo), coef, N, c);
-    if (p.teacher > 0)
-      exact_entries_kernel<A><<<static_cast<unsigned>(ceil_div(N * p.teacher, 256)), 256, 0, st>>>(
-          N, static_cast<int>(p.teacher), c, static_cast<int>(v0), p.sid, static_cast<const A*>(p.slogq),
-          static_cast<const A*>(p.z), static_cast<const A*>(p.lse), static_cast<const A*>(p.lse_lo), gT, coef, S);
+    exact_grad_kernel<A><<<static_cast<unsigned>(N), 256, 0, st>>>(
+        c, static_cast<int>(p.teacher), static_cast<int>(v0), p.sid, static_cast<const A*>(p.slogq),
+        static_cast<const A*>(p.z), static_cast<const A*>(p.lse), static_cast<const A*>(p.lse_lo), gT, coef, S);
     if (b.need_b)
       simt::colsum_kernel<A><<<static_cast<unsigned>(ceil_div(c, 32)), 256, 0, st>>>(S, N, c, g.grad_bias,
                                                                                     g.grad_bias_dtype, v0);
     SWVR_CUDA(cudaGetLastError());
     if (b.need_h)
-      SWVR_CUDA(simt::gemm_split<A>(st, N, K, c, s, S, c, 1, static_cast<const A*>(p.W) + v0 * p.ldw, p.ldw, 1, A(1), dh,
-                                    adt, K, 1, part, kLeastK));
+      SWVR_CUDA(simt::gemm_split<A>(st, N, K, c, s, S, c, 1, static_cast<const A*>(p.W) + v0 * p.ldw, p.ldw, 1,
+                                    A(v0 ? 1 : 0), one ? g.grad_h : dh, one ? g.grad_h_dtype : adt, K, 1, part, kLeastK));
     if (b.need_W)
       SWVR_CUDA(simt::gemm_split<A>(st, c, K, N, s, S, 1, c, static_cast<const A*>(p.h), p.ldh, 1, A(0),
                                     static_cast<char*>(g.grad_W) + static_cast<size_t>(v0 * g.ld_grad_W) * dtype_size(g.grad_W_dtype),
                                     g.grad_W_dtype, g.ld_grad_W, 1, part, kLeastK));
   }
-  if (b.need_h) {
+  if (b.need_h && !one) {
     simt::cast_kernel<A><<<simt::grid_for(N * K), 256, 0, st>>>(dh, g.grad_h, g.grad_h_dtype, N * K);
     SWVR_CUDA(cudaGetLastError());
   }

@@ -156,6 +156,8 @@ struct GemmParams {
   int dh_mt, dh_nt, dh_kb;   // dh: row tiles (tokens / 256), column tiles, k-blocks (chunk rows / 64)
   int v_begin;               // first vocabulary row of the chunk
   int gw_f32;                // dW output is fp32 (else the 16-bit compute dtype)
+  int dh_splits;             // dh: 0 or 1, or the number of slices of accumulators its k-blocks are dealt over,
+  int dh_slice_rows;         // each this many rows after the one before
   const float* gw_scale;     // dW is multiplied by this device value before it is stored; null: stored as it is
 };
 

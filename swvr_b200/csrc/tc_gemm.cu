@@ -49,6 +49,7 @@ struct GemmCfg {
 struct TileInfo {
   bool dw;
   int mb, nb, kblocks;
+  int kb0, slice;  // dh split along its sum: first k-block and slice of accumulators
 };
 
 // Pair tiles: dW tiles first (mb over 256-row blocks of the chunk), then dh tiles.
@@ -59,12 +60,23 @@ __device__ __forceinline__ TileInfo decode_tile(const GemmParams& p, int t) {
     ti.mb = t / p.dw_nt;
     ti.nb = t % p.dw_nt;
     ti.kblocks = (p.dw_kb + 1) / 2;  // 128-wide K-blocks
+    ti.kb0 = ti.slice = 0;
   } else {
     t -= p.dw_tiles;
     ti.dw = false;
+    const int kblocks = (p.dh_kb + 1) / 2;
+    if (p.dh_splits > 1) {
+      const int per = (kblocks + p.dh_splits - 1) / p.dh_splits;
+      ti.slice = t / (p.dh_mt * p.dh_nt);
+      t %= p.dh_mt * p.dh_nt;
+      ti.kb0 = ti.slice * per;
+      ti.kblocks = min(per, kblocks - ti.kb0);
+    } else {
+      ti.kb0 = ti.slice = 0;
+      ti.kblocks = kblocks;
+    }
     ti.mb = t / p.dh_nt;
     ti.nb = t % p.dh_nt;
-    ti.kblocks = (p.dh_kb + 1) / 2;
   }
   return ti;
 }
@@ -148,7 +160,7 @@ __global__ void __launch_bounds__(256, 1)
           const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
 #pragma unroll
           for (int hk = 0; hk < 2; ++hk) {
-            const int k0 = (2 * kb + hk) * 64;  // past K the boxes read zero fill
+            const int k0 = (2 * (ti.kb0 + kb) + hk) * 64;  // past K the boxes read zero fill
             uint8_t* a = smem + Cfg::SMEM_A + stage * Cfg::A_BYTES + hk * Cfg::HALF;
             uint8_t* b = smem + Cfg::SMEM_B + stage * Cfg::B_BYTES + hk * Cfg::HALF;
             if (ti.dw) {
@@ -266,7 +278,7 @@ __global__ void __launch_bounds__(256, 1)
           if (ti.dw)
             tma_store_2d(&tm_gw, stg, ti.nb * 256 + s * (f16out ? 64 : 32), p.v_begin + row);
           else
-            tma_reduce_add_2d(&tm_dh, stg, ti.nb * 256 + s * 32, row);
+            tma_reduce_add_2d(&tm_dh, stg, ti.nb * 256 + s * 32, ti.slice * p.dh_slice_rows + row);
           tma_store_commit();
         }
       }
