@@ -244,16 +244,22 @@ def softmax_distill(h, W, teacher_ids, teacher_logits, bias=None, *, temperature
     nat.dtype_code(cdt)
     adt = acc_dtype(cdt)
     N = math.prod(lead)
-    row = lambda t: None if t is None else t.to(adt).reshape(N).contiguous()  # noqa: E731
-    args = (h.reshape(N, h.shape[-1]), W, bias, teacher_ids.reshape(N, Kt).contiguous(),
-            teacher_logits.detach().reshape(N, Kt).contiguous(), None if teacher_lse is None else row(teacher_lse.detach()),
-            row(weight), temperature, float(logit_scale), chunk, cdt, _REDUCTIONS[reduction])
+    def row(t):
+        t = t if t.dtype == adt else t.to(adt)
+        return (t if t.dim() == 1 else t.reshape(N)).contiguous()
+
+    def flat(t, last):
+        return t if t.dim() == 2 else t.reshape(N, last)
+
+    args = (flat(h, h.shape[-1]), W, bias, flat(teacher_ids, Kt).contiguous(), flat(teacher_logits, Kt).contiguous(),
+            None if teacher_lse is None else row(teacher_lse), None if weight is None else row(weight), temperature,
+            float(logit_scale), chunk, cdt, _REDUCTIONS[reduction])
     if _eager(*args[:7]):
         out = _Distill.apply(*args)
     else:
         with torch.autocast(h.device.type, enabled=False):
             out = _distill_op(*args)[0]
-    return out.view(lead) if reduction == "none" else out
+    return out.view(lead) if reduction == "none" and len(lead) != 1 else out
 
 
 class SoftmaxDistill(nn.Module):

@@ -138,6 +138,6 @@ def embedding_lookup(tokens, E, *, scale=1.0, padding_idx=None):
         if not -V <= padding < V:
             raise ValueError(f"padding_idx {padding_idx} is outside a table of {V} rows")
         padding += V if padding < 0 else 0
-    flat = tokens.reshape(-1)
+    flat = tokens if tokens.dim() == 1 else tokens.reshape(-1)
     out = (_Embed.apply if _eager(flat, E) else _embed_op)(flat, E, float(scale), padding)
-    return out.view(*tokens.shape, E.shape[1])
+    return out if tokens.dim() == 1 else out.view(*tokens.shape, E.shape[1])

@@ -111,7 +111,7 @@ def _number(name, x, low, high, lead, open_low=False):
         if x.shape != lead:
             raise ValueError(f"{name} must be a number or have shape {tuple(lead)}, got {tuple(x.shape)}")
         nat.dtype_code(x.dtype)
-        return high if math.isfinite(high) else 1.0, x.detach().reshape(-1)
+        return high if math.isfinite(high) else 1.0, x.reshape(-1)
     x = float(x)
     if not (math.isfinite(x) and (low < x if open_low else low <= x) and x <= high):
         raise ValueError(f"{name} must be in {'(' if open_low else '['}{low:g}, {high:g}], got {x}")
@@ -139,7 +139,13 @@ def _settings(lead, u, temperature, top_k, top_p, min_p):
     return (T, k, p, m, Ts, ks, ps, ms)
 
 
+def _rows(x, lead):
+    return x if x.dim() == 2 else x.reshape(math.prod(lead), x.shape[-1])
+
+
 def _shaped(out, lead, want_logprobs):
+    if len(lead) == 1:
+        return out if want_logprobs else out[0]
     return (out[0].view(lead), out[1].view(lead)) if want_logprobs else out[0].view(lead)
 
 
@@ -165,9 +171,13 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=None, top_p=None, min_p=N
         raise ValueError(f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
     lead = logits.shape[:-1]
     args = _settings(lead, u, temperature, top_k, top_p, min_p)
-    x, uu = logits.detach().reshape(math.prod(lead), logits.shape[-1]), u.detach().reshape(-1)
-    run = _sample_logits if _eager(x, uu) else _sample_logits_op
-    return _shaped(run(x, uu, *args, bool(return_logprobs)), lead, return_logprobs)
+    x, uu = _rows(logits, lead), u if u.dim() == 1 else u.reshape(-1)
+    if _eager(x, uu):
+        with torch.no_grad():
+            out = _sample_logits(x, uu, *args, bool(return_logprobs))
+    else:
+        out = _sample_logits_op(x.detach(), uu.detach(), *args, bool(return_logprobs))
+    return _shaped(out, lead, return_logprobs)
 
 
 def softmax_sample(h, W, u, bias=None, *, temperature=1.0, top_k=None, top_p=None, min_p=None, logit_scale=1.0,
@@ -190,9 +200,12 @@ def softmax_sample(h, W, u, bias=None, *, temperature=1.0, top_k=None, top_p=Non
         raise ValueError(f"softmax_sample computes in bf16, fp16 or fp32, got {cdt}")
     lead = h.shape[:-1]
     args = _settings(lead, u, temperature, top_k, top_p, min_p)
-    h2, W2 = h.detach().reshape(math.prod(lead), h.shape[-1]), W.detach()
-    b, uu = None if bias is None else bias.detach(), u.detach().reshape(-1)
-    run = _sample_head if _eager(h2, W2, b, uu) else _sample_op
-    with torch.autocast(h.device.type, enabled=False):
-        out = run(h2, W2, b, uu, float(logit_scale), cdt, *args, bool(return_logprobs))
+    h2, uu = _rows(h, lead), u if u.dim() == 1 else u.reshape(-1)
+    if _eager(h2, W, bias, uu):
+        with torch.no_grad():
+            out = _sample_head(h2, W, bias, uu, float(logit_scale), cdt, *args, bool(return_logprobs))
+    else:
+        d = lambda t: None if t is None else t.detach()  # noqa: E731
+        with torch.autocast(h.device.type, enabled=False):
+            out = _sample_op(d(h2), d(W), d(bias), d(uu), float(logit_scale), cdt, *args, bool(return_logprobs))
     return _shaped(out, lead, return_logprobs)
