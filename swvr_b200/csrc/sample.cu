@@ -8,7 +8,7 @@
 //
 // What makes the result that of 64 bits rather than of some summation order: weights are 64-bit fixed
 // point, 2^44 for the largest (2^(62 - log2 V) where V is past 2^18), so sums are exact in any order, by any number of
-// threads.  Weights below 2^-44 of the largest are 0 (30.5 T below the maximum).
+// threads.
 //
 // A row is a cluster of 1 .. 8 CTAs, each with a contiguous share of the scores.  They are read from global memory in
 // every pass: after the first they are in L2, and shared memory full of scores would leave one CTA an SM (measured
@@ -34,6 +34,7 @@
 // hundred, they are taken.
 #include <cooperative_groups.h>
 
+#include <cfloat>
 #include <cmath>
 
 #include "common.cuh"
@@ -49,7 +50,7 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
-constexpr float kReach = 30.5f;  // e^-30.5 < 2^-44
+constexpr float kReach = 31.5f;  // e^-31.2 2^44 = 1/2: weights further below the largest score than 31.5 T round to 0
 constexpr int kRoughOne = 40;    // fp32 sums are kept in units of 2^-40 of the largest weight
 
 struct Setting {  // one value for all rows, or one per row
@@ -131,7 +132,7 @@ struct Shared {
   uint32_t count_all[kBins];
   uint32_t count[kBins], mass_lo[kBins], mass_hi[kBins];
   u64 list[kList], list_w[kList];
-  double root[64];        // 2^(j / 64)
+  double root[64];        // 2^(j / 64 + lg_one)
   u64 part[kWarps];       // per-warp results of a block reduction or scan
   u64 slot[14];           // values other CTAs of the cluster read, each written once
   u64 found[3];           // boundary bin, and count or weight before it
@@ -145,12 +146,12 @@ struct Shared {
   __device__ __forceinline__ u64 mass(int b) const { return (static_cast<u64>(mass_hi[b]) << 32) | mass_lo[b]; }
 };
 
-// A float as a double by its bits (a conversion runs at an eighth of the rate); subnormals as 0.
+// A float as a double by its bits (a conversion runs at an eighth of the rate).  0 and subnormals become some 2^-127: off by
+// less than 2^-126, for both scores of a difference.
 __device__ __forceinline__ double widen(float x) {
   const uint32_t b = __float_as_uint(x);
-  const double v = __hiloint2double(static_cast<int>((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)),
-                                    static_cast<int>(b << 29));
-  return (b & 0x7f800000u) == 0 ? 0.0 : v;
+  return __hiloint2double(static_cast<int>((((b >> 3) & 0x0fffffffu) + 0x38000000u) | (b & 0x80000000u)),
+                          static_cast<int>(b << 29));
 }
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -171,9 +172,10 @@ struct Row {
   double top_d, c64;  // top, and 64 log2(e) / T
   double invT;
   int lg_one;
-  float reach;    // scores further below have no weight
+  float reach;    // kReach T
+  float floor;    // scores below have no weight; above -inf
   float per_bin;  // bins per unit of score
-  const double* root;
+  const double* root;  // 2^(j / 64 + lg_one), j < 64
   bool rough_ok;  // fp32 weights are within their bound
   int rough_bits; // 18 or 19
   float c32, c32_lo;  // log2(e) / T in two parts
@@ -195,7 +197,7 @@ struct Row {
       for (int e = 0; e < o; ++e) v[e] += v[e + o];
     return static_cast<double>(v[0]);
   }
-  __device__ __forceinline__ bool live(float x) const { return x == top || top - x < reach; }
+  __device__ __forceinline__ bool live(float x) const { return x >= floor; }  // not NaN either
   // exp((x - top) / T) 2^lg_one, rounded.  With y = 64 log2(e) (x - top) / T = n + f, |f| <= 1/2:
   // 2^(y / 64) = 2^(n / 64) e^(f ln 2 / 64), the first factor from a table of 64, the second a polynomial of
   // degree 4 (remainder 2^-44.6), in doubles.  Adding 1.5 2^52 rounds y to n, adding 2^52 rounds the result.
@@ -211,13 +213,12 @@ struct Row {
     q = fma(f, q, a1);
     q = fma(f, q, 1.0);
     double v = root[n & 63] * q;
-    v = __hiloint2double(__double2hiint(v) + (((n >> 6) + lg_one) << 20), __double2loint(v));
+    v = __hiloint2double(__double2hiint(v) + ((n & ~63) << 14), __double2loint(v));  // n >> 6 added to the exponent
     const u64 w = static_cast<u64>(__double_as_longlong(v + 4503599627370496.0)) & 0xfffffffffffffull;
-    return x == top ? 1ull << lg_one : (top - x < reach ? w : 0ull);
+    return live(x) ? w : 0ull;
   }
   // a score d below the largest, or a little further; above -inf
   __device__ __forceinline__ float below(float d) const { return score_of(max(order_of(top - d), order_of(-INFINITY) + 3) - 2); }
-  __device__ __forceinline__ float floor_x() const { return below(reach); }  // scores below it have no weight
   // rises as x falls: subtraction, product and conversion are all monotone
   __device__ __forceinline__ int bin(float x) const {
     return x == top ? 0 : min(kBins - 1, static_cast<int>((top - x) * per_bin));
@@ -636,7 +637,7 @@ __device__ __noinline__ u64 boundary(const Scores<T>& sc, const Row& row, int bi
     return pl >= lo && pl <= hi;
   };
   while (true) {
-    const uint32_t m = gather(sc, row, row.floor_x(), member, s, cl);
+    const uint32_t m = gather(sc, row, row.floor, member, s, cl);
     if (m <= kList) {
       if (cl.block_rank() == 0) {
         u64 low = ~0ull;
@@ -731,7 +732,10 @@ __device__ __noinline__ u64 thresholds(const Scores<T>& sc, const Row& row, bool
 template <typename T>
 __device__ __forceinline__ u64 exact_total(const Scores<T>& sc, const Row& row, Shared& s) {
   u64 w = 0;
-  sc.each([&](float x, int i) { w += row.weight(x); });
+  sc.template packs<1>(threadIdx.x * Scores<T>::VEC, sc.n, kThreads * Scores<T>::VEC, [&](const typename Scores<T>::Pack& p, int) {
+#pragma unroll
+    for (int e = 0; e < Scores<T>::VEC; ++e) w += row.weight(to_float(p.e[e]));
+  });
   return block_sum(w, s);
 }
 __device__ __forceinline__ u64 rough_units(double w) { return static_cast<u64>(ldexp(w, kRoughOne)); }
@@ -755,9 +759,9 @@ __device__ __forceinline__ u64 span_weight(const Scores<T>& sc, const Row& row, 
     sc.template packs<1>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int i) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float x = to_score(p.e[e]);
+        const float x = to_float(p.e[e]);
         const u64 we = row.weight(x);
-        w += kept.keeps(x, sc.first + i + e) ? we : 0ull;
+        w += !cut || kept.keeps(x, sc.first + i + e) ? we : 0ull;
       }
     });
     return warp_sum(w);
@@ -878,11 +882,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   sc.aligned = p.aligned;
   sc.first = static_cast<uint32_t>(first);
   sc.n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(p.share), p.V - first)));
-  if (tid < 64) s.root[tid] = exp2(tid / 64.0);
+  if (tid < 64) s.root[tid] = exp2(tid / 64.0 + p.lg_one);
   // settings, while the scores are on their way
   double temp = setting(p.T, row_id);
   const bool greedy = !(temp > 0.0);
-  if (greedy) temp = 1.0;
+  temp = greedy ? 1.0 : fmax(temp, 1e-300);
   const double top_p = setting(p.p, row_id), min_p = setting(p.m, row_id), u = load_d(p.u, p.u_dt, row_id);
   const int64_t k = p.k_ptr ? (p.k_bits == 64 ? static_cast<const int64_t*>(p.k_ptr)[row_id]
                                               : static_cast<int64_t>(static_cast<const int32_t*>(p.k_ptr)[row_id]))
@@ -912,6 +916,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   row.top_d = widen(row.top);
   row.lg_one = p.lg_one;
   row.reach = kReach * static_cast<float>(temp);
+  row.floor = fmaxf(row.top - row.reach, -FLT_MAX);
   row.per_bin = static_cast<float>(kBins) / row.reach;
   row.root = s.root;
   row.c32 = static_cast<float>(1.4426950408889634 * row.invT);
@@ -965,7 +970,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
       // a nucleus is looked for among the 128 largest threads' scores, then among more
       const u64 most = min(kThreads * C / 2, 384u);
       for (u64 wanted = by_k ? static_cast<u64>(k) : min(128ull, most);; wanted = most) {
-        float reach_x = row.floor_x();  // a score that every token which may be kept reaches
+        float reach_x = row.floor;  // a score that every token which may be kept reaches
         if (by_k || by_p) {
           find_bin<true>(wanted, s);
           const int b = static_cast<int>(s.found[0]);
@@ -976,7 +981,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         if (by_m && !(by_k && by_p)) reach_x = fmaxf(reach_x, Cut(cut).x);  // (top-p after top-k weighs the first k)
         const uint32_t m = gather(sc, row, reach_x, [](float, int) { return true; }, s, cl);
         if (m > kList) break;
-        const bool all = by_k || !by_p || reach_x == row.floor_x() || reach_x == Cut(cut).x;
+        const bool all = by_k || !by_p || reach_x == row.floor || reach_x == Cut(cut).x;
         Found f = kFound;
         for (int at = 3;; ++at) {  // slots 3, 4 in the first round, 6, 7 in the second
           if (me == 0)
@@ -1020,9 +1025,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
 template <typename T>
 static cudaError_t launch_t(Params p, cudaStream_t st) {
   static_assert(kMaxCluster == 8, "cluster sizes below");
-  // two CTAs an SM and about two rounds of them, so that a row that needs its fixed-point sums does not hold up the rest
+  const bool filters = p.k_ptr || p.k > 0 || p.p.ptr || p.p.value < 1.0 || p.m.ptr || p.m.value > 0.0;
+  // Two CTAs fit an SM.  With filters one round of them (64 rows of 128256 fp32, top-k: 18 us with 256 CTAs, 32 with 512);
+  // without, two, so that a row that needs its fixed-point sums does not hold up the rest (256 rows of 128256 bf16: 66 us
+  // with 512, 77 with 256).
+  const int64_t most = (filters ? 2 : 4) * kNumSMsB200;
   int C = 1;
-  while (C < 8 && 2 * C * p.N <= 4 * kNumSMsB200 && p.V > 2048 * C) C *= 2;
+  while (C < 8 && 2 * C * p.N <= most && p.V > 2048 * C) C *= 2;
   p.share = static_cast<int>(round_up(ceil_div(std::max<int64_t>(p.V, 1), C), 32));
   p.aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.ld * sizeof(T)) % 16 == 0;
   int lg = 0;
@@ -1041,7 +1050,6 @@ static cudaError_t launch_t(Params p, cudaStream_t st) {
   cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = st;
   static_assert(sizeof(Shared) <= 48 * 1024, "more needs cudaFuncSetAttribute");
-  const bool filters = p.k_ptr || p.k > 0 || p.p.ptr || p.p.value < 1.0 || p.m.ptr || p.m.value > 0.0;
   return cudaLaunchKernelEx(&cfg, filters ? sample_kernel<T, true> : sample_kernel<T, false>, p);
 }
 
