@@ -695,7 +695,7 @@ __device__ __noinline__ u64 boundary(const Scores<T>& sc, const Row& row, int bi
 
 // The lowest kept place of top-k and top-p, whatever they leave.
 template <typename T>
-__device__ __noinline__ u64 thresholds(const Scores<T>& sc, const Row& row, bool by_k, u64 k, bool by_p, double top_p,
+__device__ __forceinline__ u64 thresholds(const Scores<T>& sc, const Row& row, bool by_k, u64 k, bool by_p, double top_p,
                                        Shared& s, cg::cluster_group& cl) {
   u64 cut = 0;
   if (by_k) {
@@ -729,8 +729,9 @@ __device__ __noinline__ u64 thresholds(const Scores<T>& sc, const Row& row, bool
 }
 
 // The weight of this CTA's scores, in units of 2^-lg_one of the largest: in fixed point, or from fp32 weights.
+// (By value: a reference to the caller's structs would keep them in local memory.)
 template <typename T>
-__device__ __forceinline__ u64 exact_total(const Scores<T>& sc, const Row& row, Shared& s) {
+__device__ __noinline__ u64 exact_total(const Scores<T> sc, const Row row, Shared& s) {
   u64 w = 0;
   sc.template packs<1>(threadIdx.x * Scores<T>::VEC, sc.n, kThreads * Scores<T>::VEC, [&](const typename Scores<T>::Pack& p, int) {
 #pragma unroll
@@ -864,6 +865,29 @@ __device__ __forceinline__ bool sweep(const Scores<T>& sc, const Row& row, u64 c
   if (kExact) return true;
   cl.sync();
   return *cl.map_shared_rank(&s.found[2], 0) != 0;
+}
+
+struct Choice {
+  uint32_t token;
+  float x;
+  bool mine;  // this thread found it
+};
+
+// Thresholds of any width, and the sweeps: out of the way of the kernel that finds few tokens.
+template <typename T>
+__device__ __noinline__ Choice choose_among_many(const Scores<T> sc, const Row row, bool by_k, u64 k, bool by_p, double top_p, u64 cut,
+                                                 double u, Shared& s) {
+  cg::cluster_group cl = cg::this_cluster();
+  if (by_k || by_p) {
+    const u64 c = thresholds(sc, row, by_k, k, by_p, top_p, s, cl);
+    cut = c > cut ? c : cut;
+  }
+  int64_t token = 0;
+  float x = 0.f;
+  bool mine = false;
+  if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 11, &token, &x, &mine, s, cl))
+    sweep<true>(sc, row, cut, u, 5, &token, &x, &mine, s, cl);
+  return {static_cast<uint32_t>(token), x, mine};
 }
 
 // kFilters: some row may have top-k, top-p or min-p; without, the kernel needs fewer registers and more of it fits an SM.
@@ -1002,12 +1026,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     }
     // -------------------------------------------------------------- many
     if (!done) {
-      if (by_k || by_p) {
-        const u64 c = thresholds(sc, row, by_k, static_cast<u64>(k), by_p, top_p, s, cl);
-        cut = c > cut ? c : cut;
-      }
-      if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 11, &token, &x_token, &mine, s, cl))
+      if constexpr (kFilters) {
+        const Choice c = choose_among_many(sc, row, by_k, static_cast<u64>(k), by_p, top_p, cut, u, s);
+        token = c.token;
+        x_token = c.x;
+        mine = c.mine;
+      } else if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 11, &token, &x_token, &mine, s, cl)) {
         sweep<true>(sc, row, cut, u, 5, &token, &x_token, &mine, s, cl);
+      }
     }
   }
   if (mine) p.token[row_id] = token;
