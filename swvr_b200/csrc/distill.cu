@@ -233,7 +233,9 @@ __global__ void __launch_bounds__(kGradThreads)
       if (a > 0.f) {
         const float as = a * fabsf(s);
         if (fp16 && as > 0.f && as < INFINITY) e = max(-100, min(100, 13 - ilogbf(as)));
-        x = max(-100, min(140, 40 - ilogbf(a)));
+        // a token adds at most 2^41 to a row of db, all of them less than 2^62
+        const int lg = 64 - __clzll(N);
+        x = max(-100, min(140, min(40, 60 - lg) - ilogbf(a)));
       }
       f[0] = ldexpf(s, e);
       f[1] = ldexpf(1.f, -e);

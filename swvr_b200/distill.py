@@ -208,7 +208,8 @@ def softmax_distill(h, W, teacher_ids, teacher_logits, bias=None, *, temperature
 
     An entry with a negative id or a logit of -inf is left out, and a token with none left has loss 0
     and no gradient.  An id at or past V makes its token's loss NaN and is reported by
-    ``_native.check_device_error()``.  ``chunk_size`` is that of ``softmax_readout``.
+    ``_native.check_device_error()``.  ``chunk_size`` is that of ``softmax_readout``; under autocast h and W are
+    cast whole.
     """
     if W.dim() != 2:
         raise ValueError(f"W must be 2-D, got {tuple(W.shape)}")
@@ -250,6 +251,11 @@ def softmax_distill(h, W, teacher_ids, teacher_logits, bias=None, *, temperature
 
     def flat(t, last):
         return t if t.dim() == 2 else t.reshape(N, last)
+
+    if teacher_logits.requires_grad:
+        teacher_logits = teacher_logits.detach()
+    if teacher_lse is not None and teacher_lse.requires_grad:
+        teacher_lse = teacher_lse.detach()
 
     args = (flat(h, h.shape[-1]), W, bias, flat(teacher_ids, Kt).contiguous(), flat(teacher_logits, Kt).contiguous(),
             None if teacher_lse is None else row(teacher_lse), None if weight is None else row(weight), temperature,

@@ -391,3 +391,26 @@ def test_wide_teacher_rows():
     check(h, W, b, ids, t)
     check(h.detach().double().requires_grad_(True), W.detach().double().requires_grad_(True),
           b.detach().double().requires_grad_(True), ids, t)
+
+
+def test_the_teacher_is_a_constant():
+    h, W, b, ids, t = make(9, 16, 60, 4, torch.float32)
+    t.requires_grad_(True)
+    L = torch.logsumexp(t, 1)
+    loss = swvr.softmax_distill(h.detach(), W.detach(), ids, t, teacher_lse=L)
+    assert not loss.requires_grad
+    loss = swvr.softmax_distill(h, W, ids, t, teacher_lse=L)
+    assert torch.autograd.grad(loss, t, allow_unused=True)[0] is None
+
+
+def test_rows_of_zero_weight_may_hold_anything():
+    """NaN scores in a dropped token reach nothing but its own loss."""
+    h, W, b, ids, t = make(40, 64, 600, 5, torch.bfloat16)
+    w = torch.ones(40, device="cuda")
+    w[7] = 0
+    clean = run(h, W, b, ids, t, weight=w)
+    with torch.no_grad():
+        h[7, 0] = math.inf
+    loss, (dh, dW, db, _) = run(h, W, b, ids, t, weight=w)
+    assert torch.equal(loss, clean[0]) and torch.equal(db, clean[1][2])
+    assert bool((dh[7] == 0).all()) and torch.equal(dh[:7], clean[1][0][:7])

@@ -331,3 +331,33 @@ def test_compiled_whole():
 
     got = torch.compile(f, fullgraph=True, backend="aot_eager")(x, h, W, b, u)
     assert all(torch.equal(a, c) for a, c in zip(got, f(x, h, W, b, u)))
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(k=30, p=0.9), dict(p=0.9999, T=1.3), dict(m=0.01)])
+def test_very_long_rows(kw):
+    """Past 2^20 scores: fixed-point weights of fewer bits, no fp32 sums."""
+    check(logits(2, 1200007, scale=3.0), uniform(2), **kw)
+
+
+def test_head_without_a_vocabulary():
+    h, W, b = head(3, 64, 5, torch.bfloat16)
+    assert swvr.softmax_sample(h, W[:0], uniform(3)).tolist() == [-1, -1, -1]
+    assert swvr.softmax_sample(h[:0], W, uniform(0)).shape == (0,)
+
+
+def test_scores_that_need_no_gradient_take_none():
+    x = logits(4, 100).requires_grad_(True)
+    tok, lp = swvr.sample_logits(x, uniform(4), return_logprobs=True)
+    assert not tok.requires_grad and not lp.requires_grad
+    h, W, b = head(4, 64, 100, torch.bfloat16)
+    assert not swvr.softmax_sample(h.requires_grad_(True), W.requires_grad_(True), uniform(4), b).requires_grad
+
+
+def test_rows_of_the_lowest_value_beside_minus_infinity():
+    """A mask of the type's lowest value is a score like any other; one of -inf is not."""
+    for dt in (torch.float32, torch.bfloat16):
+        x = torch.full((6, 400), torch.finfo(dt).min, dtype=dt, device="cuda")
+        x[:, ::2] = -math.inf
+        for kw in (dict(), dict(T=1e30), dict(k=9), dict(p=0.5), dict(m=0.9)):
+            got = check(x, uniform(6), **kw)
+            assert bool((got % 2 == 1).all())
