@@ -258,7 +258,8 @@ int swvr_embed_bwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tok
  *   out = w_n each_n (NONE, [N]), their sum (SUM), or sum / (sum(w) or N) (MEAN)
  * over the `teacher` entries (id_k, t_k) of each token; an id may occur more than once.
  * An entry with a negative id or a logit of -inf is left out; a token with none left has loss
- * 0 and no gradient.  A zero weight drops its token whatever its loss.  An id >= vocab (with a
+ * 0 and no gradient.  A zero weight drops its token whatever its loss (h must be finite in
+ * every row: 0 times inf in grad_W).  An id >= vocab (with a
  * logit above -inf) makes its token's loss and gradient NaN and sets SWVR_TOKEN_CODE.
  *
  * teacher_ids [N, teacher] (id_bits 32 or 64) and teacher_logits [N, teacher] (any dtype) are

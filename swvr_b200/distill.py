@@ -206,7 +206,8 @@ def softmax_distill(h, W, teacher_ids, teacher_logits, bias=None, *, temperature
     the inputs are fp64), differentiable in ``h``, ``W``, ``bias`` and ``weight``; the teacher is a
     constant.
 
-    An entry with a negative id or a logit of -inf is left out, and a token with none left has loss 0
+    A dropped token may have an infinite loss, but its row of ``h`` is read and must be finite (0 times inf in
+    dW).  An entry with a negative id or a logit of -inf is left out, and a token with none left has loss 0
     and no gradient.  An id at or past V makes its token's loss NaN and is reported by
     ``_native.check_device_error()``.  ``chunk_size`` is that of ``softmax_readout``; under autocast h and W are
     cast whole.
