@@ -188,7 +188,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def stream_ptr(device: torch.device) -> int:
-    if _raw_stream is not None:  # the handle alone: no Stream object
+    if _raw_stream is not None and device.index is not None:  # the handle alone: no Stream object
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
