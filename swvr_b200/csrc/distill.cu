@@ -314,11 +314,11 @@ __global__ void scaled_bias_kernel(int64_t V, const void* bias, int dt, A inv_T,
 // One block per token: picks the teacher's scores of the chunk, then updates (m, l) with the row.
 template <typename A>
 __global__ void __launch_bounds__(256)
-    exact_update_kernel(const A* __restrict__ S, int64_t C, int v0, int Kt, const int32_t* __restrict__ sid, A* z, A* m,
+    exact_update_kernel(const A* __restrict__ S, int64_t C, int64_t pitch, int v0, int Kt, const int32_t* __restrict__ sid, A* z, A* m,
                         A* l) {
   __shared__ A sh[32];
   const int64_t n = blockIdx.x;
-  const A* row = S + n * C;
+  const A* row = S + n * pitch;
   for (int k = threadIdx.x; k < Kt; k += blockDim.x) {
     const int32_t v = sid[n * Kt + k];
     if (v >= v0 && v < v0 + C) z[n * Kt + k] = row[v - v0];
@@ -337,16 +337,18 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dS of a chunk in place of S: a block per token writes the dense row, then the teacher's entries over it.
+// dS of a chunk in place of S: a block per token writes the dense row and zeros up to the pitch, then the teacher's
+// entries over it.
 template <typename A>
 __global__ void __launch_bounds__(256)
-    exact_grad_kernel(int64_t C, int Kt, int v0, const int32_t* __restrict__ sid, const A* __restrict__ slogq,
+    exact_grad_kernel(int64_t C, int64_t pitch, int Kt, int v0, const int32_t* __restrict__ sid, const A* __restrict__ slogq,
                       const A* __restrict__ z, const A* __restrict__ lse, const A* __restrict__ lse_lo,
                       const A* __restrict__ gT, const A* __restrict__ coef, A* S) {
   const int64_t n = blockIdx.x;
   const A c = coef[n], g = gT[n], hi = lse[n], lo = lse_lo[n];
-  A* row = S + n * C;
-  for (int64_t i = threadIdx.x; i < C; i += blockDim.x) row[i] = c == A(0) ? A(0) : exp_a((row[i] - hi) - lo) * c;
+  A* row = S + n * pitch;
+  for (int64_t i = threadIdx.x; i < pitch; i += blockDim.x)
+    row[i] = i >= C || c == A(0) ? A(0) : exp_a((row[i] - hi) - lo) * c;
   if (g == A(0)) return;
   __syncthreads();
   for (int j = threadIdx.x; j < Kt; j += blockDim.x) {
@@ -438,7 +440,7 @@ static ExactPlan plan_exact(const swvr_distill& p, bool bwd, bool need_h) {
   ExactPlan e{};
   const size_t es = acc_size(p);
   e.C = std::min(p.chunk, std::max<int64_t>(p.vocab, 1));
-  size_t off = align_up(es * p.n_tokens * e.C, 256);
+  size_t off = align_up(es * p.n_tokens * round_up(e.C, 4), 256);  // rows of a multiple of 4: 16-byte staging
   e.off_bias = off;
   off += align_up(es * p.vocab, 256);
   e.off_m = off;
@@ -601,7 +603,7 @@ static cudaError_t exact_scores(const swvr_distill& p, const ExactPlan& x, int64
   const int adt = sizeof(A) == 8 ? SWVR_F64 : SWVR_F32;
   return simt::gemm_bias<A>(st, p.n_tokens, c, p.hidden, static_cast<A>(p.logit_scale / p.temperature),
                             static_cast<const A*>(p.h), p.ldh, 1, static_cast<const A*>(p.W) + v0 * p.ldw, 1, p.ldw, S,
-                            adt, bias, adt, v0);
+                            adt, bias, adt, v0, round_up(c, 4));
 }
 
 template <typename A>
@@ -627,8 +629,8 @@ static int exact_fwd(const swvr_distill& p, void* out, void* ws, size_t wsb, cud
     for (int64_t v0 = 0; v0 < p.vocab; v0 += x.C) {
       const int64_t c = std::min(x.C, p.vocab - v0);
       SWVR_CUDA(exact_scores<A>(p, x, v0, c, S, bias, st));
-      exact_update_kernel<A><<<static_cast<unsigned>(N), 256, 0, st>>>(S, c, static_cast<int>(v0), static_cast<int>(p.teacher),
-                                                                       p.sid, static_cast<A*>(p.z), m, l);
+      exact_update_kernel<A><<<static_cast<unsigned>(N), 256, 0, st>>>(
+          S, c, round_up(c, 4), static_cast<int>(v0), static_cast<int>(p.teacher), p.sid, static_cast<A*>(p.z), m, l);
       SWVR_CUDA(cudaGetLastError());
     }
   }
@@ -766,22 +768,22 @@ static int exact_bwd(const swvr_distill& p, const swvr_distill_grads& g, const G
   if (bias) SWVR_CUDA(exact_bias<A>(p, bias, st));
   const bool one = x.C >= V;  // one chunk: dh goes straight to its place
   for (int64_t v0 = 0; v0 < V; v0 += x.C) {
-    const int64_t c = std::min(x.C, V - v0);
+    const int64_t c = std::min(x.C, V - v0), ld = round_up(c, 4);
     SWVR_CUDA(exact_scores<A>(p, x, v0, c, S, bias, st));
     exact_grad_kernel<A><<<static_cast<unsigned>(N), 256, 0, st>>>(
-        c, static_cast<int>(p.teacher), static_cast<int>(v0), p.sid, static_cast<const A*>(p.slogq),
+        c, ld, static_cast<int>(p.teacher), static_cast<int>(v0), p.sid, static_cast<const A*>(p.slogq),
         static_cast<const A*>(p.z), static_cast<const A*>(p.lse), static_cast<const A*>(p.lse_lo), gT, coef, S);
     if (b.need_b)
-      simt::colsum_kernel<A><<<static_cast<unsigned>(ceil_div(c, 32)), 256, 0, st>>>(S, N, c, g.grad_bias,
+      simt::colsum_kernel<A><<<static_cast<unsigned>(ceil_div(c, 32)), 256, 0, st>>>(S, N, c, ld, g.grad_bias,
                                                                                     g.grad_bias_dtype, v0);
     SWVR_CUDA(cudaGetLastError());
     if (b.need_h)
-      SWVR_CUDA(simt::gemm_split<A>(st, N, K, c, s, S, c, 1, static_cast<const A*>(p.W) + v0 * p.ldw, p.ldw, 1,
-                                    A(v0 ? 1 : 0), one ? g.grad_h : dh, one ? g.grad_h_dtype : adt, K, 1, part, kLeastK));
+      SWVR_CUDA(simt::gemm_split<A>(st, N, K, c, s, S, ld, 1, static_cast<const A*>(p.W) + v0 * p.ldw, p.ldw, 1,
+                                    A(v0 ? 1 : 0), one ? g.grad_h : dh, one ? g.grad_h_dtype : adt, K, 1, part, kLeastK, true));
     if (b.need_W)
-      SWVR_CUDA(simt::gemm_split<A>(st, c, K, N, s, S, 1, c, static_cast<const A*>(p.h), p.ldh, 1, A(0),
+      SWVR_CUDA(simt::gemm_split<A>(st, c, K, N, s, S, 1, ld, static_cast<const A*>(p.h), p.ldh, 1, A(0),
                                     static_cast<char*>(g.grad_W) + static_cast<size_t>(v0 * g.ld_grad_W) * dtype_size(g.grad_W_dtype),
-                                    g.grad_W_dtype, g.ld_grad_W, 1, part, kLeastK));
+                                    g.grad_W_dtype, g.ld_grad_W, 1, part, kLeastK, true));
   }
   if (b.need_h && !one) {
     simt::cast_kernel<A><<<simt::grid_for(N * K), 256, 0, st>>>(dh, g.grad_h, g.grad_h_dtype, N * K);

@@ -409,9 +409,10 @@ __global__ void __launch_bounds__(256) sum_kernel(int64_t n, int len, int chunks
 }
 
 // Adds the pieces of each token that spans chunks, in a fixed order: a block (32 packs wide) for each chunk in which
-// such a token begins; 16 groups of threads take every 16th of the pieces that follow, and the groups' sums are added in
-// group order.  16384 tokens, one of 82 pieces: 38 us by one row of threads per chunk.
-constexpr int kJoinGroups = 16;
+// such a token begins; 4 groups of threads take every 4th of the pieces that follow, four at a time, and the groups'
+// sums are added in group order.  16384 tokens, some 300 spanning chunks and one of 82 pieces: 38 us by one row of
+// threads per chunk, 16 us with 16 groups (most tokens have a piece or two).
+constexpr int kJoinGroups = 4;
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(32 * kJoinGroups)
@@ -435,10 +436,22 @@ __global__ void __launch_bounds__(32 * kJoinGroups)
       if (threadIdx.y == 0)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[k] = part[(chunk * 2 + 1) * D + c + k];
-#pragma unroll 2
-      for (int64_t j = chunk + 1 + threadIdx.y; j < chunks && key[j * len] == cur; j += kJoinGroups)
+      constexpr int U = 4;  // pieces in flight: their keys, then their sums
+      bool more = true;
+      for (int64_t j0 = chunk + 1 + threadIdx.y; more; j0 += U * kJoinGroups) {
+        bool is[U];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += part[j * 2 * D + c + k];
+        for (int q = 0; q < U; ++q) {
+          const int64_t j = j0 + q * kJoinGroups;
+          is[q] = j < chunks && key[j * len] == cur;
+        }
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+          if (is[q])
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[k] += part[(j0 + q * kJoinGroups) * 2 * D + c + k];
+        more = is[U - 1];
+      }
     }
 #pragma unroll
     for (int k = 0; k < VEC; ++k) sums[threadIdx.y][threadIdx.x][k] = acc[k];
@@ -543,7 +556,7 @@ static cudaError_t sums(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int64_t work = ceil_div(packs, 32) * b.chunks;
-  join_kernel<T, VEC><<<static_cast<unsigned>(std::min<int64_t>(work, 4 * kNumSMsB200)), dim3(32, kJoinGroups), 0, st>>>(
+  join_kernel<T, VEC><<<static_cast<unsigned>(std::min<int64_t>(work, 16 * kNumSMsB200)), dim3(32, kJoinGroups), 0, st>>>(
       b.len, b.chunks, packs, key, static_cast<A>(scale), static_cast<T*>(dE), lde, static_cast<const A*>(part), joins);
   return cudaGetLastError();
 }

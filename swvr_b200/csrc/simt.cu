@@ -409,15 +409,18 @@ inline int64_t splitk_floats(int64_t M, int64_t N) {
 
 template <typename T>
 cudaError_t gemm(cudaStream_t st, int64_t M, int64_t N, int64_t K, T alpha, const T* A, int64_t sam, int64_t sak,
-                 const T* B, int64_t sbk, int64_t sbn, T beta, void* C, int cdt, int64_t scm, int64_t scn) {
+                 const T* B, int64_t sbk, int64_t sbn, T beta, void* C, int cdt, int64_t scm, int64_t scn,
+                 bool a_padded = false) {
   if (M == 0 || N == 0) return cudaSuccess;
   dim3 grid(static_cast<unsigned>(ceil_div(N, BN)), static_cast<unsigned>(ceil_div(M, BM)));
   // A: unit stride along K (sak == 1) or along M (sam == 1); B: along N (sbn == 1) or along K
   const bool vec_a = sak == 1 ? vec4_ok(A, sam, sak, K) : vec4_ok(A, sak, sam, M);
   const bool vec_b = sbn == 1 ? vec4_ok(B, sbk, sbn, N) : vec4_ok(B, sbn, sbk, K);
   if constexpr (sizeof(T) == 4) {
-    // the tensor-core kernel where its 16-byte staging applies, else the CUDA-core one
-    if (tf32x3_ok(A, sam, sak, M, B, sbk, sbn, N, K))
+    // the tensor-core kernel where its 16-byte staging applies, else the CUDA-core one.  a_padded: A's rows are
+    // followed by zeros up to a multiple of 4, so its extents need not be one (B's along N does; beyond K its rows are not read)
+    if (a_padded ? tf32x3_ok(A, sam, sak, round_up(M, 4), B, sbk, sbn, N, sbn == 1 ? round_up(K, 4) : K)
+                 : tf32x3_ok(A, sam, sak, M, B, sbk, sbn, N, K))
       return launch_tf32x3_any(st, grid, M, N, K, alpha, A, sam, sak, B, sbk, sbn, beta, C, cdt, scm, scn, K, 0);
   }
   gemm_kernel<T><<<grid, 256, 0, st>>>(M, N, K, alpha, A, sam, sak, B, sbk, sbn, beta, C, cdt, scm, scn, vec_a, vec_b);
@@ -434,9 +437,11 @@ cudaError_t gemm(cudaStream_t st, int64_t M, int64_t N, int64_t K, T alpha, cons
 template <typename T>
 cudaError_t gemm_split(cudaStream_t st, int64_t M, int64_t N, int64_t K, T alpha, const T* A, int64_t sam,
                         int64_t sak, const T* B, int64_t sbk, int64_t sbn, T beta, void* C, int cdt, int64_t scm,
-                        int64_t scn, float* part, int64_t k_least = 256) {
+                        int64_t scn, float* part, int64_t k_least = 256, bool a_padded = false) {
   if constexpr (sizeof(T) == 4) {
-    if (M > 0 && N > 0 && part && tf32x3_ok(A, sam, sak, M, B, sbk, sbn, N, K)) {
+    if (M > 0 && N > 0 && part &&
+        (a_padded ? tf32x3_ok(A, sam, sak, round_up(M, 4), B, sbk, sbn, N, sbn == 1 ? round_up(K, 4) : K)
+                  : tf32x3_ok(A, sam, sak, M, B, sbk, sbn, N, K))) {
       const int64_t tiles = ceil_div(M, tf32x3::TM) * ceil_div(N, tf32x3::TN);
       int64_t splits = std::min<int64_t>({int64_t(16), ceil_div(4 * kNumSMsB200, tiles), K / k_least,
                                           splitk_floats(M, N) / (M * N)});
@@ -454,7 +459,7 @@ cudaError_t gemm_split(cudaStream_t st, int64_t M, int64_t N, int64_t K, T alpha
       }
     }
   }
-  return gemm<T>(st, M, N, K, alpha, A, sam, sak, B, sbk, sbn, beta, C, cdt, scm, scn);
+  return gemm<T>(st, M, N, K, alpha, A, sam, sak, B, sbk, sbn, beta, C, cdt, scm, scn, a_padded);
 }
 
 template <typename T>
@@ -489,11 +494,11 @@ __device__ __forceinline__ double log_t<double>(double x) { return log(x); }
 
 // S[n, :] += bias[v0:v0+C] (chunked.py:77-78)
 template <typename T>
-__global__ void add_bias_kernel(T* S, int64_t N, int64_t C, const void* bias, int bdt, int64_t v0) {
+__global__ void add_bias_kernel(T* S, int64_t N, int64_t C, int64_t pitch, const void* bias, int bdt, int64_t v0) {
   const int64_t total = N * C;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x)
-    S[i] += static_cast<T>(load_d(bias, bdt, v0 + i % C));
+    S[i / C * pitch + i % C] += static_cast<T>(load_d(bias, bdt, v0 + i % C));
 }
 
 inline unsigned grid_for(int64_t n, int threads = 256) {
@@ -508,17 +513,18 @@ inline unsigned grid_for(int64_t n, int threads = 256) {
 template <typename T>
 static cudaError_t gemm_bias(cudaStream_t st, int64_t M, int64_t N, int64_t K, T alpha, const T* A, int64_t sam,
                              int64_t sak, const T* B, int64_t sbk, int64_t sbn, T* S, int adt, const void* bias,
-                             int bdt, int64_t v0) {
+                             int bdt, int64_t v0, int64_t pitch = 0) {
+  if (pitch == 0) pitch = N;
   if constexpr (sizeof(T) == 4) {
     if (bias && M > 0 && N > 0 && tf32x3_ok(A, sam, sak, M, B, sbk, sbn, N, K)) {
       dim3 grid(static_cast<unsigned>(ceil_div(N, BN)), static_cast<unsigned>(ceil_div(M, BM)));
-      return launch_tf32x3_any(st, grid, M, N, K, alpha, A, sam, sak, B, sbk, sbn, 0.f, S, adt, N, 1, K, 0,
+      return launch_tf32x3_any(st, grid, M, N, K, alpha, A, sam, sak, B, sbk, sbn, 0.f, S, adt, pitch, 1, K, 0,
                                static_cast<const char*>(bias) + v0 * static_cast<int64_t>(dtype_size(bdt)), bdt);
     }
   }
-  cudaError_t e = gemm<T>(st, M, N, K, alpha, A, sam, sak, B, sbk, sbn, T(0), S, adt, N, 1);
+  cudaError_t e = gemm<T>(st, M, N, K, alpha, A, sam, sak, B, sbk, sbn, T(0), S, adt, pitch, 1);
   if (e != cudaSuccess || !bias) return e;
-  add_bias_kernel<T><<<grid_for(M * N), 256, 0, st>>>(S, M, N, bias, bdt, v0);
+  add_bias_kernel<T><<<grid_for(M * N), 256, 0, st>>>(S, M, N, pitch, bias, bdt, v0);
   return cudaGetLastError();
 }
 
@@ -604,14 +610,14 @@ __global__ void bwd_gs_kernel(const T* P, T* G, const T* delta, int64_t N, int64
 // (a warp reads 32 consecutive columns of one row), and the 8 row sums of a column are
 // added in r order.
 template <typename T>
-__global__ void colsum_kernel(const T* G, int64_t N, int64_t C, void* gb, int gdt, int64_t v0) {
+__global__ void colsum_kernel(const T* G, int64_t N, int64_t C, int64_t pitch, void* gb, int gdt, int64_t v0) {
   __shared__ T part[8][33];
   const int cl = threadIdx.x % 32, r = threadIdx.x / 32;
   const int64_t c = blockIdx.x * 32LL + cl;
   T s = 0;
   if (c < C) {
 #pragma unroll 8
-    for (int64_t n = r; n < N; n += 8) s += G[n * C + c];
+    for (int64_t n = r; n < N; n += 8) s += G[n * pitch + c];
   }
   part[r][cl] = s;
   __syncthreads();
@@ -756,7 +762,7 @@ static int bwd_impl(const swvr_problem& p, const swvr_grads& g, void* ws, cudaSt
       return SWVR_ERR_CUDA;
     bwd_gs_kernel<T><<<grid_for(N * c), 256, 0, st>>>(S, G, delta, N, c);
     if (need_b)
-      colsum_kernel<T><<<static_cast<unsigned>(ceil_div(c, 32)), 256, 0, st>>>(G, N, c, g.grad_bias, g.grad_bias_dtype,
+      colsum_kernel<T><<<static_cast<unsigned>(ceil_div(c, 32)), 256, 0, st>>>(G, N, c, c, g.grad_bias, g.grad_bias_dtype,
                                                                               v0);
     // gE_c = P^T gO  (chunked.py:137-138)
     if (need_E &&
