@@ -15,9 +15,10 @@
 // on 256 rows of 128256 bf16: 92 us held, see below for what it takes now).  The usual filters leave few tokens, and
 // those are found without a weight or a bin for every score:
 //   1. the largest score, and each thread's largest;
-//   2. a score that enough tokens reach: for top-k, the k-th of the threads' largest scores (k tokens are at
-//      least that large, and few more are, as long as k is well below the number of threads); for a top-p
-//      without top-k the 128-th of them, beside the weight of the whole row; min-p knows its own;
+//   2. a score that every token which may be kept reaches: for top-k, the k-th of the threads' largest scores (k tokens
+//      are at least that large, and few more are, as long as k is well below the number of threads); for a top-p
+//      without top-k, the one at which the threads' largest scores alone make up p of the row's weight (so what
+//      is kept lies above); min-p knows its own;
 //   3. the tokens that reach it are gathered in one CTA, ordered by (score, index), cut by prefix sums, and u is
 //      looked up in the running weight by index.
 // Otherwise (no filter, a wide nucleus, long runs of equal scores) thresholds come from a histogram over kBins
@@ -435,16 +436,12 @@ __device__ __forceinline__ void sort_list(int n, Shared& s) {
   __syncthreads();
 }
 
-enum Found { kFound = 1, kNotListed, kUnsure };
-
 // The token from a list of m places and weights that holds every token the filters may keep (one CTA).
-// [total_lo, total_hi] holds the weight that top-p refers to (total_hi = 0: that of the first k).  `all`: the list is
-// known to hold the whole nucleus; otherwise kNotListed is returned when it does not.  kUnsure: tokens are kept or not
-// depending on where in the range the total lies; the list is as it was.
+// [total_lo, total_hi] holds the weight that top-p refers to (total_hi = 0: that of the first k).  False when tokens are kept
+// or not depending on where in the range the total lies; the list is as it was.
 // Up to 256 entries are ranked by comparing each with all others (512 / m threads an entry), more are sorted.
-__device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool by_p, double top_p, u64 total_lo, u64 total_hi,
-                                                  bool all, u64 cut, double u, int64_t* token, float* x_token, bool* mine,
-                                                  Shared& s) {
+__device__ __forceinline__ bool choose_from_list(int m, bool by_k, u64 k, bool by_p, double top_p, u64 total_lo, u64 total_hi,
+                                                 u64 cut, double u, int64_t* token, float* x_token, bool* mine, Shared& s) {
   if (m <= 256) {
     int G = 1;  // lanes that share an entry
     while (2 * G * m <= kThreads && G < 16) G *= 2;
@@ -472,8 +469,7 @@ __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool 
     if (by_p) {
       const u64 sum = block_sum(g == 0 ? w : 0, s);
       const u64 lo = nucleus(top_p, total_hi ? total_lo : sum), hi = nucleus(top_p, total_hi ? total_hi : sum);
-      if (!all && sum < hi) return kNotListed;
-      if (lo != hi && __syncthreads_or(w != 0 && ahead >= lo && ahead < hi)) return kUnsure;
+      if (lo != hi && __syncthreads_or(w != 0 && ahead >= lo && ahead < hi)) return false;
       if (ahead >= lo) w = 0;
     }
     if (pl < cut || g != 0) w = 0;
@@ -501,7 +497,7 @@ __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool 
         *mine = true;
       }
     }
-    return kFound;
+    return true;
   }
   int n = 512;
   while (n < m) n <<= 1;
@@ -522,7 +518,6 @@ __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool 
     const u64 listed = block_sum(sum, s);
     goal_p = nucleus(top_p, total_hi ? total_lo : listed);
     const u64 hi = nucleus(top_p, total_hi ? total_hi : listed);
-    if (!all && listed < hi) return kNotListed;
     if (goal_p != hi) {
       bool unsure = false;
       u64 at = ahead;
@@ -531,7 +526,7 @@ __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool 
         unsure |= w[e] != 0 && at >= goal_p && at < hi;
         at += w[e];
       }
-      if (__syncthreads_or(unsure)) return kUnsure;
+      if (__syncthreads_or(unsure)) return false;
     }
   }
   // kept ones, by index: the place with its halves exchanged orders by (index, score)
@@ -572,7 +567,7 @@ __device__ __forceinline__ Found choose_from_list(int m, bool by_k, u64 k, bool 
     }
     ahead += w[e];
   }
-  return kFound;
+  return true;
 }
 
 // Gathers in CTA 0 the places and weights of the scores that reach reach_x; returns their number, which may be over
@@ -975,10 +970,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     bool done = false;
     if (by_m || (by_k ? static_cast<u64>(k) <= min(kThreads * C / 2, kList / 2) : by_p)) {
       u64 lo = 0, hi = 0;  // the row's weight, for top-p without top-k
-      bool exact = false;
+      bool exact = false, few = true;
+      float reach_x = row.floor;  // a score that every token which may be kept reaches
       if (by_k || by_p) {
-        clear_bins(false, s);
-        if (t_top != -INFINITY && row.live(t_top)) atomicAdd(&s.count[row.bin(t_top)], 1u);
+        clear_bins(!by_k, s);
+        if (row.live(t_top)) {
+          atomicAdd(&s.count[row.bin(t_top)], 1u);
+          if (!by_k) s.add_mass(row.bin(t_top), row.weight(t_top));
+        }
         if (!by_k) {
           if (row.rough_ok) {
             const u64 w = cluster_join<true>(rough_total(sc, row, s), 2, s, cl);
@@ -989,39 +988,31 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
             lo = hi = cluster_join<true>(exact_total(sc, row, s), 2, s, cl);
           }
         }
-        merge_bins(false, s, cl);
+        merge_bins(!by_k, s, cl);
+        if (by_k) find_bin<true>(static_cast<u64>(k), s);
+        else find_bin<false>(nucleus(top_p, hi), s);
+        const int b = static_cast<int>(s.found[0]);
+        few = b < kBins;  // else the threads' largest scores do not make it up
+        // the lower end of that bin, less what rounding may have moved
+        if (b < kBins - 1) reach_x = fmaxf(reach_x, row.below((b + 1) / row.per_bin * 1.000001f));
       }
-      // a nucleus is looked for among the 128 largest threads' scores, then among more
-      const u64 most = min(kThreads * C / 2, 384u);
-      for (u64 wanted = by_k ? static_cast<u64>(k) : min(128ull, most);; wanted = most) {
-        float reach_x = row.floor;  // a score that every token which may be kept reaches
-        if (by_k || by_p) {
-          find_bin<true>(wanted, s);
-          const int b = static_cast<int>(s.found[0]);
-          if (by_k && b == kBins) break;  // fewer threads have live scores
-          // the lower end of that bin, less what rounding may have moved
-          if (b < kBins - 1) reach_x = fmaxf(reach_x, row.below((b + 1) / row.per_bin * 1.000001f));
-        }
-        if (by_m && !(by_k && by_p)) reach_x = fmaxf(reach_x, Cut(cut).x);  // (top-p after top-k weighs the first k)
+      if (by_m && !(by_k && by_p)) reach_x = fmaxf(reach_x, Cut(cut).x);  // (top-p after top-k weighs the first k)
+      if (few) {
         const uint32_t m = gather(sc, row, reach_x, [](float, int) { return true; }, s, cl);
-        if (m > kList) break;
-        const bool all = by_k || !by_p || reach_x == row.floor || reach_x == Cut(cut).x;
-        Found f = kFound;
-        for (int at = 3;; ++at) {  // slots 3, 4 in the first round, 6, 7 in the second
+        few = m <= kList;
+        for (int slot = 3; few; ++slot) {
+          bool sure = true;
           if (me == 0)
-            f = choose_from_list(static_cast<int>(m), by_k, static_cast<u64>(k), by_p, top_p, lo, hi, all, cut, u, &token,
-                                 &x_token, &mine, s);
-          if (!by_p || by_k) break;  // always found
-          const int slot = wanted == most && most > 128 ? at + 3 : at;
-          if (tid == 0 && me == 0) s.slot[slot] = f;
+            sure = choose_from_list(static_cast<int>(m), by_k, static_cast<u64>(k), by_p, top_p, lo, hi, cut, u, &token,
+                                    &x_token, &mine, s);
+          done = true;
+          if (by_k || !by_p || exact) break;
+          if (tid == 0 && me == 0) s.slot[slot] = sure;
           cl.sync();
-          f = static_cast<Found>(*cl.map_shared_rank(&s.slot[slot], 0));
-          if (f != kUnsure || exact) break;
+          if (*cl.map_shared_rank(&s.slot[slot], 0) != 0) break;
           exact = true;
           lo = hi = cluster_join<true>(exact_total(sc, row, s), 9, s, cl);
         }
-        if (f == kFound) done = true;
-        if (done || wanted == most) break;
       }
     }
     // -------------------------------------------------------------- many
