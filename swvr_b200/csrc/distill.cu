@@ -369,8 +369,9 @@ static int check(const swvr_distill* p) {
   if (!p) return fail(SWVR_ERR_INVALID_ARGUMENT, "problem is NULL");
   if (p->n_tokens < 0 || p->hidden < 0 || p->vocab < 0 || p->teacher < 0)
     return fail(SWVR_ERR_INVALID_ARGUMENT, "negative size");
-  if (p->n_tokens >= (1ll << 31) || p->vocab >= (1ll << 31) - 1 || p->hidden >= (1ll << 31))
-    return fail(SWVR_ERR_UNSUPPORTED, "sizes must be below 2^31");
+  // (a tile's last row index fits an int)
+  if (p->n_tokens > (1ll << 31) - 512 || p->vocab > (1ll << 31) - 512 || p->hidden > (1ll << 31) - 512)
+    return fail(SWVR_ERR_UNSUPPORTED, "sizes must be at most 2^31 - 512");
   if (p->teacher > kMaxTeacher)
     return fail(SWVR_ERR_UNSUPPORTED, "at most %d teacher entries per token, got %lld", kMaxTeacher, (long long)p->teacher);
   if (p->compute_dtype < SWVR_F32 || p->compute_dtype > SWVR_F16)
@@ -476,7 +477,7 @@ static GradPlan plan_grad(const swvr_distill& p, const swvr_distill_grads& g) {
   b.NT = static_cast<int>(ceil_div(p.n_tokens, 256));
   b.Npad = static_cast<int64_t>(b.NT) * 256;
   // equal chunks of at most 2 * chunk rows, as the readout's backward (plan_bwd in abi.cu)
-  const int64_t cmax = round_up(2 * std::max<int64_t>(p.chunk, 1), 256), V = std::max<int64_t>(p.vocab, 1);
+  const int64_t cmax = round_up(2 * std::min<int64_t>(p.chunk, 1ll << 30), 256), V = std::max<int64_t>(p.vocab, 1);
   b.C = static_cast<int>(std::min<int64_t>(round_up(ceil_div(V, ceil_div(V, cmax)), 256), 1ll << 30));
   b.need_h = g.grad_h != nullptr;
   b.need_W = g.grad_W != nullptr;
@@ -598,8 +599,7 @@ static int tc_fwd_distill(const swvr_distill& p, void* out, void* ws, size_t wsb
 }
 
 template <typename A>
-static cudaError_t exact_scores(const swvr_distill& p, const ExactPlan& x, int64_t v0, int64_t c, A* S, const A* bias,
-                                cudaStream_t st) {
+static cudaError_t exact_scores(const swvr_distill& p, int64_t v0, int64_t c, A* S, const A* bias, cudaStream_t st) {
   const int adt = sizeof(A) == 8 ? SWVR_F64 : SWVR_F32;
   return simt::gemm_bias<A>(st, p.n_tokens, c, p.hidden, static_cast<A>(p.logit_scale / p.temperature),
                             static_cast<const A*>(p.h), p.ldh, 1, static_cast<const A*>(p.W) + v0 * p.ldw, 1, p.ldw, S,
@@ -628,7 +628,7 @@ static int exact_fwd(const swvr_distill& p, void* out, void* ws, size_t wsb, cud
     if (bias) SWVR_CUDA(exact_bias<A>(p, bias, st));
     for (int64_t v0 = 0; v0 < p.vocab; v0 += x.C) {
       const int64_t c = std::min(x.C, p.vocab - v0);
-      SWVR_CUDA(exact_scores<A>(p, x, v0, c, S, bias, st));
+      SWVR_CUDA(exact_scores<A>(p, v0, c, S, bias, st));
       exact_update_kernel<A><<<static_cast<unsigned>(N), 256, 0, st>>>(
           S, c, round_up(c, 4), static_cast<int>(v0), static_cast<int>(p.teacher), p.sid, static_cast<A*>(p.z), m, l);
       SWVR_CUDA(cudaGetLastError());
@@ -769,7 +769,7 @@ static int exact_bwd(const swvr_distill& p, const swvr_distill_grads& g, const G
   const bool one = x.C >= V;  // one chunk: dh goes straight to its place
   for (int64_t v0 = 0; v0 < V; v0 += x.C) {
     const int64_t c = std::min(x.C, V - v0), ld = round_up(c, 4);
-    SWVR_CUDA(exact_scores<A>(p, x, v0, c, S, bias, st));
+    SWVR_CUDA(exact_scores<A>(p, v0, c, S, bias, st));
     exact_grad_kernel<A><<<static_cast<unsigned>(N), 256, 0, st>>>(
         c, ld, static_cast<int>(p.teacher), static_cast<int>(v0), p.sid, static_cast<const A*>(p.slogq),
         static_cast<const A*>(p.z), static_cast<const A*>(p.lse), static_cast<const A*>(p.lse_lo), gT, coef, S);

@@ -561,6 +561,11 @@ static cudaError_t sums(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const
   return cudaGetLastError();
 }
 
+// One launch sorts and clears dE; otherwise three launches a pass, after a memset.
+static bool one_block(const BwdPlan& b, int64_t n, int64_t D, const void* dE, int64_t lde) {
+  return b.small && n > 0 && lde == D && (reinterpret_cast<uintptr_t>(dE) & 15u) == 0;
+}
+
 template <typename T>
 static cudaError_t bwd(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const void* tokens, int bits, const void* g,
                        int64_t ldg, double scale, int64_t padding, void* dE, int64_t lde, char* ws, cudaStream_t st) {
@@ -570,7 +575,7 @@ static cudaError_t bwd(const BwdPlan& b, int64_t n, int64_t V, int64_t D, const 
   uint32_t* joins = reinterpret_cast<uint32_t*>(ws + b.off_joins);
   uint32_t* key[2] = {reinterpret_cast<uint32_t*>(ws + b.off_key[0]), reinterpret_cast<uint32_t*>(ws + b.off_key[1])};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + b.off_pos[0]), reinterpret_cast<uint32_t*>(ws + b.off_pos[1])};
-  if (b.small && n > 0 && lde == D && (reinterpret_cast<uintptr_t>(dE) & 15u) == 0) {
+  if (one_block(b, n, D, dE, lde)) {
     const int passes = (b.bits + 8) / 9, digit = (b.bits + passes - 1) / passes;  // at most 9 bits each
     const int64_t bytes = V * D * static_cast<int64_t>(sizeof(T));
     auto launch = [&](auto kern, int items) {
@@ -664,7 +669,7 @@ int swvr_embed_bwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tok
     return fail(SWVR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, b.bytes);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  ProfScope ps(kProfEmbed, st, n_tokens > 0 ? (b.small ? 1 : 3 * b.passes) + 2 : 0);
+  ProfScope ps(kProfEmbed, st, n_tokens == 0 ? 0 : (embed::one_block(b, n_tokens, dim, grad_E, ld_grad_E) ? 1 : 3 * b.passes) + 2);
   switch (dtype) {
     case SWVR_F32:
       SWVR_CUDA(embed::bwd<float>(b, n_tokens, vocab, dim, tokens, token_bits, grad_out, ld_grad_out, scale, padding_idx,

@@ -111,9 +111,9 @@ class _Embed(torch.autograd.Function):
 
 
 def _eager(*tensors) -> bool:
-    """True where an op may be run without its custom op: no tracing, plain tensors.  It saves the
-    dispatcher's host time, most of a call on a few tokens."""
-    return not torch.compiler.is_compiling() and all(
+    """True where an op may be run without its custom op: plain tensors, and no tracing or dispatch mode that has to
+    see it.  It saves the dispatcher's host time, most of a call on a few tokens."""
+    return not (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()) and all(
         t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
 
 

@@ -148,3 +148,25 @@ def test_two_streams_at_once():
     for loss, token, grads in got:
         assert torch.equal(loss, want[0]) and torch.equal(token, want[1])
         assert all(torch.equal(a, c) for a, c in zip(grads, got[0][2]))
+
+
+def test_a_dispatch_mode_sees_the_operators():
+    """Tracers and counters that work by a dispatch mode get the custom ops, and the same results."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    seen = []
+
+    class Record(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    args = parts(torch.bfloat16)
+    u = torch.rand(96, device="cuda")
+    run = lambda: (*torch.autograd.grad(step(*args), args[:4]),  # noqa: E731
+                   swvr.softmax_sample(torch.tanh(args[0].detach()[args[4]]), args[0].detach(), u, top_k=9))
+    want = run()
+    with Record():
+        got = run()
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    for op in ("embed", "embed_bwd", "distill", "distill_bwd", "sample"):
+        assert f"swvr_b200.{op}.default" in seen
