@@ -11,10 +11,14 @@
 // threads.
 //
 // A row is a cluster of 1 .. 8 CTAs, each with a contiguous share of the scores.  They are read from global memory in
-// every pass: after the first they are in L2, and shared memory full of scores would leave one CTA an SM (measured
-// on 256 rows of 128256 bf16: 92 us held, see below for what it takes now).  The usual filters leave few tokens, and
-// those are found without a weight or a bin for every score:
-//   1. the largest score, and each thread's largest;
+// every pass: after the first they are in L2, and shared memory full of scores would leave one CTA an SM (256 rows of 128256
+// bf16 then took 92 us; now 47).  What bounds it: at many rows the first pass, 11 instructions a score against HBM's
+// 66 MB (29 of the 47 us; the floor is 10), and the rows left open (below); at few rows the chain of cluster barriers and L2
+// round trips, some 6 us a row whatever its length (1 row of 152064 fp32, top-k and top-p: 12 us; 16 rows, top-p 0.9: 20 us;
+// 300 rows of 10007 with all three filters, one round of CTAs: 29 us).
+//
+// The usual filters leave few tokens, and those are found without a weight or a bin for every score:
+//   1. the largest score, and each thread's largest; for a top-p without top-k, and where there is no filter, the weight of all;
 //   2. a score that every token which may be kept reaches: for top-k, the k-th of the threads' largest scores (k tokens
 //      are at least that large, and few more are, as long as k is well below the number of threads); for a top-p
 //      without top-k, the one at which the threads' largest scores alone make up p of the row's weight (so what
@@ -26,13 +30,14 @@
 // (score, index) until kList members are left; a last pass over all scores sums the kept weights per warp, in
 // index order, and the warp whose range holds u rescans it.
 //
-// Sums over all scores (the row's weight for top-p, the last pass) are first taken with fp32 weights, an eighth of the
-// instructions.  A weight 2^y, y <= 0 in octaves, is then off by |y| 2 2^-24 ln 2 (difference and product rounded, the
-// factor in two parts) + 2^-22 (ex2) + 3 2^-24 (sums) relatively at most, and the weighted mean of |y| is at most the
-// distribution's entropy, log2 V: no partial sum is off by more than d = 2^-19 of the total up to V = 200000,
-// 2^-18 up to 2^20.  Where what is decided lies more than that from its border (2 d: both the running
-// weight and the total may be off) the fixed-point sums would decide the same; otherwise, a few rows in a
-// hundred, they are taken.
+// Sums over all scores (the row's weight for top-p, the last pass) are first taken with fp32 weights, a quarter of the
+// instructions, and where a row needs the sums of all its scores they come out of the pass that finds the largest: weights
+// are taken relative to a power of two, so a sum moves to a larger one exactly.  x / T in octaves is split
+// into an integer and a rest |f| <= 0.55; 2^f is off by 0.6 2^-24 (roundings of f) + 4 2^-24 (ex2), sums of eight by 3 2^-24,
+// and the fixed point itself (V weights of 2^-45, V up to 2^20) by 2^-25, relatively: no partial sum is off by more than
+// d = 9 2^-24 of the total.  Where what is decided lies more than that from its border (2 d: both the
+// running weight and the total may be off) the fixed-point sums would decide the same; otherwise, a row in a hundred,
+// they are taken.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -52,7 +57,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
 constexpr float kReach = 31.5f;  // e^-31.2 2^44 = 1/2: weights further below the largest score than 31.5 T round to 0
-constexpr int kRoughOne = 40;    // fp32 sums are kept in units of 2^-40 of the largest weight
+constexpr int kRoughOne = 40;    // fp32 sums are kept in units of 2^-40 of a power of two near the largest weight
 
 struct Setting {  // one value for all rows, or one per row
   const void* ptr;
@@ -76,7 +81,9 @@ struct Params {
   int lg_one;     // log2 of the fixed-point weight of the largest score: 44 or less
   bool aligned;   // rows start on 16-byte boundaries
   int64_t row0;   // first row of x among the rows of the settings, u and the outputs
+  int stage;      // 0: all rows, to the end; 1: those that need fixed-point sums are left open; 2: the open ones
 };
+constexpr int64_t kOpen = -2;
 
 __device__ __forceinline__ double setting(const Setting& s, int64_t row) { return s.ptr ? load_d(s.ptr, s.dt, row) : s.value; }
 
@@ -168,7 +175,42 @@ __device__ __forceinline__ float to_score(T v) {
   return f != f ? -INFINITY : f + 0.f;
 }
 
+// fp32 weights: 2^(x c), c = log2(e) / T.
+constexpr float kMagic = 12582912.f;  // 1.5 2^23: adding it rounds to an integer, which the low bits then hold
+struct Octaves {
+  float c, c_lo;  // c in two parts
+  float low;      // -2^20 / c: scores below it (and -inf and NaN) count as it
+
+  __device__ __forceinline__ explicit Octaves(double cd)
+      : c(static_cast<float>(cd)), c_lo(static_cast<float>(cd - c)), low(-1048576.f / c) {}
+  // the nearest integer to x c, plus kMagic's bits
+  __device__ __forceinline__ int place(float x) const { return __float_as_int(fmaf(fmaxf(x, low), c, kMagic)); }
+  // 2^(x c) over 2^(the integer of place `ref`), at least some 2^-125 and at most 2^64 for x up to 64 octaves above ref
+  __device__ __forceinline__ float weight(float x, int ref) const {
+    x = fmaxf(x, low);
+    const float t = fmaf(x, c, kMagic);
+    const float f = fmaf(x, c_lo, fmaf(x, c, kMagic - t));
+    const int k = max(__float_as_int(t) - ref, -125);
+    return __int_as_float(__float_as_int(ex2(f)) + k * (1 << 23));
+  }
+  // the sum over a pack of scores
+  template <int VEC, typename P>
+  __device__ __forceinline__ double pack(const P& p, int ref) const {
+    float v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = weight(to_float(p.e[e]), ref);
+#pragma unroll
+    for (int o = VEC / 2; o > 0; o /= 2)
+#pragma unroll
+      for (int e = 0; e < o; ++e) v[e] += v[e + o];
+    return static_cast<double>(v[0]);
+  }
+};
+
 struct Row {
+  Octaves oct;
+  int ref;        // fp32 weights are relative to 2^(the integer of this place: the largest score's)
+  bool rough_ok;  // they are within their bound
   float top;      // the largest score
   double top_d, c64;  // top, and 64 log2(e) / T
   double invT;
@@ -177,26 +219,11 @@ struct Row {
   float floor;    // scores below have no weight; above -inf
   float per_bin;  // bins per unit of score
   const double* root;  // 2^(j / 64 + lg_one), j < 64
-  bool rough_ok;  // fp32 weights are within their bound
-  int rough_bits; // 18 or 19
-  float c32, c32_lo;  // log2(e) / T in two parts
 
-  // -inf and NaN: 2^-88, nothing
-  __device__ __forceinline__ float rough(float x) const {
-    const float d = fmaxf(x - top, -2.f * reach);
-    return ex2(fmaf(d, c32, d * c32_lo));
-  }
-  // the sum over a pack of scores
-  template <int VEC, typename P>
-  __device__ __forceinline__ double rough_pack(const P& p) const {
-    float v[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = rough(to_float(p.e[e]));
-#pragma unroll
-    for (int o = VEC / 2; o > 0; o /= 2)
-#pragma unroll
-      for (int e = 0; e < o; ++e) v[e] += v[e + o];
-    return static_cast<double>(v[0]);
+  __device__ __forceinline__ float rough(float x) const { return oct.weight(x, ref); }
+  // 2^-40 of 2^(the integer of ref) in units of 2^-lg_one of the largest weight
+  __device__ __forceinline__ double unit() const {
+    return ldexp(exp2((ref - __float_as_int(kMagic)) - top_d * (c64 / 64)), lg_one - kRoughOne);
   }
   __device__ __forceinline__ bool live(float x) const { return x >= floor; }  // not NaN either
   // exp((x - top) / T) 2^lg_one, rounded.  With y = 64 log2(e) (x - top) / T = n + f, |f| <= 1/2:
@@ -235,7 +262,6 @@ struct Scores {
   int n;
   uint32_t first;  // its index in the row
 
-  __device__ __forceinline__ float at(int i) const { return to_score(x[i]); }
   struct alignas(16) Pack {
     T e[VEC];
   };
@@ -723,7 +749,7 @@ __device__ __forceinline__ u64 thresholds(const Scores<T>& sc, const Row& row, b
   return cut;
 }
 
-// The weight of this CTA's scores, in units of 2^-lg_one of the largest: in fixed point, or from fp32 weights.
+// The weight of this CTA's scores, in units of 2^-lg_one of the largest.
 // (By value: a reference to the caller's structs would keep them in local memory.)
 template <typename T>
 __device__ __noinline__ u64 exact_total(const Scores<T> sc, const Row row, Shared& s) {
@@ -734,14 +760,43 @@ __device__ __noinline__ u64 exact_total(const Scores<T> sc, const Row row, Share
   });
   return block_sum(w, s);
 }
-__device__ __forceinline__ u64 rough_units(double w) { return static_cast<u64>(ldexp(w, kRoughOne)); }
+__device__ __forceinline__ u64 rough_units(double w, int octaves = 0) { return static_cast<u64>(ldexp(w, kRoughOne + octaves)); }
+// how far an fp32 sum of these units may be off
+__device__ __forceinline__ u64 rough_error(u64 total) { return (total >> 21) + (total >> 24) + 1; }
+
+// Scores per warp: each has a contiguous sixteenth of its CTA's share.
 template <typename T>
-__device__ __forceinline__ u64 rough_total(const Scores<T>& sc, const Row& row, Shared& s) {
-  constexpr int VEC = Scores<T>::VEC;
+__device__ __forceinline__ int warp_span(const Scores<T>& sc) {
+  constexpr int STEP = 32 * Scores<T>::VEC;
+  return (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;
+}
+
+// This thread's largest score among its warp's, and with kSum the weight of those it reads, relative to 2^(the integer of ref).
+// ref follows the largest score only once that is 64 octaves above it.
+template <bool kSum, typename T>
+__device__ __forceinline__ void first_pass(const Scores<T>& sc, const Octaves& oct, float* t_top, double* sum, int* ref) {
+  constexpr int VEC = Scores<T>::VEC, STEP = 32 * VEC;
+  const int span = warp_span(sc), i0 = min(sc.n, static_cast<int>(threadIdx.x) / 32 * span), i1 = min(sc.n, i0 + span);
+  float top = -INFINITY;  // (fmaxf leaves NaN out)
   double w = 0;
-  sc.template packs<2>(threadIdx.x * VEC, sc.n, kThreads * VEC,
-                       [&](const typename Scores<T>::Pack& p, int) { w += row.template rough_pack<VEC>(p); });
-  return block_sum(rough_units(w), s);
+  int r = 0;
+  sc.template packs<kSum ? 2 : 4>(i0 + static_cast<int>(threadIdx.x) % 32 * VEC, i1, STEP, [&](const typename Scores<T>::Pack& p, int) {
+    float m = to_float(p.e[0]);
+#pragma unroll
+    for (int e = 1; e < VEC; ++e) m = fmaxf(m, to_float(p.e[e]));
+    top = fmaxf(top, m);
+    if constexpr (kSum) {
+      const int at = oct.place(m);
+      if (at - r > 64) {
+        w = ldexp(w, r - at);
+        r = at;
+      }
+      w += oct.template pack<VEC>(p, r);
+    }
+  });
+  *t_top = top + 0.f;
+  *sum = w;
+  *ref = r;
 }
 
 // Weights of the scores [i0, i1) of this CTA at or ahead of the cut, summed over the warp; i0 a multiple of VEC.
@@ -764,7 +819,7 @@ __device__ __forceinline__ u64 span_weight(const Scores<T>& sc, const Row& row, 
   } else {
     double r = 0;
     if (!cut) {
-      sc.template packs<2>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int) { r += row.template rough_pack<VEC>(p); });
+      sc.template packs<2>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int) { r += row.oct.template pack<VEC>(p, row.ref); });
     } else {
       sc.template packs<2>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int i) {
         float t = 0.f;
@@ -780,17 +835,19 @@ __device__ __forceinline__ u64 span_weight(const Scores<T>& sc, const Row& row, 
   }
 }
 
-// The token from all scores at or ahead of the cut, by sums in index order: of each warp's sixteenth of the share; where
-// the goal falls, of sixteenths of that; then of single scores.  Rough sums: false where the border is too near.
+// The token from all scores at or ahead of the cut, by sums in index order: of each warp's sixteenth of the share (w, or taken
+// here where there is none); where the goal falls, of sixteenths of that; then of single scores.  Rough sums: false where
+// the border is too near.
+constexpr u64 kNone = ~0ull;
 template <bool kExact, typename T>
-__device__ __forceinline__ bool sweep(const Scores<T>& sc, const Row& row, u64 cut, double u, int slot, int64_t* token,
+__device__ __forceinline__ bool sweep(const Scores<T>& sc, const Row& row, u64 cut, double u, int slot, u64 w, int64_t* token,
                                       float* x_token, bool* mine, Shared& s, cg::cluster_group& cl) {
   constexpr int VEC = Scores<T>::VEC, STEP = 32 * VEC;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const unsigned me = cl.block_rank();
-  const int span = (sc.n + STEP * kWarps - 1) / (STEP * kWarps) * STEP;  // scores per warp, contiguous
+  const int span = warp_span(sc);
   const Cut kept(cut);
-  u64 w = span_weight<kExact>(sc, row, kept, cut != 0, min(sc.n, warp * span), min(sc.n, (warp + 1) * span));
+  if (w == kNone) w = span_weight<kExact>(sc, row, kept, cut != 0, min(sc.n, warp * span), min(sc.n, (warp + 1) * span));
   __syncthreads();
   if (lane == 0) s.part[warp] = w;
   __syncthreads();
@@ -808,7 +865,7 @@ __device__ __forceinline__ bool sweep(const Scores<T>& sc, const Row& row, u64 c
     if (c < me) ahead += v[c];
     total += v[c];
   }
-  const u64 goal = goal_of(u, total), margin = kExact ? 0 : (total >> (row.rough_bits - 1)) + 2;
+  const u64 goal = goal_of(u, total), margin = kExact ? 0 : 2 * rough_error(total);
   if (ahead < goal && goal <= ahead + own) {  // this CTA's share holds it
     int part = 0;
     while (part < kWarps - 1 && ahead + s.part[part] < goal) ahead += s.part[part++];
@@ -880,12 +937,12 @@ __device__ __noinline__ Choice choose_among_many(const Scores<T> sc, const Row r
   int64_t token = 0;
   float x = 0.f;
   bool mine = false;
-  if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 11, &token, &x, &mine, s, cl))
-    sweep<true>(sc, row, cut, u, 5, &token, &x, &mine, s, cl);
+  if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 11, kNone, &token, &x, &mine, s, cl))
+    sweep<true>(sc, row, cut, u, 5, kNone, &token, &x, &mine, s, cl);
   return {static_cast<uint32_t>(token), x, mine};
 }
 
-// kFilters: some row may have top-k, top-p or min-p; without, the kernel needs fewer registers and more of it fits an SM.
+// kFilters: some row may have top-k, top-p or min-p; without, the kernel needs fewer registers.
 template <typename T, bool kFilters>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -894,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   const unsigned C = cl.num_blocks(), me = cl.block_rank();
   const int64_t r = blockIdx.x / C, row_id = p.row0 + r;
   const int tid = threadIdx.x;
-  constexpr int VEC = Scores<T>::VEC;
+  if (!kFilters && p.stage == 2 && p.token[row_id] != kOpen) return;  // the whole cluster: the token is written at the end
   const int64_t first = static_cast<int64_t>(me) * p.share;
   Scores<T> sc;
   sc.x = static_cast<const T*>(p.x) + r * p.ld + first;
@@ -913,14 +970,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   const bool by_k = kFilters && k > 0 && k < p.V, by_p = kFilters && top_p < 1.0, by_m = kFilters && min_p > 0.0;
   const double lm = by_m && !greedy ? log(min(min_p, 1.0)) : 0.0, invT = 1.0 / temp;
 
-  // ---------------------------------------------------------------- the largest score
-  float t_top = -INFINITY;  // of this thread (fmaxf leaves NaN out)
-  sc.template packs<4>(tid * VEC, sc.n, kThreads * VEC, [&](const typename Scores<T>::Pack& q, int) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) t_top = fmaxf(t_top, to_float(q.e[k]));
-  });
-  t_top += 0.f;
-  Row row;
+  // ---------------------------------------------------------------- the largest score, and the weight of all
+  const Octaves oct(1.4426950408889634 * invT);
+  float t_top;  // of this thread
+  double t_sum;
+  int t_ref;
+  const bool by_all = !greedy && (kFilters ? by_p && !by_k : p.stage != 2);  // the weight of all scores is asked for
+  if (by_all) first_pass<true>(sc, oct, &t_top, &t_sum, &t_ref);
+  else first_pass<false>(sc, oct, &t_top, &t_sum, &t_ref);
+  Row row{oct};
   row.top = score_of(static_cast<uint32_t>(cluster_join<false>(block_max32(order_of(t_top), s), 0, s, cl)));
   if (p.V == 0 || row.top == -INFINITY) {  // nothing to choose from
     if (me == 0 && tid == 0) {
@@ -938,10 +996,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   row.floor = fmaxf(row.top - row.reach, -FLT_MAX);
   row.per_bin = static_cast<float>(kBins) / row.reach;
   row.root = s.root;
-  row.c32 = static_cast<float>(1.4426950408889634 * row.invT);
-  row.c32_lo = static_cast<float>(1.4426950408889634 * row.invT - row.c32);
-  row.rough_bits = p.V <= 200000 ? 19 : 18;
-  row.rough_ok = p.V <= (1 << 20) && row.top < INFINITY && row.c32 > 1e-30f && row.c32 < 1e30f;
+  row.ref = oct.place(row.top);
+  row.rough_ok = p.V <= (1 << 20) && oct.c > 1e-25f && oct.c < 1e25f && fabsf(row.top) * oct.c < 524288.f;
+  const u64 weight = by_all && row.rough_ok ? rough_units(t_sum, t_ref - row.ref) : 0;  // of the scores that this thread read
 
   int64_t token = 0;
   float x_token = row.top;
@@ -980,9 +1037,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         }
         if (!by_k) {
           if (row.rough_ok) {
-            const u64 w = cluster_join<true>(rough_total(sc, row, s), 2, s, cl);
-            lo = (w - (w >> row.rough_bits) - 1) << (row.lg_one - kRoughOne);
-            hi = (w + (w >> row.rough_bits) + 1) << (row.lg_one - kRoughOne);
+            const u64 w = cluster_join<true>(block_sum(weight, s), 2, s, cl);
+            const double unit = row.unit();
+            lo = static_cast<u64>(static_cast<double>(w - rough_error(w)) * unit);
+            hi = static_cast<u64>(static_cast<double>(w + rough_error(w)) * unit) + 1;
           } else {
             exact = true;
             lo = hi = cluster_join<true>(exact_total(sc, row, s), 2, s, cl);
@@ -1022,8 +1080,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         token = c.token;
         x_token = c.x;
         mine = c.mine;
-      } else if (!row.rough_ok || !sweep<false>(sc, row, cut, u, 11, &token, &x_token, &mine, s, cl)) {
-        sweep<true>(sc, row, cut, u, 5, &token, &x_token, &mine, s, cl);
+      } else if (!row.rough_ok || p.stage == 2 || !sweep<false>(sc, row, 0, u, 11, warp_sum(weight), &token, &x_token, &mine, s, cl)) {
+        if (p.stage == 1) {
+          if (me == 0 && tid == 0) p.token[row_id] = kOpen;
+          cl.sync();
+          return;
+        }
+        sweep<true>(sc, row, 0, u, 5, kNone, &token, &x_token, &mine, s, cl);
       }
     }
   }
@@ -1040,20 +1103,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
 
 // ------------------------------------------------------------------ host
 template <typename T>
-static cudaError_t launch_t(Params p, cudaStream_t st) {
-  static_assert(kMaxCluster == 8, "cluster sizes below");
-  const bool filters = p.k_ptr || p.k > 0 || p.p.ptr || p.p.value < 1.0 || p.m.ptr || p.m.value > 0.0;
-  // Two CTAs fit an SM.  With filters one round of them (64 rows of 128256 fp32, top-k: 18 us with 256 CTAs, 32 with 512);
-  // without, two, so that a row that needs its fixed-point sums does not hold up the rest (256 rows of 128256 bf16: 66 us
-  // with 512, 77 with 256).
-  const int64_t most = (filters ? 2 : 4) * kNumSMsB200;
-  int C = 1;
-  while (C < 8 && 2 * C * p.N <= most && p.V > 2048 * C) C *= 2;
+static cudaError_t launch_c(Params p, int C, bool filters, cudaStream_t st) {
   p.share = static_cast<int>(round_up(ceil_div(std::max<int64_t>(p.V, 1), C), 32));
-  p.aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.ld * sizeof(T)) % 16 == 0;
-  int lg = 0;
-  while ((1ll << lg) < p.V) ++lg;
-  p.lg_one = std::min(44, 62 - lg);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1068,6 +1119,29 @@ static cudaError_t launch_t(Params p, cudaStream_t st) {
   cfg.stream = st;
   static_assert(sizeof(Shared) <= 48 * 1024, "more needs cudaFuncSetAttribute");
   return cudaLaunchKernelEx(&cfg, filters ? sample_kernel<T, true> : sample_kernel<T, false>, p);
+}
+
+template <typename T>
+static cudaError_t launch_t(Params p, cudaStream_t st) {
+  static_assert(kMaxCluster == 8, "cluster sizes below");
+  const bool filters = p.k_ptr || p.k > 0 || p.p.ptr || p.p.value < 1.0 || p.m.ptr || p.m.value > 0.0;
+  // Two CTAs fit an SM: one round of them (64 rows of 128256 fp32, top-k: 17 us with 256 CTAs, 32 with 512).  Rows that need
+  // fixed-point sums would hold up the others where a row has few CTAs: without filters they are left to a second launch that
+  // gives each of them as many as its length allows (256 rows of 128256 bf16: 53 us in one
+  // launch of 512 CTAs, 47 in two; 55 where a few clusters look for the open rows and one may get two of them).
+  int wide = 1;
+  while (wide < kMaxCluster && p.V > 2048 * wide) wide *= 2;
+  int C = wide;
+  while (C > 1 && C * p.N > 2 * kNumSMsB200) C /= 2;
+  p.aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.ld * sizeof(T)) % 16 == 0;
+  int lg = 0;
+  while ((1ll << lg) < p.V) ++lg;
+  p.lg_one = std::min(44, 62 - lg);
+  p.stage = !filters && C < wide ? 1 : 0;
+  cudaError_t e = launch_c<T>(p, C, filters, st);
+  if (e != cudaSuccess || p.stage == 0) return e;
+  p.stage = 2;
+  return launch_c<T>(p, wide, false, st);
 }
 
 static cudaError_t launch(const Params& p, cudaStream_t st) {
@@ -1117,8 +1191,9 @@ static int64_t head_rows(const swvr_problem& p) {
 static int check_head(const swvr_problem* p) {
   if (!p) return fail(SWVR_ERR_INVALID_ARGUMENT, "problem is NULL");
   if (p->n_tokens < 0 || p->hidden < 0 || p->vocab < 0) return fail(SWVR_ERR_INVALID_ARGUMENT, "negative size");
-  if (p->n_tokens >= (1ll << 28) || p->vocab >= (1ll << 31) || p->hidden >= (1ll << 31))
-    return fail(SWVR_ERR_UNSUPPORTED, "sizes must be below 2^31 (rows 2^28)");
+  // (a tile's last row index fits an int)
+  if (p->n_tokens >= (1ll << 28) || p->vocab > (1ll << 31) - 512 || p->hidden > (1ll << 31) - 512)
+    return fail(SWVR_ERR_UNSUPPORTED, "sizes must be at most 2^31 - 512 (rows below 2^28)");
   if (p->compute_dtype != SWVR_F32 && !is_tc(p->compute_dtype))
     return fail(SWVR_ERR_UNSUPPORTED, "sampling computes in bf16, fp16 or fp32");
   if (p->bias && !float_dtype(p->bias_dtype)) return fail(SWVR_ERR_INVALID_ARGUMENT, "unknown bias dtype %d", p->bias_dtype);

@@ -361,3 +361,46 @@ def test_rows_of_the_lowest_value_beside_minus_infinity():
         for kw in (dict(), dict(T=1e30), dict(k=9), dict(p=0.5), dict(m=0.9)):
             got = check(x, uniform(6), **kw)
             assert bool((got % 2 == 1).all())
+
+
+def test_a_row_gives_the_same_token_in_any_batch():
+    """Many rows, which have few CTAs each, against the same rows in small batches: u on borders of the running weight
+    (where fp32 sums leave the token open), temperatures at both ends, rows with nothing to choose from."""
+    N, V = 310, 9001
+    x = logits(N, V, torch.bfloat16)
+    T = torch.where(torch.arange(N, device="cuda") % 7 < 5, 0.9, 1.0)
+    T[::41], T[1::41], T[2::41] = 0.0, 1e-30, 1e30
+    x[3::41] = -math.inf
+    x[4::41, 100] = math.inf
+    w = exact(x, uniform(N), T=T)[2].cumsum(1)
+    u = uniform(N).double()
+    u[::2] = (w.gather(1, torch.randint(0, V, (N, 1), generator=torch.Generator().manual_seed(3)).cuda())[:, 0] / w[:, -1])[::2]
+    u = u.nan_to_num().clamp(0, 1 - 2.0 ** -53)
+    call = lambda i, j: swvr.sample_logits(x[i:j], u[i:j], temperature=T[i:j], return_logprobs=True)  # noqa: E731
+    got, lp = call(0, N)
+    assert near(got, *exact(x, u, T=T)[::2], u, V)
+    for i in range(0, N, 31):
+        tok, part = call(i, i + 31)
+        assert torch.equal(tok, got[i:i + 31]) and torch.equal(part, lp[i:i + 31])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again, lp2 = call(0, N)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, got) and torch.equal(lp2, lp)
+    del graph
+
+
+def test_fp32_sums_far_from_zero():
+    """Scores whose integer part in octaves is large, or that rise along the row by more than fp32's range of weights."""
+    V = 6000
+    u = uniform(20)
+    for shift in (0.0, 3e4, -3e4, 3e5, -3e5):
+        x = (logits(20, V) + shift)
+        for kw in (dict(), dict(p=0.9), dict(T=0.25)):
+            check(x, u, **kw)
+    ramp = torch.linspace(-4000, 4000, V, device="cuda").expand(20, V) + logits(20, V)
+    for kw in (dict(), dict(p=0.9), dict(T=300.0), dict(T=300.0, p=0.9)):
+        check(ramp, u, **kw)
+        check(ramp.flip(1), u, **kw)
