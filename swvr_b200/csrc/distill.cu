@@ -53,7 +53,7 @@ constexpr int kMaxTeacher = 1024;  // entries per token: the sort's shared memor
 // One warp per token: log q of each entry, their sum, and the entries sorted by id (each entry's rank
 // is the number of entries before it, K_t^2 / 32 compares a lane: K_t is tens).  Entries with a negative id or a
 // logit of -inf are left out (id INT_MAX, q = 0, sorted behind); an id >= V is an error: the token's
-// loss and gradient are NaN.
+// loss and gradient are NaN.  8192 tokens of 64 entries: 20 us.
 template <typename A>
 __global__ void __launch_bounds__(32 * kWarps)
     teacher_kernel(int64_t N, int64_t V, int Kt, const void* __restrict__ ids, int bits, const void* __restrict__ t,
@@ -136,7 +136,8 @@ __device__ __forceinline__ void total_loss(int64_t N, bool mean, const A* each, 
 
 // Sources of (m, l): `splits` partial slots of head_kernel in log2 units (slot (n / 256 * splits + s) * 256
 // + n % 256), or one natural-unit pair per token (splits = 0).  The block that finishes last sums the tokens (all of
-// them, in a fixed order); `done` counts finished blocks and is cleared by teacher_kernel.
+// them, in a fixed order); `done` counts finished blocks and is cleared by teacher_kernel.  2048 tokens of 64 entries: 5.3 us
+// (a second launch for the sum would cost more than the last block's 2 us); 8192 tokens of 64: 37 us.
 template <typename A>
 __global__ void __launch_bounds__(32 * kWarps)
     each_kernel(int64_t N, int Kt, int splits, const A* __restrict__ m, const A* __restrict__ l,
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(32 * kWarps)
 // gradient.  Then the ranges, from the largest |gT| max(1, sum q), a:
 // f[0] what dS is multiplied by when stored, f[1] its undoing (dh, dW), f[2] the binary exponent of db's fixed point.
 // fp16 dS is scaled by a power of two that puts its largest value near 2^13, so that small gradients (1 / N of a
-// mean) do not fall below fp16's range; bf16 has fp32's.
+// mean) do not fall below fp16's range; bf16 has fp32's.  8192 tokens: 7.5 us; one block, so that the ranges need no second launch.
 constexpr int kGradThreads = 1024;
 
 template <typename A>
@@ -254,7 +255,8 @@ __device__ __forceinline__ A merged_q(const int32_t* sid, const A* slogq, int j,
   return q;
 }
 
-// The teacher entries of vocabulary rows [v0, v1): written over the dense dS^T, and their part of db.
+// The teacher entries of vocabulary rows [v0, v1): written over the dense dS^T, and their part of db.  A thread an entry,
+// bound by reading the ids and by scattered 2-byte stores: 8192 x 64 entries, 9 us a chunk.
 template <bool kBF16>
 __global__ void __launch_bounds__(256)
     entries_kernel(int64_t N, int Kt, int v0, int v1, const int32_t* __restrict__ sid, const float* __restrict__ slogq,
@@ -292,7 +294,7 @@ __global__ void db_kernel(int rows, int v0, int TS, const float* __restrict__ pa
   store_d(gb, gb_dt, v0 + i, s);
 }
 
-// dh from its slices of accumulators, added in slice order.
+// dh from its slices of accumulators, added in slice order.  Bound by HBM: 8192 x 2560, one slice (126 MB): 26 us.
 __global__ void cast_scaled_kernel(const float* __restrict__ src, int slices, int64_t slice, const float* __restrict__ f,
                                    void* dst, int dt, int64_t n) {
   const float k = f[1];
@@ -311,7 +313,7 @@ __global__ void scaled_bias_kernel(int64_t V, const void* bias, int dt, A inv_T,
   if (v < V) out[v] = static_cast<A>(load_d(bias, dt, v)) * inv_T;
 }
 
-// One block per token: picks the teacher's scores of the chunk, then updates (m, l) with the row.
+// One block per token: picks the teacher's scores of the chunk, then updates (m, l) with the row.  256 rows of 1000: 3.7 us.
 template <typename A>
 __global__ void __launch_bounds__(256)
     exact_update_kernel(const A* __restrict__ S, int64_t C, int64_t pitch, int v0, int Kt, const int32_t* __restrict__ sid, A* z, A* m,

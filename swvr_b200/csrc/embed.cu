@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(kSmallThreads)
 // block.  A token that begins and ends inside a chunk is written to dE at once; the part of
 // the chunk's first token that began earlier goes to part[chunk][0], the part of its last token
 // that goes on (and began here) to part[chunk][1], and the chunk to the list of those that join_kernel starts from (in any
-// order: each is joined by itself).
+// order: each is joined by itself).  Four rows in flight a thread.  Bound by HBM and its latency: 16384 rows of 2560 bf16 in 30 us
+// (84 MB read, some 50 written: 4.4 TB/s).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) sum_kernel(int64_t n, int len, int chunks, int packs, uint32_t V,
                                                   const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
