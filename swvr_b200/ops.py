@@ -112,8 +112,10 @@ def _problem(h, W, E, bias, scale, chunk, cdt) -> nat.Problem:
 def _prepare_k(x, cdt):
     """``x`` [rows, K] as the library takes it: in ``cdt``, with K zero-padded to a multiple of 8 on
     the tensor-core path (zero columns add nothing to h . W^T)."""
-    K = x.shape[1]
-    if _tensor_core(cdt) and K % 8 != 0:
+    K, tc = x.shape[1], _tensor_core(cdt)
+    if x.dtype is cdt and x.stride() == (K, 1) and (not tc or K > 0 and K % 8 == 0 and x.data_ptr() % 16 == 0):
+        return x  # as it is, without the questions below (a few us of host time)
+    if tc and K % 8 != 0:
         x = torch.nn.functional.pad(x.to(cdt), (0, (K + 7) // 8 * 8 - K))
     return _operand(x, cdt)
 
