@@ -226,8 +226,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(int64_t n, S
 }
 
 // Up to kSmallSort pairs: one block sorts them in shared memory while the other blocks of the launch clear dE, which takes
-// longer where it matters (778 MB: 125 us; the sort of 16384 pairs with 18-bit keys: 14 us).  Pairs stay in registers, `digit`
-// bits a pass; warp w owns items [w * 32 * ITEMS, ...), so ranks follow the list order as above.
+// longer where it matters (778 MB: 125 us; the sort of 16384 pairs with 18-bit keys: 39 us, of 8192: 21 us).  Pairs stay in
+// registers, `digit` bits a pass; warp w owns items [w * 32 * ITEMS, ...), so ranks follow the list order as above.  The sorted list
+// is put together in shared memory: scattered stores of it took 9 us more.
 constexpr int kSmallThreads = 1024, kSmallSort = 16 * kSmallThreads, kSmallDigits = 512;
 
 struct SmallSmem {
@@ -292,19 +293,22 @@ __device__ __forceinline__ void small_sort(int n, const SortIn& in, int bits, in
         run += c;
       }
     __syncthreads();
-    const bool last = shift + digit >= bits;
-    uint32_t* ko = last ? key_out : sk;
-    uint32_t* po = last ? pos_out : sp;
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
       if (base + r * 32 + lane < n) {
         const uint32_t o = s.cnt[warp][(key[r] >> shift) & (digits - 1u)] + rank[r];
-        ko[o] = key[r];
-        po[o] = pos[r];
+        sk[o] = key[r];
+        sp[o] = pos[r];
       }
     }
-    if (last) return;
     __syncthreads();
+    if (shift + digit >= bits) {
+      for (int i = t; i < n; i += kSmallThreads) {
+        key_out[i] = sk[i];
+        pos_out[i] = sp[i];
+      }
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
       const int i = base + r * 32 + lane;

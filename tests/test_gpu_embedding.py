@@ -233,3 +233,36 @@ def test_compiled_whole():
     want = torch.autograd.grad(f(tok, E), E)[0]
     got = torch.autograd.grad(torch.compile(f, fullgraph=True, backend="aot_eager")(tok, E), E)[0]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,N,V,D", [(torch.bfloat16, 3000, 40000, 2560), (torch.float32, 1, 9001, 4104), (torch.float16, 16384, 2000003, 40),
+                                         (torch.float64, 700, 100000, 250)])
+def test_gradient_of_a_large_table(dtype, N, V, D):
+    """Every row that no token names is zero, in a buffer that held something else, and the others are the
+    sums.  Tokens crowd at both ends and in runs, among them the padding row."""
+    gen = torch.Generator().manual_seed(V)
+    tok = torch.randint(0, V, (N,), generator=gen)
+    tok[::3] = torch.randint(0, min(V, 40), (len(tok[::3]),), generator=gen)
+    tok[1::5] = V - 1 - torch.randint(0, min(V, 40), (len(tok[1::5]),), generator=gen)
+    tok[::7] = 5
+    tok = tok.cuda()
+    E = torch.zeros(V, D, dtype=dtype, device="cuda", requires_grad=True)
+    g = torch.randn(N, D, device="cuda").to(dtype)
+    for pad in (None, 5):
+        junk = torch.full((V, D), 7.0, dtype=dtype, device="cuda")
+        del junk  # the gradient's memory, from the same cache
+        dE, = torch.autograd.grad(swvr.embedding_lookup(tok, E, scale=0.5, padding_idx=pad), E, g)
+        named = torch.zeros(V, dtype=torch.bool, device="cuda")
+        named[tok] = True
+        if pad is not None:
+            named[pad] = False
+        assert not bool(dE[~named].any())
+        rows, where = torch.unique(tok, return_inverse=True)
+        want = torch.zeros(len(rows), D, dtype=torch.float64, device="cuda").index_add_(0, where, 0.5 * g.double())
+        most = torch.zeros_like(want).index_add_(0, where, 0.5 * g.double().abs())
+        keep = named[rows]
+        count = torch.bincount(where, minlength=len(rows))[:, None].double()
+        acc = 2.0 ** -53 if dtype == torch.float64 else 2.0 ** -24
+        # the sum of count terms in fp32 / fp64, the product with scale exact, rounded once
+        bound = count * acc * most + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).tiny
+        assert bool(((dE[rows].double() - want).abs() <= bound)[keep].all())
