@@ -12,8 +12,8 @@
 //
 // A row is a cluster of 1 .. 8 CTAs, each with a contiguous share of the scores.  They are read from global memory in
 // every pass: after the first they are in L2, and shared memory full of scores would leave one CTA an SM (256 rows of 128256
-// bf16 then took 92 us; now 47).  What bounds it: at many rows the first pass, 11 instructions a score against HBM's
-// 66 MB (29 of the 47 us; the floor is 10), and the rows left open (below); at few rows the chain of cluster barriers and L2
+// bf16 then took 92 us; now 47).  What bounds it: at many rows the first pass (29 of the 47 us for 66 MB; FMAs in
+// pairs, more loads in flight or loads ahead of the work did not shorten it) and the rows left open (below); at few rows the chain of cluster barriers and L2
 // round trips, some 6 us a row whatever its length (1 row of 152064 fp32, top-k and top-p: 12 us; 16 rows, top-p 0.9: 20 us;
 // 300 rows of 10007 with all three filters, one round of CTAs: 29 us).
 //
@@ -57,6 +57,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
 constexpr float kReach = 31.5f;  // e^-31.2 2^44 = 1/2: weights further below the largest score than 31.5 T round to 0
+constexpr int kRoughMost = 1 << 20;  // longest row with fp32 sums
 constexpr int kRoughOne = 40;    // fp32 sums are kept in units of 2^-40 of a power of two near the largest weight
 
 struct Setting {  // one value for all rows, or one per row
@@ -997,7 +998,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   row.per_bin = static_cast<float>(kBins) / row.reach;
   row.root = s.root;
   row.ref = oct.place(row.top);
-  row.rough_ok = p.V <= (1 << 20) && oct.c > 1e-25f && oct.c < 1e25f && fabsf(row.top) * oct.c < 524288.f;
+  row.rough_ok = p.V <= kRoughMost && oct.c > 1e-25f && oct.c < 1e25f && fabsf(row.top) * oct.c < 524288.f;
   const u64 weight = by_all && row.rough_ok ? rough_units(t_sum, t_ref - row.ref) : 0;  // of the scores that this thread read
 
   int64_t token = 0;
@@ -1118,6 +1119,7 @@ static cudaError_t launch_c(Params p, int C, bool filters, cudaStream_t st) {
   cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = st;
   static_assert(sizeof(Shared) <= 48 * 1024, "more needs cudaFuncSetAttribute");
+  ProfScope ps(kProfSample, st);
   return cudaLaunchKernelEx(&cfg, filters ? sample_kernel<T, true> : sample_kernel<T, false>, p);
 }
 
@@ -1127,8 +1129,8 @@ static cudaError_t launch_t(Params p, cudaStream_t st) {
   const bool filters = p.k_ptr || p.k > 0 || p.p.ptr || p.p.value < 1.0 || p.m.ptr || p.m.value > 0.0;
   // Two CTAs fit an SM: one round of them (64 rows of 128256 fp32, top-k: 17 us with 256 CTAs, 32 with 512).  Rows that need
   // fixed-point sums would hold up the others where a row has few CTAs: without filters they are left to a second launch that
-  // gives each of them as many as its length allows (256 rows of 128256 bf16: 53 us in one
-  // launch of 512 CTAs, 47 in two; 55 where a few clusters look for the open rows and one may get two of them).
+  // gives each of them as many as its length allows (256 rows of 128256 bf16: 53 us in one launch of 512 CTAs, 47 in two; 55 where a
+  // few clusters look for the open rows and one may get two of them).
   int wide = 1;
   while (wide < kMaxCluster && p.V > 2048 * wide) wide *= 2;
   int C = wide;
@@ -1137,7 +1139,7 @@ static cudaError_t launch_t(Params p, cudaStream_t st) {
   int lg = 0;
   while ((1ll << lg) < p.V) ++lg;
   p.lg_one = std::min(44, 62 - lg);
-  p.stage = !filters && C < wide ? 1 : 0;
+  p.stage = !filters && C < wide && p.V <= kRoughMost ? 1 : 0;
   cudaError_t e = launch_c<T>(p, C, filters, st);
   if (e != cudaSuccess || p.stage == 0) return e;
   p.stage = 2;
@@ -1274,7 +1276,6 @@ int swvr_sample_logits(int64_t n_rows, int64_t vocab, const void* logits, int32_
   p.x = logits;
   p.dt = dtype;
   p.ld = ld;
-  ProfScope ps(kProfSample, static_cast<cudaStream_t>(stream));
   SWVR_CUDA(sample::launch(p, static_cast<cudaStream_t>(stream)));
   return SWVR_OK;
 }
@@ -1306,7 +1307,6 @@ int swvr_sample(const swvr_problem* p, const swvr_sampling* sampling, void* work
     if (p->vocab > 0) SWVR_TRY(sample::head_scores(*p, n0, n, static_cast<float*>(workspace), ld, st));
     q.N = n;
     q.row0 = n0;
-    ProfScope ps(kProfSample, st);
     SWVR_CUDA(sample::launch(q, st));
   }
   return SWVR_OK;
