@@ -136,3 +136,13 @@ def test_distill_fake_impls_give_shapes(dtype, adt):
     grads = torch.ops.swvr_b200.distill_bwd(out, h, W, b, ids, t, None, w, *saved, 2.0, 1.0, 8192, dtype, nat.REDUCE_MEAN,
                                             True, False, True, True)
     assert [tuple(g.shape) for g in grads] == [(6, 16), (0,), (100,), (6,)] and grads[3].dtype == adt
+
+
+@pytest.mark.parametrize("field", ["N", "V"])
+def test_sizes_within_a_tile_of_2_31_are_refused(field):
+    """A tile's last row index has to fit an int."""
+    lib, n = nat.lib(), ctypes.c_size_t(0)
+    small = dict(N=1, V=1, Kt=1)
+    for size, code in ((2 ** 31 - 512, nat.OK), (2 ** 31 - 511, nat.ERR_UNSUPPORTED)):
+        assert lib.swvr_distill_fwd_workspace_size(_problem(**{**small, field: size}), ctypes.byref(n)) == code
+    assert lib.swvr_distill_bwd_workspace_size(_problem(**small, chunk=2 ** 62), nat.DistillGrads(), ctypes.byref(n)) == nat.OK

@@ -111,3 +111,16 @@ def test_sampling_fake_impls_give_shapes():
     assert tok.shape == lp.shape == (5,) and tok.dtype == torch.int64 and lp.dtype == torch.float32
     tok, lp = torch.ops.swvr_b200.sample(m(5, 16), m(90, 16), None, m(5), 1.0, torch.bfloat16, *rest, False)
     assert tok.shape == (5,) and lp.shape == (0,)
+
+
+def test_a_vocabulary_within_a_tile_of_2_31_is_refused():
+    """A tile's last row index has to fit an int."""
+    lib, n = nat.lib(), ctypes.c_size_t(0)
+    p = nat.Problem()
+    p.n_tokens, p.hidden, p.compute_dtype, p.bias_dtype = 1, 64, nat.BF16, nat.F32
+    p.h = p.W = 1 << 20
+    p.ldh = p.ldw = 64
+    p.logit_scale = 1.0
+    for vocab, code in ((2 ** 31 - 512, nat.OK), (2 ** 31 - 511, nat.ERR_UNSUPPORTED)):
+        p.vocab = vocab
+        assert lib.swvr_sample_workspace_size(p, ctypes.byref(n)) == code
