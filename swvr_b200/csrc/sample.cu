@@ -145,7 +145,8 @@ struct Shared {
   u64 part[kWarps];       // per-warp results of a block reduction or scan
   u64 slot[14];           // values other CTAs of the cluster read, each written once
   u64 found[3];           // boundary bin, and count or weight before it
-  uint32_t n_list;
+  uint32_t n_list;        // read by the cluster's other CTAs
+  uint32_t n_kept;        // by this CTA alone
 
   __device__ __forceinline__ void add_mass(int b, u64 w) {
     const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&mass_lo[b], lo);
@@ -500,15 +501,15 @@ __device__ __forceinline__ bool choose_from_list(int m, bool by_k, u64 k, bool b
       if (ahead >= lo) w = 0;
     }
     if (pl < cut || g != 0) w = 0;
-    if (threadIdx.x == 0) s.n_list = 0;
+    if (threadIdx.x == 0) s.n_kept = 0;  // (other CTAs may still read n_list)
     const u64 goal = goal_of(u, block_sum(w, s));  // its barriers: the list has been read, the count is 0
     if (w != 0) {  // kept ones move together
-      const uint32_t j = atomicAdd(&s.n_list, 1u);
+      const uint32_t j = atomicAdd(&s.n_kept, 1u);
       s.list[j] = pl;
       s.list_w[j] = w;
     }
     __syncthreads();
-    const uint32_t kept = s.n_list;
+    const uint32_t kept = s.n_kept;
     for (uint32_t e = threadIdx.x; e < kept; e += kThreads) {
       const u64 mine_pl = s.list[e];
       const uint32_t low = static_cast<uint32_t>(mine_pl);  // complemented index: a larger one comes first
