@@ -111,9 +111,11 @@ class _Embed(torch.autograd.Function):
 
 
 def _eager(*tensors) -> bool:
-    """True where an op may be run without its custom op: plain tensors, and no tracing or dispatch mode that has to
-    see it.  It saves the dispatcher's host time, most of a call on a few tokens."""
-    return not (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()) and all(
+    """True where an op may be run without its custom op: plain tensors, and no tracing, dispatch mode or functorch
+    transform (``torch.func.vmap`` and the like, whose tensors are of the plain type) that has to see it.  It saves the
+    dispatcher's host time, most of a call on a few tokens."""
+    return not (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()
+                or torch._C._are_functorch_transforms_active()) and all(
         t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
 
 

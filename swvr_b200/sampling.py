@@ -172,7 +172,7 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     lead = logits.shape[:-1]
     args = _settings(lead, u, temperature, top_k, top_p, min_p)
     x, uu = _rows(logits, lead), u if u.dim() == 1 else u.reshape(-1)
-    if _eager(x, uu):
+    if _eager(x, uu, *args[4:]):
         with torch.no_grad():
             out = _sample_logits(x, uu, *args, bool(return_logprobs))
     else:
@@ -201,7 +201,7 @@ def softmax_sample(h, W, u, bias=None, *, temperature=1.0, top_k=None, top_p=Non
     lead = h.shape[:-1]
     args = _settings(lead, u, temperature, top_k, top_p, min_p)
     h2, uu = _rows(h, lead), u if u.dim() == 1 else u.reshape(-1)
-    if _eager(h2, W, bias, uu):
+    if _eager(h2, W, bias, uu, *args[4:]):
         with torch.no_grad():
             out = _sample_head(h2, W, bias, uu, float(logit_scale), cdt, *args, bool(return_logprobs))
     else:
