@@ -33,9 +33,9 @@
 // Sums over all scores (the row's weight for top-p, the last pass) are first taken with fp32 weights, a quarter of the
 // instructions, and where a row needs the sums of all its scores they come out of the pass that finds the largest: weights
 // are taken relative to a power of two, so a sum moves to a larger one exactly.  x / T in octaves is split
-// into an integer and a rest |f| <= 0.55; 2^f is off by 0.6 2^-24 (roundings of f) + 4 2^-24 (ex2), sums of eight by 3 2^-24,
-// and the fixed point itself (V weights of 2^-45, V up to 2^20) by 2^-25, relatively: no partial sum is off by more than
-// d = 9 2^-24 of the total.  Where what is decided lies more than that from its border (2 d: both the
+// into an integer and a rest |f| <= 0.55; 2^f is off by 0.6 2^-24 (roundings of f) + 4 2^-24 (ex2), sums of eight, in a tree, by 3 2^-24,
+// and the fixed point itself (V weights of half a unit, V up to 2^20) by up to 2 2^-24, relatively: no partial sum is off by more than
+// d = 10 2^-24 of the total (rough_error).  Where what is decided lies more than that from its border (2 d: both the
 // running weight and the total may be off) the fixed-point sums would decide the same; otherwise, a row in a hundred,
 // they are taken.
 #include <cooperative_groups.h>
@@ -45,6 +45,7 @@
 
 #include "common.cuh"
 #include "ptx.cuh"
+#include "sample_sums.cuh"
 #include "tc.cuh"
 
 namespace swvr {
@@ -57,7 +58,6 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 1024, kList = 1024;
 constexpr int kBinsPer = kBins / kThreads;
 constexpr float kReach = 31.5f;  // e^-31.2 2^44 = 1/2: weights further below the largest score than 31.5 T round to 0
-constexpr int kRoughMost = 1 << 20;  // longest row with fp32 sums
 constexpr int kRoughOne = 40;    // fp32 sums are kept in units of 2^-40 of a power of two near the largest weight
 
 struct Setting {  // one value for all rows, or one per row
@@ -201,11 +201,7 @@ struct Octaves {
     float v[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = weight(to_float(p.e[e]), ref);
-#pragma unroll
-    for (int o = VEC / 2; o > 0; o /= 2)
-#pragma unroll
-      for (int e = 0; e < o; ++e) v[e] += v[e + o];
-    return static_cast<double>(v[0]);
+    return static_cast<double>(tree_sum<VEC>(v));
   }
 };
 
@@ -763,8 +759,6 @@ __device__ __noinline__ u64 exact_total(const Scores<T> sc, const Row row, Share
   return block_sum(w, s);
 }
 __device__ __forceinline__ u64 rough_units(double w, int octaves = 0) { return static_cast<u64>(ldexp(w, kRoughOne + octaves)); }
-// how far an fp32 sum of these units may be off
-__device__ __forceinline__ u64 rough_error(u64 total) { return (total >> 21) + (total >> 24) + 1; }
 
 // Scores per warp: each has a contiguous sixteenth of its CTA's share.
 template <typename T>
@@ -824,13 +818,13 @@ __device__ __forceinline__ u64 span_weight(const Scores<T>& sc, const Row& row, 
       sc.template packs<2>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int) { r += row.oct.template pack<VEC>(p, row.ref); });
     } else {
       sc.template packs<2>(i0 + lane * VEC, i1, STEP, [&](const Pack& p, int i) {
-        float t = 0.f;
+        float v[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float x = to_score(p.e[e]);
-          t += kept.keeps(x, sc.first + i + e) ? row.rough(x) : 0.f;
+          v[e] = kept.keeps(x, sc.first + i + e) ? row.rough(x) : 0.f;
         }
-        r += static_cast<double>(t);
+        r += static_cast<double>(tree_sum<VEC>(v));
       });
     }
     return warp_sum(rough_units(r));
@@ -1137,9 +1131,7 @@ static cudaError_t launch_t(Params p, cudaStream_t st) {
   int C = wide;
   while (C > 1 && C * p.N > 2 * kNumSMsB200) C /= 2;
   p.aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.ld * sizeof(T)) % 16 == 0;
-  int lg = 0;
-  while ((1ll << lg) < p.V) ++lg;
-  p.lg_one = std::min(44, 62 - lg);
+  p.lg_one = lg_one_of(p.V);
   p.stage = !filters && C < wide && p.V <= kRoughMost ? 1 : 0;
   cudaError_t e = launch_c<T>(p, C, filters, st);
   if (e != cudaSuccess || p.stage == 0) return e;
