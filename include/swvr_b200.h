@@ -268,7 +268,8 @@ int swvr_embed_bwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tok
  * int32.  sid, slogq, z, lse, lse_lo, qsum, each and stats are written by the forward and read by the backward: the
  * caller keeps them, and h, W, bias, weight and the sizes unchanged, in between.  W and h as in
  * swvr_problem.  At most 1024 teacher entries.  [N, vocab] is never materialised on the
- * tensor-core path; the fp32 / fp64 path stages `chunk` vocabulary rows of it.
+ * tensor-core path; the fp32 / fp64 path stages `chunk` vocabulary rows of it, and takes at most
+ * 65535 * 128 tokens.
  */
 typedef struct swvr_distill {
   int64_t n_tokens, hidden, vocab, teacher;

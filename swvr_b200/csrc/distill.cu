@@ -374,6 +374,8 @@ static int check(const swvr_distill* p) {
   // (a tile's last row index fits an int)
   if (p->n_tokens > (1ll << 31) - 512 || p->vocab > (1ll << 31) - 512 || p->hidden > (1ll << 31) - 512)
     return fail(SWVR_ERR_UNSUPPORTED, "sizes must be at most 2^31 - 512");
+  if (!is_tc(p->compute_dtype) && p->n_tokens > simt::kMostRows)
+    return fail(SWVR_ERR_UNSUPPORTED, "at most %lld tokens in fp32 / fp64", (long long)simt::kMostRows);
   if (p->teacher > kMaxTeacher)
     return fail(SWVR_ERR_UNSUPPORTED, "at most %d teacher entries per token, got %lld", kMaxTeacher, (long long)p->teacher);
   if (p->compute_dtype < SWVR_F32 || p->compute_dtype > SWVR_F16)
@@ -442,7 +444,7 @@ struct ExactPlan {
 static ExactPlan plan_exact(const swvr_distill& p, bool bwd, bool need_h) {
   ExactPlan e{};
   const size_t es = acc_size(p);
-  e.C = std::min(p.chunk, std::max<int64_t>(p.vocab, 1));
+  e.C = std::min({p.chunk, std::max<int64_t>(p.vocab, 1), simt::kMostRows});  // a chunk's rows are those of its dW product
   size_t off = align_up(es * p.n_tokens * round_up(e.C, 4), 256);  // rows of a multiple of 4: 16-byte staging
   e.off_bias = off;
   off += align_up(es * p.vocab, 256);

@@ -1177,10 +1177,12 @@ static int params(const swvr_sampling* o, int64_t N, int64_t V, Params* p) {
   return SWVR_OK;
 }
 
-// Rows whose fp32 scores are held at a time: at most 256 MiB of them, at least one row.
+// Rows whose fp32 scores are held at a time: at most 256 MiB of them, at least one row, and no more than a launch of the
+// fp32 product takes.
 static int64_t head_rows(const swvr_problem& p) {
   const int64_t pitch = round_up(std::max<int64_t>(p.vocab, 1), 4) * 4;
-  return std::max<int64_t>(1, std::min<int64_t>(p.n_tokens, (256ll << 20) / pitch));
+  const int64_t most = is_tc(p.compute_dtype) ? p.n_tokens : std::min(p.n_tokens, simt::kMostRows);
+  return std::max<int64_t>(1, std::min<int64_t>(most, (256ll << 20) / pitch));
 }
 
 static int check_head(const swvr_problem* p) {

@@ -22,6 +22,7 @@ namespace simt {
 // coalesce for row- and column-major operands alike, 16 bytes at a time where the layout allows
 // it; the fp32 kernel reads its fragments from shared memory 16 bytes at a time.
 constexpr int BM = 128, BN = 128, BK = 8, PAD = 4;
+constexpr int64_t kMostRows = 65535LL * BM;  // of C in a launch: row tiles are grid.y
 
 template <typename T>
 struct GemmTileLoader {

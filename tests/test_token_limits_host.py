@@ -1,0 +1,42 @@
+"""CPU tests of the sizes at which the token operators' launches and workspaces have to give way."""
+import ctypes
+
+import pytest
+
+from swvr_b200 import _native as nat
+from test_distill_host import _problem
+
+
+def test_fp32_head_takes_tiny_vocabularies_in_chunks_of_rows():
+    """The fp32 product has at most 65535 row tiles of 128 in a launch."""
+    lib, n = nat.lib(), ctypes.c_size_t(0)
+    p = nat.Problem()
+    p.hidden, p.compute_dtype, p.bias_dtype = 8, nat.F32, nat.F32
+    p.h = p.W = 1 << 20
+    p.ldh = p.ldw = 8
+    p.logit_scale = 1.0
+    for vocab in (1, 4, 8):
+        p.vocab = vocab
+        for rows in (65535 * 128, 65535 * 128 + 1, (1 << 28) - 1):
+            p.n_tokens = rows
+            assert lib.swvr_sample_workspace_size(p, ctypes.byref(n)) == nat.OK
+            assert n.value == min(65535 * 128, (256 << 20) // (16 * ((vocab + 3) // 4))) * 16 * ((vocab + 3) // 4)
+
+
+@pytest.mark.parametrize("dt", [nat.F32, nat.F64])
+def test_exact_path_takes_what_its_products_can_launch(dt):
+    """At most 65535 row tiles of 128: tokens past that are refused, chunks of the vocabulary are kept to it, and the
+    largest sizes that are taken do not wrap the workspace's."""
+    lib, n, most = nat.lib(), ctypes.c_size_t(0), 65535 * 128
+    g = nat.DistillGrads()
+    g.grad_out = g.grad_h = g.grad_W = 1 << 20
+    g.ld_grad_W = 1
+    for N, code in ((most, nat.OK), (most + 1, nat.ERR_UNSUPPORTED), (2 ** 31 - 512, nat.ERR_UNSUPPORTED)):
+        p = _problem(N=N, K=1, V=2 ** 31 - 512, Kt=1, dt=dt, chunk=2 ** 62)
+        assert lib.swvr_distill_fwd_workspace_size(p, ctypes.byref(n)) == code
+        assert lib.swvr_distill_bwd_workspace_size(p, g, ctypes.byref(n)) == code
+    p = _problem(N=most, K=1, V=2 ** 31 - 512, Kt=1, dt=dt, chunk=2 ** 62)
+    assert lib.swvr_distill_fwd_workspace_size(p, ctypes.byref(n)) == nat.OK
+    assert n.value >= most * most * (8 if dt == nat.F64 else 4)
+    p = _problem(N=2 ** 31 - 512, K=8, V=1000, Kt=1, dt=nat.BF16)  # the tensor-core path has no such tiles
+    assert lib.swvr_distill_fwd_workspace_size(p, ctypes.byref(n)) == nat.OK
