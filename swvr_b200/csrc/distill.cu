@@ -441,7 +441,7 @@ struct ExactPlan {
   size_t off_bias, off_m, off_l, off_done, off_dh, off_part, bytes;
 };
 
-static ExactPlan plan_exact(const swvr_distill& p, bool bwd, bool need_h) {
+static ExactPlan plan_exact(const swvr_distill& p, bool need_h, bool need_W) {
   ExactPlan e{};
   const size_t es = acc_size(p);
   e.C = std::min({p.chunk, std::max<int64_t>(p.vocab, 1), simt::kMostRows});  // a chunk's rows are those of its dW product
@@ -455,14 +455,12 @@ static ExactPlan plan_exact(const swvr_distill& p, bool bwd, bool need_h) {
   e.off_done = off;
   off += 256;
   e.off_dh = off;
-  if (bwd && need_h) off += align_up(es * p.n_tokens * p.hidden, 256);
-  // slices of a product split along its sum, where its 128 x 128 tiles would leave SMs idle (simt::gemm_split)
+  if (need_h) off += align_up(es * p.n_tokens * p.hidden, 256);
+  // slices of dh and dW split along their sums, where 128 x 128 tiles would leave SMs idle (simt::gemm_split)
   e.off_part = off;
-  if (es == 4) {
-    int64_t most = simt::splitk_floats(p.n_tokens, e.C);
-    if (bwd) most = std::max({most, simt::splitk_floats(p.n_tokens, p.hidden), simt::splitk_floats(e.C, p.hidden)});
-    off += align_up(4 * most, 256);
-  }
+  if (es == 4)
+    off += align_up(4 * std::max(need_h ? simt::splitk_floats(p.n_tokens, p.hidden) : 0,
+                                 need_W ? simt::splitk_floats(e.C, p.hidden) : 0), 256);
   e.bytes = off + 256;
   return e;
 }
@@ -757,7 +755,7 @@ static int tc_bwd_distill(const swvr_distill& p, const swvr_distill_grads& g, co
 
 template <typename A>
 static int exact_bwd(const swvr_distill& p, const swvr_distill_grads& g, const GradPlan& b, char* w, cudaStream_t st) {
-  const ExactPlan x = plan_exact(p, true, b.need_h);
+  const ExactPlan x = plan_exact(p, b.need_h, b.need_W);
   const int64_t N = p.n_tokens, K = p.hidden, V = p.vocab;
   const int adt = sizeof(A) == 8 ? SWVR_F64 : SWVR_F32;
   const A s = static_cast<A>(p.logit_scale);
@@ -797,7 +795,7 @@ static int exact_bwd(const swvr_distill& p, const swvr_distill_grads& g, const G
 }
 
 static size_t bwd_bytes(const swvr_distill& p, const GradPlan& b) {
-  return b.bytes + (is_tc(p.compute_dtype) ? 0 : plan_exact(p, true, b.need_h).bytes);
+  return b.bytes + (is_tc(p.compute_dtype) ? 0 : plan_exact(p, b.need_h, b.need_W).bytes);
 }
 
 }  // namespace distill

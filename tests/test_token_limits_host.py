@@ -40,3 +40,26 @@ def test_exact_path_takes_what_its_products_can_launch(dt):
     assert n.value >= most * most * (8 if dt == nat.F64 else 4)
     p = _problem(N=2 ** 31 - 512, K=8, V=1000, Kt=1, dt=nat.BF16)  # the tensor-core path has no such tiles
     assert lib.swvr_distill_fwd_workspace_size(p, ctypes.byref(n)) == nat.OK
+
+
+def test_exact_forward_asks_for_no_split_sums():
+    """The scores' product is never split along its sum: the forward's workspace is the staged scores, the scaled bias, two
+    numbers a token and a counter; the backward adds the gradients of the tokens, dh, and slices of dh and dW where asked for."""
+    lib, n = nat.lib(), ctypes.c_size_t(0)
+    N, K, V, slack = 1024, 64, 10007, 8192
+    p = _problem(N=N, K=K, V=V, Kt=8, dt=nat.F32)
+    assert lib.swvr_distill_fwd_workspace_size(p, ctypes.byref(n)) == nat.OK
+    fwd = 4 * (N * 8192 + V + 2 * N)
+    assert fwd <= n.value <= fwd + slack
+
+    def bwd(h=None, W=None):
+        g = nat.DistillGrads()
+        g.grad_out, g.grad_h, g.grad_W, g.ld_grad_W = 1 << 20, h, W, K
+        assert lib.swvr_distill_bwd_workspace_size(p, g, ctypes.byref(n)) == nat.OK
+        return n.value - fwd
+
+    both = 4 * 2 * N  # g T and g T sum q
+    assert both <= bwd() <= both + slack
+    assert both + 4 * 17 * N * K <= bwd(h=1 << 20) <= both + 4 * 17 * N * K + slack  # dh and 16 slices of it
+    assert both + 4 * 16 * 8192 * K <= bwd(W=1 << 20) <= both + 4 * 16 * 8192 * K + slack
+    assert both + 4 * (16 * 8192 + N) * K <= bwd(h=1 << 20, W=1 << 20) <= both + 4 * (16 * 8192 + N) * K + slack
