@@ -10,6 +10,7 @@
 // 16-bit p would lose the difference where the student has learnt the teacher).
 // The teacher's part of db is a sum over tokens in no fixed order: it is added in 64-bit fixed point, where
 // order does not matter.
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -24,6 +25,17 @@ template <typename A>
 __device__ __forceinline__ A load_a(const void* p, int dt, int64_t i) {
   if constexpr (sizeof(A) == 8) return load_d(p, dt, i);
   else return load_f(p, dt, i);
+}
+// A teacher's logit: fp64 ones past fp32's range count as its ends there (a mask of the type's lowest value is no -inf).
+template <typename A>
+__device__ __forceinline__ A load_logit(const void* p, int dt, int64_t i) {
+  if constexpr (sizeof(A) == 4) {
+    if (dt == SWVR_F64) {
+      const double d = static_cast<const double*>(p)[i];
+      return static_cast<A>(isfinite(d) ? fmin(fmax(d, -static_cast<double>(FLT_MAX)), static_cast<double>(FLT_MAX)) : d);
+    }
+  }
+  return load_a<A>(p, dt, i);
 }
 __device__ __forceinline__ float exp_a(float x) { return expf(x); }
 __device__ __forceinline__ double exp_a(double x) { return exp(x); }
@@ -70,7 +82,7 @@ __global__ void __launch_bounds__(32 * kWarps)
   for (int k = lane; k < Kt; k += 32) {
     const int64_t i = n * Kt + k;
     const int64_t v = bits == 64 ? static_cast<const int64_t*>(ids)[i] : static_cast<int64_t>(static_cast<const int32_t*>(ids)[i]);
-    const A x = load_a<A>(t, t_dt, i) * inv_T;
+    const A x = load_logit<A>(t, t_dt, i);
     const bool dead = v < 0 || x == -static_cast<A>(INFINITY);
     if (!dead && v >= V) bad = true;
     tv[k] = dead ? -static_cast<A>(INFINITY) : x;
@@ -81,17 +93,20 @@ __global__ void __launch_bounds__(32 * kWarps)
   mx = warp_max(mx);
   A sum = 0;
   for (int k = lane; k < Kt; k += 32)
-    if (id[k] != INT_MAX) sum += exp_a(tv[k] - mx);
+    if (id[k] != INT_MAX) sum += exp_a((tv[k] - mx) * inv_T);
   sum = warp_sum(sum);
   bad = __any_sync(0xffffffffu, bad);
-  // log q from differences to the largest: the logsumexp itself would round at its own size
-  const A ref = t_lse ? t_lse[n] : mx, lsum = t_lse ? A(0) : log_a(sum);
+  // log q from differences to the largest: the logsumexp itself would round at its own size, and t / T may be past the
+  // type's range where the differences are not (entries at its lowest value, T below 1)
+  const A lsum = log_a(sum);
   A qs = 0;
   for (int k = lane; k < Kt; k += 32) {
     const int32_t mine = id[k];
     int rank = 0;
     for (int j = 0; j < Kt; ++j) rank += id[j] < mine || (id[j] == mine && j < k);
-    const A lq = mine == INT_MAX ? -static_cast<A>(INFINITY) : (tv[k] - ref) - lsum;
+    const A lq = mine == INT_MAX ? -static_cast<A>(INFINITY)
+                 : t_lse         ? fma(tv[k], inv_T, -t_lse[n])
+                                 : (tv[k] - mx) * inv_T - lsum;
     sid[n * Kt + rank] = mine;
     slogq[n * Kt + rank] = lq;
     if (mine != INT_MAX) qs += exp_a(lq);
