@@ -3,48 +3,32 @@
 
 #include <cuda.h>
 
-#include <map>
-#include <mutex>
-#include <utility>
+#include <atomic>
 
 #include "common.cuh"
 
 namespace swvr {
 namespace tc {
 
-// How many clusters of `cfg` (of two CTAs) of this kernel can be resident on the current device, with its
-// dynamic shared memory allowed: asked of the runtime once per kernel and device (the two calls take some
-// 10 us of host time, more than a launch).
-inline cudaError_t resident_clusters(const void* kern, const cudaLaunchConfig_t& cfg, int* clusters) {
-  static std::mutex mu;
-  static std::map<std::pair<int, const void*>, int> known;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lk(mu);
-  const auto it = known.find({dev, kern});
-  if (it != known.end()) {
-    *clusters = it->second;
-    return cudaSuccess;
-  }
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cfg.dynamicSmemBytes));
-  if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(clusters, kern, &cfg);
-  if (e == cudaSuccess) known[{dev, kern}] = *clusters;
-  return e;
+// Dynamic shared memory beyond 48 KiB allowed for a kernel.  It holds for the current context alone, so it is asked for at
+// every launch.
+inline cudaError_t allow_smem(const void* kern, int bytes) {
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-// Dynamic shared memory beyond 48 KiB allowed for a kernel, once per kernel and device.
-inline cudaError_t allow_smem(const void* kern, int bytes) {
-  static std::mutex mu;
-  static std::map<std::pair<int, const void*>, int> known;
+// How many clusters of `cfg` (of two CTAs) of this kernel can be resident on the current device, with its dynamic shared
+// memory allowed.  `known`, one per kernel, keeps the number by device (0: not asked yet): the question takes some 10 us of host time,
+// more than a launch, and a number from another context costs speed at most.
+constexpr int kKnownDevices = 32;
+using KnownClusters = std::atomic<int>[kKnownDevices];
+inline cudaError_t resident_clusters(const void* kern, const cudaLaunchConfig_t& cfg, KnownClusters& known, int* clusters) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = allow_smem(kern, static_cast<int>(cfg.dynamicSmemBytes));
   if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lk(mu);
-  int& most = known[{dev, kern}];
-  if (most >= bytes) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) most = bytes;
+  if (dev < kKnownDevices && (*clusters = known[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  e = cudaOccupancyMaxActiveClusters(clusters, kern, &cfg);
+  if (e == cudaSuccess && dev < kKnownDevices) known[dev].store(*clusters, std::memory_order_relaxed);
   return e;
 }
 

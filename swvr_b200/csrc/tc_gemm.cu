@@ -316,8 +316,9 @@ static cudaError_t launch(const GemmMaps& m, const GemmParams& prm, int max_pair
   cfg.dynamicSmemBytes = Cfg::SMEM_ALLOC;
   cfg.stream = st;
   cfg.gridDim = dim3(2 * 74, 1, 1);
+  static KnownClusters known;
   int clusters = 0;
-  const cudaError_t e = resident_clusters(reinterpret_cast<const void*>(kern), cfg, &clusters);
+  const cudaError_t e = resident_clusters(reinterpret_cast<const void*>(kern), cfg, known, &clusters);
   if (e != cudaSuccess) return e;
   const int tiles = prm.dw_tiles + prm.dh_tiles;
   int pairs = std::min(std::min(clusters, max_pairs), tiles);

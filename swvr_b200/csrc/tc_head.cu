@@ -390,8 +390,9 @@ static cudaError_t launch_head(const HeadMaps& m, const HeadParams& prm, int max
   cfg.dynamicSmemBytes = Cfg::SMEM_ALLOC;
   cfg.stream = st;
   cfg.gridDim = dim3(2 * 74, 1, 1);
+  static KnownClusters known;
   int clusters = 0;
-  const cudaError_t e = resident_clusters(reinterpret_cast<const void*>(kern), cfg, &clusters);
+  const cudaError_t e = resident_clusters(reinterpret_cast<const void*>(kern), cfg, known, &clusters);
   if (e != cudaSuccess) return e;
   int pairs = std::min(std::min(clusters, max_pairs), prm.units);
   if (pairs < 1) pairs = 1;
