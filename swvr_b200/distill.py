@@ -19,7 +19,7 @@ from torch import nn
 
 from . import _native as nat
 from .api import _compute_dtype, _weight_of
-from .embedding import _eager
+from .embedding import _eager, _refuse_forward_ad
 from .ops import (_REDUCTIONS, _grad_buffer, _ld, _no_grad_marker, _prepare_k, _require_cuda, _tensor_core, _workspace,
                   acc_dtype, default_chunk_size)
 
@@ -244,8 +244,10 @@ def softmax_distill(h, W, teacher_ids, teacher_logits, bias=None, *, temperature
     nat.dtype_code(teacher_logits.dtype)
     cdt = _compute_dtype(h, W)
     nat.dtype_code(cdt)
+    _refuse_forward_ad("softmax_distill", h, W, bias, weight)
     adt = acc_dtype(cdt)
     N = math.prod(lead)
+
     def row(t):
         t = t if t.dtype == adt else t.to(adt)
         return (t if t.dim() == 1 else t.reshape(N)).contiguous()

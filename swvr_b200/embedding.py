@@ -11,6 +11,7 @@ and sums each one's rows in order, in fp32 (fp64 for fp64), without atomics.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .ops import _require_cuda, _workspace
@@ -119,6 +120,18 @@ def _eager(*tensors) -> bool:
         t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
 
 
+def _refuse_forward_ad(name, *tensors):
+    """Raise where a tensor carries a tangent (``torch.func.jvp``, dual tensors): a custom op would pass none on, and
+    forward mode would take that for a derivative of zero."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        while t is not None and torch._C._functorch.is_batchedtensor(t):
+            t = torch._C._functorch.get_unwrapped(t)
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 def embedding_lookup(tokens, E, *, scale=1.0, padding_idx=None):
     """``scale * E[tokens]``: tokens ``[...]`` (int64 or int32) into the rows of ``E`` ``[V, D]``;
     returns ``[..., D]`` in E's dtype, the product rounded once, differentiable in ``E``.
@@ -140,6 +153,7 @@ def embedding_lookup(tokens, E, *, scale=1.0, padding_idx=None):
         if not -V <= padding < V:
             raise ValueError(f"padding_idx {padding_idx} is outside a table of {V} rows")
         padding += V if padding < 0 else 0
+    _refuse_forward_ad("embedding_lookup", E)
     flat = tokens if tokens.dim() == 1 else tokens.reshape(-1)
     out = (_Embed.apply if _eager(flat, E) else _embed_op)(flat, E, float(scale), padding)
     return out if tokens.dim() == 1 else out.view(*tokens.shape, E.shape[1])

@@ -89,3 +89,26 @@ def test_sampling_under_vmap(device, logprobs):
     for fn, arg in ((f, x), (g, h)):
         got, want = torch.func.vmap(fn)(arg, u, T), fn(arg, u, T)
         assert torch.equal(got[0], want[0]) and torch.allclose(got[1], want[1], atol=1e-5) if logprobs else torch.equal(got, want)
+
+
+@pytest.mark.parametrize("batched", [False, True])
+def test_forward_mode_is_refused_not_zero(device, batched):
+    """A tangent that the operator would drop raises; one that does not reach it does no harm."""
+    E, W, b, t, w = inputs(device, (11, 8), (11, 8), (11,), (5, 3), (5,))
+    tok = torch.randint(0, 11, (5,), generator=torch.Generator().manual_seed(1)).to(device)
+    ids = torch.randint(0, 11, (5, 3), generator=torch.Generator().manual_seed(2)).to(device)
+    h = E[:5].clone()
+    lookup = lambda E: swvr.embedding_lookup(tok, E)  # noqa: E731
+    loss = lambda h=h, W=W, b=b, w=w: swvr.softmax_distill(h, W, ids, t, b, weight=w)  # noqa: E731
+    for f, x in ((lookup, E), (loss, h), (lambda x: loss(W=x), W), (lambda x: loss(b=x), b), (lambda x: loss(w=x), w)):
+        g = torch.func.vmap(f) if batched else f
+        x = torch.stack([x, x]) if batched else x
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(g, (x,), (x,))
+        if not batched:
+            with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+                f(torch.autograd.forward_ad.make_dual(x, x))
+    beside = lambda x: x + lookup(E).sum() + loss().sum()  # noqa: E731
+    beside = torch.func.vmap(beside) if batched else beside
+    x = torch.ones(2, 3, device=device)
+    assert torch.equal(torch.func.jvp(beside, (x,), (x,))[1], x)
