@@ -8,8 +8,8 @@
 // GEMMs.  kHeadGrad stores the dense part p * sum q; the entries of teacher tokens, p * sum q - q, come
 // from the forward's fp32 scores and are written over it in one rounding (subtracting q from the
 // 16-bit p would lose the difference where the student has learnt the teacher).
-// The teacher's part of db is a sum over tokens in no fixed order: it is added in 64-bit fixed point, where
-// order does not matter.
+// The teacher's part of db is a sum over tokens in no fixed order: it is added in fixed point, where order does not matter, in
+// two 64-bit words a row: what a contribution has below the first word's unit goes to the second.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -212,7 +212,9 @@ __global__ void __launch_bounds__(32 * kWarps)
 // ------------------------------------------------------------------ backward
 // One block.  Per token: gT = g_n T (g_n: upstream, weight and denominator), coef = gT sum q, and the weight's
 // gradient.  Then the ranges, from the largest |gT| max(1, sum q), a:
-// f[0] what dS is multiplied by when stored, f[1] its undoing (dh, dW), f[2] the binary exponent of db's fixed point.
+// f[0] what dS is multiplied by when stored, f[1] its undoing (dh, dW), f[2] the binary exponent of the units of db's first
+// word, f[3] how much finer those of its second are.  Both words have 60 - log2 N bits, 92 in all at 8192 tokens: a row whose
+// contributions are 2^-60 of the largest still has them to fp32's accuracy.
 // fp16 dS is scaled by a power of two that puts its largest value near 2^13, so that small gradients (1 / N of a
 // mean) do not fall below fp16's range; bf16 has fp32's.  8192 tokens: 7.5 us; one block, so that the ranges need no second launch.
 constexpr int kGradThreads = 1024;
@@ -245,17 +247,18 @@ __global__ void __launch_bounds__(kGradThreads)
   if (threadIdx.x < 32) {
     a = warp_max(most[threadIdx.x]);
     if (threadIdx.x == 0) {
+      // a token adds less than 2^(bits + 1) to a word of a row, all of them less than 2^61
+      const int bits = 60 - (64 - __clzll(N));
       int e = 0, x = 0;
       if (a > 0.f) {
         const float as = a * fabsf(s);
         if (fp16 && as > 0.f && as < INFINITY) e = max(-100, min(100, 13 - ilogbf(as)));
-        // a token adds at most 2^41 to a row of db, all of them less than 2^62
-        const int lg = 64 - __clzll(N);
-        x = max(-100, min(140, min(40, 60 - lg) - ilogbf(a)));
+        x = max(-100, min(140, bits - ilogbf(a)));
       }
       f[0] = ldexpf(s, e);
       f[1] = ldexpf(1.f, -e);
       f[2] = static_cast<float>(x);
+      f[3] = static_cast<float>(bits);
     }
   }
 }
@@ -294,7 +297,12 @@ __global__ void __launch_bounds__(256)
     if constexpr (kBF16) static_cast<__nv_bfloat16*>(ds)[at] = __float2bfloat16_rn(o);
     else static_cast<__half*>(ds)[at] = __float2half_rn(o);
   }
-  if (db) atomicAdd(db + v, static_cast<unsigned long long>(__double2ll_rn(ldexp(-static_cast<double>(g) * q, static_cast<int>(f[2])))));
+  if (db) {
+    const double d = ldexp(-static_cast<double>(g) * q, static_cast<int>(f[2]));
+    const long long hi = __double2ll_rn(d), lo = __double2ll_rn(ldexp(d - static_cast<double>(hi), static_cast<int>(f[3])));
+    if (hi) atomicAdd(db + 2ll * v, static_cast<unsigned long long>(hi));
+    if (lo) atomicAdd(db + 2ll * v + 1, static_cast<unsigned long long>(lo));
+  }
 }
 
 // db[v] of a chunk: the token splits' partial sums in split order, and the teacher's part.
@@ -305,7 +313,8 @@ __global__ void db_kernel(int rows, int v0, int TS, const float* __restrict__ pa
   const float* p = part + static_cast<int64_t>(i / 256) * TS * 256 + i % 256;
   double s = 0;
   for (int t = 0; t < TS; ++t) s += static_cast<double>(p[t * 256]);
-  s += ldexp(static_cast<double>(static_cast<long long>(fix[v0 + i])), -static_cast<int>(f[2]));
+  const long long hi = static_cast<long long>(fix[2ll * (v0 + i)]), lo = static_cast<long long>(fix[2ll * (v0 + i) + 1]);
+  s += ldexp(static_cast<double>(hi) + ldexp(static_cast<double>(lo), -static_cast<int>(f[3])), -static_cast<int>(f[2]));
   store_d(gb, gb_dt, v0 + i, s);
 }
 
@@ -522,7 +531,7 @@ static GradPlan plan_grad(const swvr_distill& p, const swvr_distill_grads& g) {
     if (b.need_h && tiles > 0)
       b.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({b.pairs / tiles, kblocks / 4, 16})));
     b.off_fix = off;
-    if (b.need_b) off += align_up(p.vocab * 8, 256);
+    if (b.need_b) off += align_up(p.vocab * 16, 256);
     b.off_dh = off;
     if (b.need_h) off += align_up(static_cast<size_t>(b.slices > 1 ? b.slices * b.Npad : p.n_tokens) * p.hidden * 4, 256);
     b.clear = off - b.off_fix;

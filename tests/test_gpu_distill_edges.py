@@ -68,3 +68,25 @@ def test_same_bits_at_sizes_whose_sums_are_split(dtype, N, K, V):
         torch.randn(1 << 24, device="cuda").sum()
         loss, grads = run(h, W, b, ids, t)
         assert torch.equal(loss, first[0]) and all(torch.equal(a, c) for a, c in zip(grads[:3], first[1][:3]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", ["entries", "tokens"])
+def test_small_gradients_of_the_bias_keep_their_bits(dtype, case):
+    """Rows of the bias whose student and teacher probabilities are e^-30 and less, or which get entries only of
+    tokens with a small upstream gradient: to the same relative accuracy as the others."""
+    N, K, V = 40, 64, 500
+    h, W, b, ids, t = make(N, K, V, 24, dtype, spread=4.0)
+    b = b.detach().float().requires_grad_(True)
+    if case == "entries":
+        t = 8 * t
+        check(h, W, b, ids, t, T=0.5)
+        return
+    with torch.no_grad():  # each half of the vocabulary is what half of the tokens know
+        b[: V // 2] = 0
+        half = (torch.arange(N, device="cuda") % 2 == 0)
+        h[:, 0] = torch.where(half, 6.0, -6.0).to(dtype)
+        W[:, 0] = torch.where(torch.arange(V, device="cuda") < V // 2, 4.0, -4.0).to(dtype)
+    ids = ids % (V // 2) + torch.where(half, 0, V // 2)[:, None]
+    up = torch.where(half, 1.0, 2.0 ** -50).cuda()
+    check(h, W, b, ids, t, reduction="none", up=up)
