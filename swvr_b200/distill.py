@@ -210,7 +210,9 @@ def softmax_distill(h, W, teacher_ids, teacher_logits, bias=None, *, temperature
     dW).  An entry with a negative id or a logit of -inf is left out, and a token with none left has loss 0
     and no gradient.  An id at or past V makes its token's loss NaN and is reported by
     ``_native.check_device_error()``.  ``chunk_size`` is that of ``softmax_readout``; under autocast h and W are
-    cast whole.
+    cast whole, in the forward and again in the backward, as they are copied where the hidden size is no multiple of 8 in 16
+    bits.  W is the whole vocabulary, not a shard of it.  fp32 and fp64 take at most 65535 * 128 tokens.  There is no
+    forward-mode derivative.
     """
     if W.dim() != 2:
         raise ValueError(f"W must be 2-D, got {tuple(W.shape)}")

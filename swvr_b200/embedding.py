@@ -139,7 +139,8 @@ def embedding_lookup(tokens, E, *, scale=1.0, padding_idx=None):
     ``padding_idx`` (negative: from the end, as ``nn.Embedding``) names a row that takes no
     gradient.  Rows of ``E`` may be strided.  A token outside ``[0, V)`` is an error that the host
     learns of at ``_native.check_device_error()``: its row comes back as NaN and the gradient
-    leaves it out.  Autocast leaves the lookup in E's dtype, as torch's own.
+    leaves it out.  Autocast leaves the lookup in E's dtype, as torch's own.  E is the whole table, not a shard of it.  There is
+    no forward-mode derivative.
     """
     if E.dim() != 2:
         raise ValueError(f"E must be 2-D, got {tuple(E.shape)}")

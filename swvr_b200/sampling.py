@@ -158,9 +158,9 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     ``top_p`` times what ``top_k`` left, ``min_p`` the tokens with ``w >= min_p``; the token is the first in
     index order whose running weight over the kept ones exceeds ``u`` times their sum.  A
     temperature of 0 takes the largest score, the lowest index among equals.  Each setting is a number for
-    all rows or a tensor of u's shape; in a tensor a temperature <= 0 means the largest score, and values
-    outside the other settings' ranges turn them off (top_p <= 0 keeps one token).  Scores of -inf and
-    NaN are never chosen; a row with nothing else gives -1.  Rows may be strided.
+    all rows or a tensor of u's shape; in a tensor a temperature <= 0 or NaN means the largest score, and values
+    outside the other settings' ranges turn them off, except that top_p <= 0 keeps one token and min_p > 1 counts as 1.
+    Scores of -inf and NaN are never chosen; a row with nothing else gives -1.  Rows may be strided.
 
     ``return_logprobs=True`` also returns ``log softmax(x / temperature)`` of each token over its whole row,
     in fp32.  There is no gradient.
@@ -187,7 +187,9 @@ def softmax_sample(h, W, u, bias=None, *, temperature=1.0, top_k=None, top_p=Non
 
     The products run in the readout's compute dtype (bf16, fp16 or fp32; the autocast dtype under
     autocast) with fp32 accumulation; the scores are never rounded.  At most 256 MiB of them are
-    held at a time.
+    held at a time.  h and W are taken in that dtype: under autocast over parameters of another one, or
+    with a hidden size that is no multiple of 8 in 16 bits, all of W is copied at every call, so a server keeps W as it is
+    used.  W is the whole vocabulary, not a shard of it.
     """
     if W.dim() != 2:
         raise ValueError(f"W must be 2-D, got {tuple(W.shape)}")
