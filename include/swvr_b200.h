@@ -12,7 +12,8 @@
  *   - `stream` is a cudaStream_t (may be NULL for the legacy default stream).  All work is
  *     enqueued on it; nothing here synchronises the stream or the device.
  *   - The library never allocates or frees device memory: callers pass every output and a
- *     workspace of at least the size the matching *_workspace_size() call returns.
+ *     workspace of at least the size the matching *_workspace_size() call returns, 16-byte
+ *     aligned (the operators on tokens refuse another).
  *   - Return value: SWVR_OK (0) or a negative SWVR_ERR_* code; swvr_last_error() then holds
  *     a message (per host thread).  Errors raised by a bounded device-side wait surface on
  *     the host through swvr_device_error().

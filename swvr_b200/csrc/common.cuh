@@ -27,6 +27,8 @@ enum : uint32_t {
   kErrSelftest = 0x7F00,  // swvr_selftest_wait_timeout
 };
 
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 inline size_t dtype_size(int dt) {
   switch (dt) {
     case SWVR_F32: return 4;

@@ -838,6 +838,7 @@ int swvr_distill_fwd(const swvr_distill* p, void* out, void* workspace, size_t w
   SWVR_TRY(distill::check(p));
   if (!out && (p->n_tokens > 0 || p->reduction != SWVR_REDUCE_NONE)) return fail(SWVR_ERR_INVALID_ARGUMENT, "NULL output");
   if (!workspace && p->n_tokens > 0) return fail(SWVR_ERR_INVALID_ARGUMENT, "NULL workspace");
+  if (!aligned16(workspace)) return fail(SWVR_ERR_UNSUPPORTED, "workspace not 16-byte aligned");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (is_tc(p->compute_dtype)) return distill::tc_fwd_distill(*p, out, workspace, workspace_bytes, st);
   if (p->compute_dtype == SWVR_F64) return distill::exact_fwd<double>(*p, out, workspace, workspace_bytes, st);
@@ -878,6 +879,7 @@ int swvr_distill_bwd(const swvr_distill* p, const swvr_distill_grads* g, void* w
   const size_t need = distill::bwd_bytes(*p, b);
   if (workspace_bytes < need) return fail(SWVR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, need);
   if (!workspace) return fail(SWVR_ERR_INVALID_ARGUMENT, "NULL workspace");
+  if (!aligned16(workspace)) return fail(SWVR_ERR_UNSUPPORTED, "workspace not 16-byte aligned");
   char* w = static_cast<char*>(workspace);
   if (is_tc(p->compute_dtype)) return distill::tc_bwd_distill(*p, *g, b, w, st);
   if (p->compute_dtype == SWVR_F64) return distill::exact_bwd<double>(*p, *g, b, w, st);

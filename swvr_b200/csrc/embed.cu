@@ -669,6 +669,7 @@ int swvr_embed_bwd(int64_t n_tokens, int64_t vocab, int64_t dim, const void* tok
   if (vocab == 0 || dim == 0) return SWVR_OK;
   if (!grad_E || (n_tokens > 0 && (!tokens || !grad_out || !workspace)))
     return fail(SWVR_ERR_INVALID_ARGUMENT, "NULL pointer");
+  if (!aligned16(workspace)) return fail(SWVR_ERR_UNSUPPORTED, "workspace not 16-byte aligned");
   const embed::BwdPlan b = embed::plan_bwd(n_tokens, vocab, dim, dtype);
   if (n_tokens > 0 && workspace_bytes < b.bytes)
     return fail(SWVR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, b.bytes);

@@ -1292,6 +1292,7 @@ int swvr_sample(const swvr_problem* p, const swvr_sampling* sampling, void* work
   SWVR_TRY(swvr_sample_workspace_size(p, &need));
   if (workspace_bytes < need) return fail(SWVR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, need);
   if (!workspace) return fail(SWVR_ERR_INVALID_ARGUMENT, "NULL workspace");
+  if (!aligned16(workspace)) return fail(SWVR_ERR_UNSUPPORTED, "workspace not 16-byte aligned");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t rows = sample::head_rows(*p), ld = round_up(std::max<int64_t>(p->vocab, 1), 4);
   q.x = workspace;

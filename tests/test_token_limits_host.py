@@ -63,3 +63,23 @@ def test_exact_forward_asks_for_no_split_sums():
     assert both + 4 * 17 * N * K <= bwd(h=1 << 20) <= both + 4 * 17 * N * K + slack  # dh and 16 slices of it
     assert both + 4 * 16 * 8192 * K <= bwd(W=1 << 20) <= both + 4 * 16 * 8192 * K + slack
     assert both + 4 * (16 * 8192 + N) * K <= bwd(h=1 << 20, W=1 << 20) <= both + 4 * (16 * 8192 + N) * K + slack
+
+
+def test_workspaces_have_to_be_aligned():
+    """The kernels read and write them 16 bytes at a time: one that starts elsewhere is refused before any launch."""
+    lib, buf, n = nat.lib(), 1 << 20, ctypes.c_size_t(0)
+    for off in (1, 4, 8):
+        assert lib.swvr_embed_bwd(4, 9, 8, buf, 64, buf, 8, 1.0, -1, buf, nat.BF16, 8, buf + off, 1 << 30, None) == nat.ERR_UNSUPPORTED
+        for dt in (nat.BF16, nat.F32, nat.F64):
+            p, g = _problem(dt=dt), nat.DistillGrads()
+            g.grad_out = g.grad_bias = p.bias = buf
+            assert lib.swvr_distill_fwd(p, buf, buf + off, 1 << 40, None) == nat.ERR_UNSUPPORTED
+            assert lib.swvr_distill_bwd(p, g, buf + off, 1 << 40, None) == nat.ERR_UNSUPPORTED
+        p, s = nat.Problem(), nat.Sampling()
+        p.n_tokens, p.hidden, p.vocab, p.compute_dtype, p.bias_dtype = 4, 64, 1000, nat.BF16, nat.F32
+        p.h = p.W = buf
+        p.ldh = p.ldw = 64
+        p.logit_scale = s.temperature = s.top_p = 1.0
+        s.u, s.u_dtype, s.tokens = buf, nat.F32, buf
+        assert lib.swvr_sample(p, s, buf + off, 1 << 30, None) == nat.ERR_UNSUPPORTED
+    assert "aligned" in nat.last_error()
