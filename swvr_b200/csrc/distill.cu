@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(32 * kWarps)
 // One block.  Per token: gT = g_n T (g_n: upstream, weight and denominator), coef = gT sum q, and the weight's
 // gradient.  Then the ranges, from the largest |gT| max(1, sum q), a:
 // f[0] what dS is multiplied by when stored, f[1] its undoing (dh, dW), f[2] the binary exponent of the units of db's first
-// word, f[3] how much finer those of its second are.  Both words have 60 - log2 N bits, 92 in all at 8192 tokens: a row whose
+// word, f[3] how much finer those of its second are.  Both words have 59 - log2 N bits, 92 in all at 8192 tokens: a row whose
 // contributions are 2^-60 of the largest still has them to fp32's accuracy.
 // fp16 dS is scaled by a power of two that puts its largest value near 2^13, so that small gradients (1 / N of a
 // mean) do not fall below fp16's range; bf16 has fp32's.  8192 tokens: 7.5 us; one block, so that the ranges need no second launch.
